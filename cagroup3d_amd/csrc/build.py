@@ -27,7 +27,10 @@ SOURCES = {
     "program.hip": [],                       # cg3d_run_program: the launch-table executor (include/cagroup3d_program.h)
     "optim.hip": ["-ffp-contract=off"],      # same rounding as the oracle's plain C (and torch's kernel: no contraction across statements)
 }
-COMMON = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"] + os.environ.get("CG3D_HIPCC_EXTRA", "").split()
+# packed fp32 instructions (two floats of a register pair at once) are kept out of every file: some of their forms have given wrong
+# results on this hardware now and then, and the compiler makes them from ordinary float code by itself
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+COMMON = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"] + NO_PACKED_FP32 + os.environ.get("CG3D_HIPCC_EXTRA", "").split()
 # (CG3D_HIPCC_EXTRA: dev builds on the GPU box, e.g. -DCG3D_TILE_TRACE; the shipped library is built without it)
 
 
