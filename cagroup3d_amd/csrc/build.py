@@ -18,6 +18,8 @@ SOURCES = {
     "spconv_tile2.hip": ["-munsafe-fp-atomics"],
     "linear.hip": ["-munsafe-fp-atomics"],
     "gather_scatter.hip": ["-munsafe-fp-atomics"],
+    "expert_rows.hip": [],
+    "int8_linear.hip": [],
     "iou3d_nms.hip": ["-ffp-contract=off"],
     "stages.hip": ["-ffp-contract=off", "-munsafe-fp-atomics"],     # stage-level fused ops of the heads (RoI matching / targets / grid, class rows, proposals)
     "knn.hip": ["-ffp-contract=off"],

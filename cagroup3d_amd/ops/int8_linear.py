@@ -1,0 +1,140 @@
+"""Products in 8-bit integers with a scale for each row and each output channel (csrc/int8_linear.hip), dense or with a matrix of
+its own for each expert's rows: the served form of the kernel-size-1 convolutions, the RoI contraction and the per-class products.
+
+    weight = int8_weight(conv.kernel)                       # once: [cin, cout] (or [E, cin, cout]), quantised per output channel
+    y = int8_linear(x, weight, bias)                        # rows in floats are quantised per row in the call
+    q, scale = quantize_rows(x)                             # or once for several products:
+    y = int8_linear(q, weight, bias, scale=scale, out_dtype=torch.bfloat16)
+    y = int8_linear(x, weight, plan=plan, gather=True)      # each expert's tokens with its matrix (ops/expert_rows.expert_plan)
+
+The integer sums are exact, so results do not depend on how the work is split.  There is no gradient: a call on inputs that require
+one, with gradients enabled, is refused."""
+from ctypes import c_int32, c_int64
+
+import torch
+
+from .. import _lib
+from .._lib import ptr
+from .expert_rows import DTYPES, FLOATS, ExpertPlan, need, on_device
+
+MAX_CIN = 131071                  # the int32 sum of so many products of 8-bit values cannot overflow
+
+
+def _no_grad_for(who, *tensors):
+    need(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)),
+         "%s has no gradient: call it under torch.no_grad() or on detached tensors", who)
+
+
+class Int8Weight:
+    """Weights in the product kernels' order.  packed int8 (cg3d_int8_weight_bytes), scale float32 [E, cout]."""
+
+    __slots__ = ("packed", "scale", "n_experts", "cin", "cout", "grouped")
+
+    def __init__(self, packed, scale, n_experts, cin, cout, grouped):
+        self.packed, self.scale, self.n_experts, self.cin, self.cout, self.grouped = packed, scale, n_experts, cin, cout, grouped
+
+    @property
+    def device(self):
+        return self.packed.device
+
+
+def int8_weight(w, scale=None):
+    """w [cin, cout] or [E, cin, cout] (the layout of the framework's kernels).  Floats: every output channel is quantised to
+    scale * (-127 .. 127), scale = max |w| / 127.  int8: `scale` float32 [cout] ([E, cout]) must be given and w is taken as it is."""
+    need(isinstance(w, torch.Tensor) and w.dtype in DTYPES and w.dim() in (2, 3),
+         "int8_weight: w must be float32, bfloat16, float16 or int8, [cin, cout] or [experts, cin, cout]")
+    grouped = w.dim() == 3
+    e, cin, cout = w.shape if grouped else (1,) + tuple(w.shape)
+    need(1 <= e <= 1024 and 1 <= cin <= MAX_CIN and 1 <= cout <= 1 << 20,
+         "int8_weight: w of shape %s (experts in 1 .. 1024, cin in 1 .. %d, cout in 1 .. 2^20)", tuple(w.shape), MAX_CIN)
+    if w.dtype == torch.int8:
+        need(isinstance(scale, torch.Tensor) and scale.dtype == torch.float32 and tuple(scale.shape) == ((e, cout) if grouped else (cout,))
+             and scale.device == w.device, "int8_weight: weights in 8 bits need their scale, float32 %s, beside them",
+             [e, cout] if grouped else [cout])
+    else:
+        need(scale is None, "int8_weight: the scale of weights in floats is computed here")
+    lib = _lib.get()
+    w = w.detach().contiguous()
+    lib.check(w)
+    with on_device(w):
+        packed = torch.empty(int(lib.raw("cg3d_int8_weight_bytes")(e, cin, cout)), dtype=torch.int8, device=w.device)
+        if scale is None:
+            out, ws = torch.empty((2, e, cout), dtype=torch.float32, device=w.device)
+        else:
+            out, ws = scale.detach().clone().view(e, cout), None          # (the handle's own: the caller may reuse the memory)
+        lib.call("cg3d_int8_weight", ptr(w), c_int32(DTYPES[w.dtype]), c_int32(e), c_int32(cin), c_int32(cout), ptr(packed),
+                 ptr(out) if ws is not None else None, ptr(ws), lib.stream())
+    return Int8Weight(packed, out, e, cin, cout, grouped)
+
+
+def _rows_in(who, x, dtypes):
+    need(isinstance(x, torch.Tensor) and x.dtype in dtypes and x.dim() == 2, "%s: x must be [rows, cin] of %s", who,
+         " / ".join(str(d).replace("torch.", "") for d in dtypes))
+    need(1 <= x.shape[1] <= MAX_CIN and x.shape[0] < 2 ** 31, "%s: x of shape %s (cin in 1 .. %d)", who, tuple(x.shape), MAX_CIN)
+
+
+def quantize_rows(x):
+    """x [rows, cin] float32 / bfloat16 / float16 -> (q int8 [rows, cin], scale float32 [rows]): scale = max |x| / 127 of each row,
+    q = the nearest level, ties to the even one.  A row of zeros has the scale 0, one with an infinity or a NaN the scale NaN."""
+    _rows_in("quantize_rows", x, FLOATS)
+    _no_grad_for("quantize_rows", x)
+    lib = _lib.get()
+    x = x.detach().contiguous()
+    lib.check(x)
+    n, cin = x.shape
+    with on_device(x):
+        q = torch.empty((n, cin), dtype=torch.int8, device=x.device)
+        scale = torch.empty(n, dtype=torch.float32, device=x.device)
+        lib.call("cg3d_int8_quantize_rows", ptr(x), c_int32(DTYPES[x.dtype]), c_int64(n), c_int32(cin), c_int64(cin), ptr(q), ptr(scale),
+                 lib.stream())
+    return q, scale
+
+
+def int8_linear(x, weight, bias=None, scale=None, out_dtype=None, plan=None, gather=False):
+    """x [rows, cin] float32 / bfloat16 / float16 (quantised here) or int8 with `scale` float32 [rows] -> [rows, cout] of out_dtype
+    (default: x's own, float32 for int8) = x @ weight (+ bias [cout], or [E, cout] with a plan).
+
+    plan (ops/expert_rows.expert_plan): weight holds plan.n_experts matrices and each row is multiplied by its expert's; x has the
+    plan's rows ([T * k, cin], what expert_gather gives), or with gather=True the tokens ([T, cin]), whose rows are picked in the
+    product -- quantised once for a token, not once for a row.  Rows behind the last are zeros."""
+    need(isinstance(weight, Int8Weight), "int8_linear: weight must come from int8_weight")
+    _rows_in("int8_linear", x, tuple(DTYPES))
+    need(x.shape[1] == weight.cin, "int8_linear: x has %d columns, weight %d rows", x.shape[1], weight.cin)
+    out_dtype = out_dtype or (torch.float32 if x.dtype == torch.int8 else x.dtype)
+    need(out_dtype in FLOATS, "int8_linear: out_dtype must be float32, bfloat16 or float16")
+    if x.dtype == torch.int8:
+        need(isinstance(scale, torch.Tensor) and scale.dtype == torch.float32 and tuple(scale.shape) == (x.shape[0],),
+             "int8_linear: rows in 8 bits need their scale, float32 [%d]", x.shape[0])
+    else:
+        need(scale is None, "int8_linear: the scale of rows in floats is computed here")
+    if plan is None:
+        need(weight.n_experts == 1 and not gather, "int8_linear: %d matrices (or gather) need a plan", weight.n_experts)
+        n_rows = x.shape[0]
+    else:
+        need(isinstance(plan, ExpertPlan), "int8_linear: plan must come from expert_plan")
+        need(weight.n_experts == plan.n_experts, "int8_linear: %d matrices for a plan of %d experts", weight.n_experts, plan.n_experts)
+        n_rows = plan.n_rows
+        n_x = plan.n_tokens if gather else n_rows
+        need(x.shape[0] == n_x, "int8_linear: x has %d rows, the plan %d", x.shape[0], n_x)
+    per_expert = bias is not None and bias.dim() == 2
+    if bias is not None:
+        need(bias.dtype in FLOATS and tuple(bias.shape) in ((weight.cout,), (weight.n_experts, weight.cout) if weight.grouped else ()),
+             "int8_linear: bias must be floats [%d]%s, got %s", weight.cout,
+             " or [%d, %d]" % (weight.n_experts, weight.cout) if weight.grouped else "", tuple(bias.shape))
+    _no_grad_for("int8_linear", x, bias, scale)
+    for t in (weight.packed, bias, scale, plan and plan.offsets):
+        need(t is None or t.device == x.device, "int8_linear: x is on %s, another argument on %s", x.device, t is not None and t.device)
+    lib = _lib.get()
+    x = x.detach().contiguous()
+    bias = None if bias is None else bias.detach().to(torch.float32).contiguous()
+    scale = None if scale is None else scale.detach().contiguous()
+    lib.check(x, bias, scale)
+    with on_device(x):
+        y = torch.empty((n_rows, weight.cout), dtype=out_dtype, device=x.device)
+        ws_bytes = int(lib.raw("cg3d_int8_linear_ws_bytes")(DTYPES[x.dtype], x.shape[0], weight.cin, n_rows, weight.cout, weight.n_experts))
+        ws = torch.empty(ws_bytes, dtype=torch.int8, device=x.device) if ws_bytes > 0 else None
+        lib.call("cg3d_int8_linear", ptr(x), c_int32(DTYPES[x.dtype]), ptr(scale), c_int64(x.shape[0]), c_int32(weight.cin), ptr(weight.packed),
+                 ptr(weight.scale), ptr(bias), c_int32(per_expert), ptr(plan.offsets) if plan else None,
+                 ptr(plan.rows) if plan and gather else None, ptr(y), c_int32(DTYPES[out_dtype]), c_int64(n_rows), c_int32(weight.cout),
+                 c_int32(weight.n_experts), ptr(ws), lib.stream())
+    return y

@@ -577,6 +577,59 @@ int cg3d_adamw_step(const int64_t *table, const int32_t *pid, int64_t nrows, con
                     float lr, float beta1, float beta2, float eps, float weight_decay, float bias_correction1,
                     float bias_correction2, cg3d_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Rows sorted by expert and back: the routing of rows to groups with matrices of their own (the general form of what the
+ * class-aware head does with its voxels), with weights and gradients.
+ *   experts  [n_tokens, k] ids, int32 (wide = 0) or int64 (wide = 1); an id outside [0, n_experts) has no row.
+ *   plan: P = n_tokens * k pairs p = t * k + s sorted by id, pairs of one id in ascending order:
+ *     offsets int32 [n_experts + 1]  rows of expert e are [offsets[e], offsets[e + 1])
+ *     rows    int32 [P]              the token of each row; -1 behind offsets[n_experts]
+ *     pos     int32 [P]              the row of each pair; negative: none (~pos is one of the rows behind the last, which the
+ *                                    passes that write rows clear)
+ *   1 <= n_experts <= 1024, k >= 1, P < 2^31; ws: cg3d_expert_plan_ws_bytes bytes (may be NULL where that is 0).
+ * Element types `dtype` of rows, `wtype` of weights: CG3D_DT_F32 / _BF16 / _F16.  Rows are contiguous [*, c] of any width.
+ *   gather:       out[pos] = x[t]              (out [P, c]; rows without a pair are zeros)
+ *   combine:      out[t] = sum_s w[t, s] * y[pos[t, s]]   (w NULL: all ones -- also the gather's gradient); fp32 sums in slot
+ *                 order, rounded once; a token without rows gives zeros
+ *   combine_bwd:  dy[pos] = w[t, s] * dout[t] (rows without a pair: zeros), dw[t, s] = <dout[t], y[pos]> (0 without a row);
+ *                 dy or dw may be NULL (not both); y may be NULL without dw */
+#define CG3D_DT_F32 0
+#define CG3D_DT_BF16 1
+#define CG3D_DT_F16 2
+#define CG3D_DT_I8 3
+int64_t cg3d_expert_plan_ws_bytes(int64_t n_tokens, int32_t k, int32_t n_experts);
+int cg3d_expert_plan(const void *experts, int32_t wide, int64_t n_tokens, int32_t k, int32_t n_experts, int32_t *offsets, int32_t *rows,
+                     int32_t *pos, void *ws, cg3d_stream_t stream);
+int cg3d_expert_gather(const void *x, int32_t dtype, const int32_t *pos, int64_t n_tokens, int32_t k, int32_t c, void *out,
+                       cg3d_stream_t stream);
+int cg3d_expert_combine(const void *y, int32_t dtype, const int32_t *pos, const void *w, int32_t wtype, int64_t n_tokens, int32_t k,
+                        int32_t c, void *out, cg3d_stream_t stream);
+int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, const int32_t *pos, const void *w, int32_t wtype,
+                            int64_t n_tokens, int32_t k, int32_t c, void *dy, void *dw, cg3d_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Products in 8-bit integers with a scale for each row and each output channel, dense or grouped by expert (inference).
+ *   y[r, n] = (sum_k q[r, k] * w[k, n]) * sx[r] * sw[n] + bias[n]; the sum is exact (int32, cin <= 131071).
+ *   quantize_rows: scale[r] = max_k |x[r, k]| / 127, q = 127 x / max rounded to the nearest level, ties to even, decided exactly;
+ *     a row with an infinity or NaN: scale NaN, q 0; q [n][pitch], bytes [cin, pitch) zeros.
+ *   weight: w [n_experts][cin][cout] -> packed (cg3d_int8_weight_bytes bytes, 16-byte aligned; the kernels' own order).  Floats:
+ *     quantised by the same rule for each (expert, channel), scale [n_experts][cout] is written, ws = 4 * n_experts * cout bytes;
+ *     CG3D_DT_I8: packed as they are, scale and ws are not used (the caller holds the scales).
+ *   linear: x [n_x][cin] of `dtype`; CG3D_DT_I8: sx [n_x] given; floats: quantised in the call (sx NULL or ignored), ws =
+ *     cg3d_int8_linear_ws_bytes bytes, 16-byte aligned.  bias: NULL, [cout], or [n_experts][cout] (bias_per_expert = 1).
+ *     Dense: offsets = rows = NULL, n_experts = 1, n_x = n_rows.  Grouped: offsets [n_experts + 1] of cg3d_expert_plan; row r of y
+ *     is the product of row rows[r] of x (rows NULL: row r, n_x = n_rows) with its expert's matrix; rows at and behind
+ *     offsets[n_experts] are zeros.  y [n_rows][cout] of out_dtype. */
+int64_t cg3d_int8_weight_bytes(int32_t n_experts, int32_t cin, int32_t cout);
+int cg3d_int8_weight(const void *w, int32_t dtype, int32_t n_experts, int32_t cin, int32_t cout, int8_t *packed, float *scale, void *ws,
+                     cg3d_stream_t stream);
+int cg3d_int8_quantize_rows(const void *x, int32_t dtype, int64_t n, int32_t cin, int64_t pitch, int8_t *q, float *scale,
+                            cg3d_stream_t stream);
+int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts);
+int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, int64_t n_x, int32_t cin, const int8_t *w, const float *sw,
+                     const float *bias, int32_t bias_per_expert, const int32_t *offsets, const int32_t *rows, void *y, int32_t out_dtype,
+                     int64_t n_rows, int32_t cout, int32_t n_experts, void *ws, cg3d_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,435 @@
+"""Products in 8-bit integers (ops/int8_linear.py, csrc/int8_linear.hip).
+
+CPU (-m "not gpu"): the oracle's restatement against a plain implementation in 64 bits, the refusals.  -m gpu: the HIP kernels
+against the same -- every type in and out, sizes around the tiles, long contractions, single rows, experts without rows, dropped
+pairs, gathered rows -- the levels at exact ties and at the ends of the types' ranges, a captured graph, another stream, a layer of
+experts as it is served."""
+import pytest
+import torch
+
+from cagroup3d_amd import _lib
+from cagroup3d_amd.ops.expert_rows import expert_combine, expert_gather, expert_plan
+from cagroup3d_amd.ops.int8_linear import MAX_CIN, int8_linear, int8_weight, quantize_rows
+
+F32, BF16, F16, I8 = torch.float32, torch.bfloat16, torch.float16, torch.int8
+HALF = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}       # half a step, relative to the value
+TINY = {F32: 2.0 ** -126, BF16: 2.0 ** -126, F16: 2.0 ** -25}    # below the normal range a step is this and not relative
+
+
+def plain_levels(x):
+    """(q, scale in 64 bits) of each row: products and quotient in 64 bits place every value on its own side of a border."""
+    v = x.double()
+    top = v.abs().amax(1, keepdim=True)
+    q = torch.round(v * 127 / torch.where(top > 0, top, torch.ones_like(top)))
+    return q, (top / 127).squeeze(1)
+
+
+def check_levels(x, q, scale):
+    want_q, want_s = plain_levels(x.cpu())
+    assert q.dtype == I8 and scale.dtype == F32
+    assert torch.equal(q.cpu().double(), want_q)
+    assert bool(((scale.cpu().double() - want_s).abs() <= 2.0 ** -24 * want_s + 2.0 ** -150).all())
+
+
+def make(n, cin, cout, dtype, seed, experts=None):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn((experts, cin, cout) if experts else (cin, cout), generator=g) / cin ** 0.5
+    if dtype == I8:
+        x, sx = torch.randint(-128, 128, (n, cin), generator=g).to(I8), torch.rand(n, generator=g) + 0.1
+    else:
+        x, sx = (torch.randn(n, cin, generator=g) * torch.exp(torch.randn(n, 1, generator=g))).to(dtype), None
+        x[torch.rand(n, generator=g) < 0.1] = 0
+    return x, sx, w, torch.randn((experts, cout) if experts else (cout,), generator=g)
+
+
+def reference(x, sx, wq, sw, bias, expert, token):
+    """64 bits: rows token[r] of x times the matrix of expert[r] -> (result, sum of the absolute values of its two terms)."""
+    q, s = (x.cpu().double(), sx.cpu().double()) if x.dtype == I8 else plain_levels(x.cpu())
+    wq, sw = wq.cpu().double(), sw.cpu().double()
+    y = torch.zeros(len(expert), wq.shape[2], dtype=torch.float64)
+    for e in expert.unique().tolist():
+        if e >= 0:
+            m = expert == e
+            y[m] = q[token[m]] @ wq[e] * s[token[m]].unsqueeze(1) * sw[e]
+    size = y.abs()
+    if bias is not None:
+        b = bias.cpu().double()
+        b = torch.where((expert >= 0).unsqueeze(1), b[expert.clamp(min=0)] if b.dim() == 2 else b, 0.0)
+        y, size = y + b, size + b.abs()
+    return y, size
+
+
+def close(got, want, size, out):
+    """fp32: the sum converted, two products with scales that are themselves rounded once, one addition -- 6 half-steps of the
+    terms' sizes -- and one rounding to the output's type."""
+    assert got.dtype == out and bool(torch.isfinite(got).all())
+    tol = (6 * 2.0 ** -24 * size) * (1 + HALF[out]) + HALF[out] * want.abs() * (1 + 2.0 ** -7) + TINY[out]
+    off = (got.cpu().double() - want).abs()
+    assert bool((off <= tol).all()), float((off - tol).max())
+
+
+def dense(n, cin, cout, dtype, out, bias, seed, dev, offset=0):
+    x, sx, w, b = make(n, cin, cout, dtype, seed)
+    wq, sw = plain_levels(w.t().contiguous())                     # a channel of w is a row here
+    weight = int8_weight(w.to(dev))
+    assert bool(((weight.scale.cpu().double().view(-1) - sw).abs() <= 2.0 ** -24 * sw).all())
+    if offset:                                                    # x behind an odd number of elements of its storage
+        x = torch.cat([torch.zeros(offset, dtype=x.dtype), x.reshape(-1)]).to(dev)[offset:].view(n, cin)
+    y = int8_linear(x.to(dev), weight, b.to(dev) if bias else None, scale=None if sx is None else sx.to(dev), out_dtype=out)
+    want, size = reference(x, sx, wq.t().unsqueeze(0), sw.unsqueeze(0), b if bias else None, torch.zeros(n, dtype=torch.long), torch.arange(n))
+    assert y.shape == (n, cout)
+    close(y, want, size, out)
+    return y
+
+
+def grouped(ids, experts, cin, cout, dtype, out, bias, gather, seed, dev):
+    t, k = ids.shape
+    x, sx, w, b = make(t if gather else t * k, cin, cout, dtype, seed, experts)
+    if bias == 1:
+        b = b[0]
+    wq, sw = plain_levels(w.transpose(1, 2).reshape(-1, cin))
+    wq, sw = wq.view(experts, cout, cin).transpose(1, 2), sw.view(experts, cout)
+    plan = expert_plan(ids.to(dev), experts)
+    rows, off = plan.rows.cpu().long(), plan.offsets.cpu().long()
+    expert = torch.bucketize(torch.arange(t * k), off[1:], right=True)
+    expert[expert == experts] = -1
+    y = int8_linear(x.to(dev), int8_weight(w.to(dev)), b.to(dev) if bias else None, scale=None if sx is None else sx.to(dev), out_dtype=out,
+                    plan=plan, gather=gather)
+    want, size = reference(x, sx, wq, sw, b if bias else None, expert, rows.clamp(min=0) if gather else torch.arange(t * k))
+    close(y, want, size, out)
+    assert bool((y[int(off[-1]):] == 0).all())
+    return y
+
+
+def ids_of(t, k, experts, kind, seed):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, experts, (t, k), generator=g)
+    if kind == "dropped":
+        ids[torch.rand(t, k, generator=g) < 0.4] = -1
+    elif kind == "one":
+        ids[:] = experts // 2
+    elif kind == "none":
+        ids[:] = -1
+    return ids
+
+
+ODD = [(1, 1, 1), (1, 64, 64), (2, 16, 8), (15, 63, 65), (17, 65, 63), (33, 100, 7), (16, 128, 128), (70, 200, 77), (129, 257, 130)]
+
+
+@pytest.mark.parametrize("n,cin,cout", ODD)
+@pytest.mark.parametrize("dtype,out,bias", [(F32, F32, True), (BF16, BF16, False), (F16, F16, True), (I8, F32, False), (I8, BF16, True)])
+def test_oracle_is_the_definition(oracle, n, cin, cout, dtype, out, bias):
+    with _lib.use_library(oracle):
+        dense(n, cin, cout, dtype, out, bias, 1, "cpu")
+
+
+@pytest.mark.parametrize("kind", ["uniform", "dropped", "one", "none"])
+@pytest.mark.parametrize("gather", [False, True])
+def test_oracle_grouped(oracle, kind, gather):
+    with _lib.use_library(oracle):
+        grouped(ids_of(20, 2, 5, kind, 2), 5, 33, 18, F32, F32, 2, gather, 3, "cpu")
+        grouped(ids_of(20, 2, 5, kind, 2), 5, 33, 18, I8, F16, 1, gather, 3, "cpu")
+
+
+def levels_cases():
+    """Rows whose elements sit on and beside the borders between levels, at the ends of the type's range too."""
+    m = torch.arange(-127, 127).double()
+    ties = (2 * m + 1) / 254                                     # times the largest magnitude: half-way between two levels
+    rows = []
+    for top in (1.0, 254.0, 127.0, 3.0, 2.0 ** -20, 254 * 2.0 ** -149, 127 * 2.0 ** -140, 2.0 ** -126, 3.3e38, 1.7e-37):
+        r = torch.cat([torch.tensor([top]).double(), ties * top]).float()
+        rows += [r, torch.nextafter(r, torch.zeros(())), torch.cat([r[:1], torch.nextafter(r[1:], 2 * r[1:])])]
+    rows.append(torch.zeros(255))
+    rows.append(torch.cat([torch.tensor([2.0 ** -149]), torch.zeros(254)]))
+    return torch.stack(rows)
+
+
+def levels(dev):
+    x = levels_cases().to(dev)
+    check_levels(x, *quantize_rows(x))
+    g = torch.Generator().manual_seed(4)
+    for dtype in (BF16, F16):                                    # short significands: exact ties everywhere
+        v = torch.randint(-254, 255, (300, 61), generator=g).to(dtype).to(dev)
+        check_levels(v, *quantize_rows(v))
+        v = (torch.randn(300, 130, generator=g) * 1e-6).to(dtype).to(dev)
+        check_levels(v, *quantize_rows(v))
+
+
+def nonfinite(dev):
+    x = torch.randn(6, 40, generator=torch.Generator().manual_seed(5)).to(dev)
+    x[1, 7], x[2, 39], x[3, 0], x[4] = float("inf"), float("nan"), float("-inf"), 0.0
+    q, s = quantize_rows(x)
+    bad = torch.tensor([False, True, True, True, False, False]).to(dev)
+    assert torch.equal(torch.isnan(s), bad) and bool((q[bad] == 0).all()) and float(s[4]) == 0.0
+    w = int8_weight(torch.randn(40, 9, generator=torch.Generator().manual_seed(6)).to(dev))
+    b = torch.ones(9, device=dev)
+    for dt in (F32, BF16):
+        y = int8_linear(x.to(dt), w, b)
+        assert bool(torch.isnan(y[bad]).all()) and bool(torch.isfinite(y[~bad]).all()) and bool((y[4] == 1).all())
+
+
+def test_oracle_levels_and_nonfinite(oracle):
+    with _lib.use_library(oracle):
+        levels("cpu")
+        nonfinite("cpu")
+
+
+def test_oracle_weights_in_8_bits(oracle):
+    with _lib.use_library(oracle):
+        eight_bit_weights("cpu")
+
+
+def eight_bit_weights(dev):
+    g = torch.Generator().manual_seed(7)
+    wq, sw = torch.randint(-128, 128, (3, 70, 20), generator=g).to(I8), torch.rand(3, 20, generator=g)
+    x = torch.randint(-128, 128, (12, 70), generator=g).to(I8)
+    sx = torch.rand(12, generator=g)
+    plan = expert_plan(torch.arange(12).view(6, 2).remainder(3).to(dev), 3)
+    handle_scale = sw.clone().to(dev)
+    handle = int8_weight(wq.to(dev), handle_scale)
+    handle_scale.zero_()                                          # the handle keeps its own
+    y = int8_linear(x.to(dev), handle, scale=sx.to(dev), plan=plan)
+    expert = torch.bucketize(torch.arange(12), plan.offsets.cpu().long()[1:], right=True)
+    want, size = reference(x, sx, wq, sw, None, expert, torch.arange(12))
+    close(y, want, size, F32)
+    assert torch.equal(int8_linear(x.to(dev), int8_weight(wq[0].to(dev), sw[0].to(dev)), scale=sx.to(dev))[:1],
+                       int8_linear(x[:1].to(dev), int8_weight(wq[0].to(dev), sw[0].to(dev)), scale=sx[:1].to(dev)))
+
+
+def refusals(dev):
+    x, w = torch.zeros(4, 8, device=dev), int8_weight(torch.ones(8, 6, device=dev))
+    w3 = int8_weight(torch.ones(3, 8, 6, device=dev))
+    q, s = torch.zeros(4, 8, dtype=I8, device=dev), torch.zeros(4, device=dev)
+    plan = expert_plan(torch.zeros(2, 2, dtype=torch.int64, device=dev), 3)
+    one = torch.ones(6, device=dev)
+    for bad in (lambda: int8_weight(torch.ones(8, device=dev)), lambda: int8_weight(torch.ones(8, 6, device=dev).double()),
+                lambda: int8_weight(torch.ones(0, 6, device=dev)), lambda: int8_weight(torch.ones(8, 0, device=dev)),
+                lambda: int8_weight(torch.ones(MAX_CIN + 1, 1, device=dev)), lambda: int8_weight(torch.ones(1025, 1, 1, device=dev)),
+                lambda: int8_weight(q), lambda: int8_weight(q, s), lambda: int8_weight(x, one), lambda: int8_weight(q, torch.zeros(8, device=dev).double()),
+                lambda: quantize_rows(x[0]), lambda: quantize_rows(x.double()), lambda: quantize_rows(q), lambda: quantize_rows(x[:, :0]),
+                lambda: quantize_rows(x.clone().requires_grad_()),
+                lambda: int8_linear(x, x), lambda: int8_linear(x[:, :7], w), lambda: int8_linear(x[0], w), lambda: int8_linear(x.double(), w),
+                lambda: int8_linear(q, w), lambda: int8_linear(q, w, scale=s[:3]), lambda: int8_linear(q, w, scale=s.double()), lambda: int8_linear(x, w, scale=s),
+                lambda: int8_linear(x, w, one[:5]), lambda: int8_linear(x, w, one.long()), lambda: int8_linear(x, w, one.view(1, 6)),
+                lambda: int8_linear(x, w, out_dtype=torch.float64), lambda: int8_linear(x, w, out_dtype=I8),
+                lambda: int8_linear(x, w3), lambda: int8_linear(x, w, gather=True), lambda: int8_linear(x, w, plan=plan),
+                lambda: int8_linear(x[:3], w3, plan=plan), lambda: int8_linear(x, w3, plan=plan, gather=True), lambda: int8_linear(x, w3, plan=(1, 2)),
+                lambda: int8_linear(x, w3, one.view(1, 6).expand(2, 6), plan=plan), lambda: int8_linear(x.clone().requires_grad_(), w)):
+        with pytest.raises(_lib.CG3DError):
+            bad()
+    with torch.no_grad():
+        assert int8_linear(x.clone().requires_grad_(), w).shape == (4, 6)
+
+
+def test_refusals(oracle):
+    with _lib.use_library(oracle):
+        refusals("cpu")
+        assert int8_linear(torch.zeros(0, 8), int8_weight(torch.ones(8, 6))).shape == (0, 6)
+        assert quantize_rows(torch.zeros(0, 8))[0].shape == (0, 8)
+
+
+def test_entry_points_refuse(oracle):
+    """The C-ABI's own checks (the same conditions in the library and in its restatement; nothing is launched)."""
+    f = torch.zeros(4096)
+    a = f.data_ptr()
+    for lib in (oracle, _lib.bind(_lib.HIP_LIB_PATH)):
+        for e, cin, cout in ((0, 8, 8), (1025, 8, 8), (1, 0, 8), (1, MAX_CIN + 1, 8), (1, 8, 0), (1, 8, (1 << 20) + 1)):
+            assert lib.raw("cg3d_int8_weight_bytes")(e, cin, cout) == -1
+            assert lib.raw("cg3d_int8_weight")(a, 0, e, cin, cout, a, a, a, None) == -1
+        for args in ((None, 0, 1, 8, 8, a, a, a), (a, 4, 1, 8, 8, a, a, a), (a, 0, 1, 8, 8, None, a, a), (a, 0, 1, 8, 8, a + 4, a, a),
+                     (a, 0, 1, 8, 8, a, None, a), (a, 0, 1, 8, 8, a, a, None), (a + 2, 0, 1, 8, 8, a, a, a), (a + 1, 1, 1, 8, 8, a, a, a)):
+            assert lib.raw("cg3d_int8_weight")(*args, None) == -1, args
+        for args in ((a, 3, 4, 8, 8, a, a), (a, 0, -1, 8, 8, a, a), (a, 0, 4, 0, 8, a, a), (a, 0, 4, 8, 7, a, a), (None, 0, 4, 8, 8, a, a),
+                     (a, 0, 4, 8, 8, None, a), (a, 0, 4, 8, 8, a, None), (a + 2, 0, 4, 8, 8, a, a), (a, 0, 4, 8, 8, a, a + 2)):
+            assert lib.raw("cg3d_int8_quantize_rows")(*args, None) == -1, args
+        good = dict(x=a, dtype=0, sx=None, n_x=4, cin=8, w=a, sw=a, bias=None, bpe=0, offsets=None, rows=None, y=a, out=0, n_rows=4, cout=6, e=1, ws=a)
+        for change in (dict(dtype=4), dict(dtype=-1), dict(out=3), dict(out=-1), dict(bpe=2), dict(n_x=3), dict(e=2), dict(rows=a), dict(x=None),
+                       dict(w=None), dict(sw=None), dict(y=None), dict(ws=None), dict(ws=a + 4), dict(x=a + 2), dict(w=a + 8), dict(y=a + 2),
+                       dict(sw=a + 2), dict(bias=a + 1), dict(dtype=3, ws=None), dict(dtype=3, sx=a + 2), dict(n_x=-4, n_rows=-4), dict(cin=0), dict(cout=0),
+                       dict(offsets=a, n_x=3), dict(offsets=a, rows=a, n_x=0), dict(n_rows=1 << 31, n_x=1 << 31)):
+            assert lib.raw("cg3d_int8_linear")(*{**good, **change}.values(), None) == -1, change
+
+
+def test_no_cpu_fallback():
+    with _lib.use_library(_lib.bind(_lib.HIP_LIB_PATH)):
+        with pytest.raises(_lib.CG3DError):
+            int8_weight(torch.zeros(4, 2))
+        with pytest.raises(_lib.CG3DError):
+            quantize_rows(torch.zeros(4, 2))
+
+
+# ------------------------------------------------------------------------------------------------------------------- GPU
+@pytest.mark.gpu
+def test_hip_levels_and_nonfinite(hip):
+    levels("cuda")
+    nonfinite("cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,cin", [(1, 1), (3, 15), (1000, 64), (77, 250), (513, 512), (130, 1025), (65, 4096), (9, 5000), (3, 43904), (2, MAX_CIN)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_hip_quantize_rows(hip, n, cin, dtype):
+    x = make(n, cin, 1, dtype, 11)[0].cuda()
+    check_levels(x, *quantize_rows(x))
+
+
+WIDE = [(1, 64, 64), (1, 4096, 256), (5, 512, 320), (16, 1000, 72), (31, 2048, 100), (64, 512, 512), (65, 576, 64), (127, 64, 128), (128, 128, 64),
+        (300, 512, 192), (1003, 200, 77), (513, 1024, 300), (2050, 384, 136), (4099, 64, 64), (700, 1100, 520), (40, 43904, 128), (300, 9000, 64),
+        (3, MAX_CIN, 5), (5000, 130, 40), (256, 2048, 512), (1000, 640, 640)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,cin,cout", ODD + WIDE)
+@pytest.mark.parametrize("dtype,out,bias", [(F32, F32, True), (BF16, BF16, True), (F16, F16, False), (I8, F32, True), (I8, BF16, False)])
+def test_hip_dense(hip, n, cin, cout, dtype, out, bias):
+    dense(n, cin, cout, dtype, out, bias, 12, "cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,cin,cout", [(70, 200, 77), (130, 64, 64), (5, 512, 64), (260, 1024, 128)])
+def test_hip_dense_at_odd_addresses(hip, n, cin, cout):
+    for dtype, out in ((F32, F32), (BF16, BF16), (F16, F16), (I8, F32)):
+        dense(n, cin, cout, dtype, out, True, 13, "cuda", offset=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,k,experts,cin,cout,kind", [
+    (1, 1, 1, 64, 64, "uniform"), (1, 2, 18, 128, 64, "uniform"), (4, 2, 64, 512, 512, "uniform"), (20, 2, 5, 33, 18, "dropped"),
+    (300, 2, 18, 128, 64, "dropped"), (300, 2, 18, 128, 64, "one"), (50, 2, 7, 70, 90, "none"), (900, 4, 61, 96, 200, "uniform"),
+    (64, 1, 200, 100, 70, "uniform"), (1500, 2, 3, 640, 256, "dropped"), (700, 2, 4, 1024, 130, "uniform"), (3000, 2, 10, 64, 64, "uniform"),
+    (16, 4, 1024, 64, 32, "uniform")])
+@pytest.mark.parametrize("dtype,out,bias,gather", [(F32, F32, 2, True), (BF16, BF16, 0, True), (F16, F16, 1, False), (I8, F32, 2, True), (I8, BF16, 2, False)])
+def test_hip_grouped(hip, t, k, experts, cin, cout, kind, dtype, out, bias, gather):
+    grouped(ids_of(t, k, experts, kind, 14), experts, cin, cout, dtype, out, bias, gather, 15, "cuda")
+
+
+@pytest.mark.gpu
+def test_hip_largest_sum_does_not_wrap(hip):
+    """Every product at its largest: -128 * -128 over the longest contraction."""
+    x = torch.full((3, MAX_CIN), -128, dtype=I8, device="cuda")
+    w = int8_weight(torch.full((MAX_CIN, 2), -128, dtype=I8, device="cuda"), torch.ones(2, device="cuda"))
+    y = int8_linear(x, w, scale=torch.ones(3, device="cuda"))
+    want = 16384.0 * MAX_CIN
+    assert bool(((y.double() - want).abs() <= 2.0 ** -24 * want).all())
+
+
+@pytest.mark.gpu
+def test_hip_weights_in_8_bits(hip):
+    eight_bit_weights("cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_hip_quantised_first_is_the_same(hip, dtype):
+    """A row quantised in the call and one quantised before it give the same bits, whichever kernel takes them."""
+    for n, cin, cout in ((1, 512, 512), (40, 100, 70), (3000, 256, 128), (600, 1500, 64), (9, 6000, 130)):
+        x, _, w, b = make(n, cin, cout, dtype, 16)
+        x, weight, b = x.cuda(), int8_weight(w.cuda()), b.cuda()
+        q, s = quantize_rows(x)
+        assert torch.equal(int8_linear(x, weight, b, out_dtype=F32), int8_linear(q, weight, b, scale=s))
+
+
+@pytest.mark.gpu
+def test_hip_gather_is_the_gathered_product(hip):
+    for t, cin in ((5, 128), (2000, 128), (300, 700)):
+        ids = ids_of(t, 2, 18, "dropped", 17).cuda()
+        plan = expert_plan(ids, 18)
+        x, _, w, b = make(t, cin, 64, BF16, 18, 18)
+        x, weight, b = x.cuda(), int8_weight(w.cuda()), b.cuda()
+        assert torch.equal(int8_linear(x, weight, b, plan=plan, gather=True), int8_linear(expert_gather(x, plan), weight, b, plan=plan))
+
+
+@pytest.mark.gpu
+def test_hip_views_and_bias_types(hip):
+    x, _, w, b = make(64, 96, 40, BF16, 19)
+    x, w, b = x.cuda(), w.cuda(), b.cuda()
+    want = int8_linear(x, int8_weight(w), b.to(BF16).float())
+    assert torch.equal(int8_linear(x.t().contiguous().t(), int8_weight(w.t().contiguous().t()), b.to(BF16)), want)
+    wide = torch.randn(64, 200, device="cuda").to(BF16)
+    wide[:, 50:146] = x
+    assert torch.equal(int8_linear(wide[:, 50:146], int8_weight(w), b.to(BF16)), want)
+
+
+@pytest.mark.gpu
+def test_hip_graph_replays_with_new_inputs(hip):
+    """A served layer of experts captured once, replayed on new tokens with eager calls between; two graphs share nothing."""
+    t, k, e = 700, 2, 18
+    weight = int8_weight(make(1, 640, 128, F32, 20, e)[2].cuda())
+    small = int8_weight(make(1, 128, 64, F32, 21, e)[2].cuda())
+    ids = [ids_of(t, k, e, "dropped", s).cuda() for s in (22, 23, 24)]
+    xs = [make(t, 640, 1, BF16, s)[0].cuda() for s in (22, 23, 24)]
+    gate = torch.rand(t, k, device="cuda")
+
+    def step(i, x):
+        plan = expert_plan(i, e)
+        return expert_combine(int8_linear(int8_linear(x, weight, plan=plan, gather=True), small, plan=plan), plan, gate)
+    static = [(ids[0].clone(), xs[0].clone()) for _ in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*static[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for i, x in static:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(i, x))
+        graphs.append(g)
+    for turn in range(3):
+        for j in range(2):
+            static[j][0].copy_(ids[(turn + j) % 3])
+            static[j][1].copy_(xs[(turn + j) % 3])
+        for g in graphs:
+            g.replay()
+        for j in range(2):
+            assert torch.equal(outs[j], step(ids[(turn + j) % 3], xs[(turn + j) % 3]))
+
+
+@pytest.mark.gpu
+def test_hip_on_another_stream(hip):
+    x, _, w, b = make(3000, 700, 192, BF16, 25)
+    x, weight, b = x.cuda(), int8_weight(w.cuda()), b.cuda()
+    want = int8_linear(x, weight, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = int8_linear(x, weight, b)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_hip_served_layer_of_experts(hip):
+    """Two products of each token's experts and the weighted combination, against the same in 64 bits on the same levels."""
+    t, k, e, c, n = 500, 2, 10, 128, 256
+    ids = ids_of(t, k, e, "uniform", 26)
+    x, _, w1, b1 = make(t, c, n, BF16, 27, e)
+    w2 = make(1, n, c, F32, 28, e)[2]
+    gate = torch.rand(t, k)
+    plan = expert_plan(ids.cuda(), e)
+    h = torch.relu(int8_linear(x.cuda(), int8_weight(w1.cuda()), b1.cuda(), plan=plan, gather=True, out_dtype=F32))
+    y = int8_linear(h, int8_weight(w2.cuda()), plan=plan)
+    out = expert_combine(y, plan, gate.cuda())
+    rows, off = plan.rows.cpu().long(), plan.offsets.cpu().long()
+    expert = torch.bucketize(torch.arange(t * k), off[1:], right=True)
+
+    def levels_of(w):
+        q, s = plain_levels(w.transpose(1, 2).reshape(-1, w.shape[1]))
+        return q.view(e, w.shape[2], w.shape[1]).transpose(1, 2), s.view(e, w.shape[2])
+    want, size = reference(x, None, *levels_of(w1), b1, expert, rows)
+    close(h, torch.relu(want), size, F32)
+    want, size = reference(h, None, *levels_of(w2), None, expert, torch.arange(t * k))
+    close(y, want, size, F32)
+    pos = plan.pos.cpu().long()
+    terms = y.cpu().double()[pos] * gate.double().unsqueeze(2)
+    assert bool(((out.cpu().double() - terms.sum(1)).abs() <= (k + 2) * 2.0 ** -24 * terms.abs().sum(1)).all())
+
+
+@pytest.mark.gpu
+def test_hip_refusals(hip):
+    refusals("cuda")
+    w = int8_weight(torch.ones(8, 6, device="cuda"))
+    for bad in (lambda: int8_linear(torch.zeros(4, 8), w), lambda: int8_linear(torch.zeros(4, 8, device="cuda"), w, torch.zeros(6))):
+        with pytest.raises(_lib.CG3DError):
+            bad()
+    assert int8_linear(torch.zeros(0, 8, device="cuda"), w).shape == (0, 6)
