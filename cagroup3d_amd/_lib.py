@@ -99,7 +99,7 @@ _SIGNATURES = {
     "cg3d_ball_query": (c_int32, [c_int32, c_int32, c_int32, c_float, c_int32, P, P, P, P]),
     "cg3d_sort_vertices": (c_int32, [c_int32, c_int32, c_int32, P, P, P, P, P]),
     "cg3d_expert_plan_ws_bytes": (c_int64, [c_int64, c_int32, c_int32]),
-    "cg3d_expert_plan": (c_int32, [P, c_int32, c_int64, c_int32, c_int32, P, P, P, P, P]),
+    "cg3d_expert_plan": (c_int32, [P, c_int32, c_int64, c_int32, c_int32, P, P, P, P, P, P]),
     "cg3d_expert_gather": (c_int32, [P, c_int32, P, c_int64, c_int32, c_int32, P, P]),
     "cg3d_expert_combine": (c_int32, [P, c_int32, P, P, c_int32, c_int64, c_int32, c_int32, P, P]),
     "cg3d_expert_combine_bwd": (c_int32, [P, P, c_int32, P, P, c_int32, c_int64, c_int32, c_int32, P, P, P]),

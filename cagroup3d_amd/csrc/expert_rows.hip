@@ -7,13 +7,17 @@
 //   gather       r[row(t, s)] = x[t]                    its gradient   dx[t] = sum_s dr[row(t, s)]
 //   combine      o[t] = sum_s w[t, s] y[row(t, s)]      its gradient   dy[row(t, s)] = w[t, s] do[t],  dw[t, s] = <do[t], y[row(t, s)]>
 //
-// All four passes run token by token: a token's own row is read (written) once for its k slots, the rows in expert order are
-// whole lines at arbitrary places, and no sum needs an atomic -- every result is the same from run to run.  The T * k - offsets[E]
-// rows behind the last are given to the pairs without a row (pos = ~row, negative), so that the pass that writes rows clears them
-// too.  Sums are held in fp32 in slot order and rounded once.
+// Every pass runs over what it WRITES, row by row or token by token, so that writes are streamed and only reads jump (the gather of
+// 155 773 x 2 rows of 256 bytes: 41 us token by token, 29 us row by row), and no sum needs an atomic: results are the same from run to
+// run.  The T * k - offsets[E] rows behind the last belong to the pairs without a row (pos = ~row, pairs = ~pair, negative), so that
+// the passes that write rows clear them, and their weights' gradients.  Sums are held in fp32 in slot order and rounded once.
 #include "cg3d_common.h"
 
 #define EX_MAX_EXPERTS 1024
+#define EX_THREADS 512               // of the plan's workgroups
+#define EX_STEPS 4                   // ids of a lane in flight
+#define EX_CHUNK (EX_THREADS * EX_STEPS)
+#define EX_BLOCKS 256
 
 // ---------------------------------------------------------------- element types
 struct ex_bf16 {
@@ -64,39 +68,11 @@ static __device__ __forceinline__ uint64_t ex_peers(int key, bool in, int bits) 
 }
 static __device__ __forceinline__ uint64_t ex_below(int lane) { return (1ull << lane) - 1; }
 
-// counts of the keys of pairs [p0, p1) into the wave's row h[0 .. E]
-static __device__ __forceinline__ void ex_wave_count(const void *ids, int32_t wide, int64_t p0, int64_t p1, int E, int bits, int lane,
-                                                     int32_t *h) {
-    for (int64_t p = p0; p < p1; p += 64) {
-        const bool in = p + lane < p1;
-        const int key = in ? ex_key(ids, wide, p + lane, E) : E;
-        const uint64_t m = ex_peers(key, in, bits);
-        if (in && (m & ex_below(lane)) == 0) atomicAdd(&h[key], __popcll(m));    // (the first of its peers; no other wave's row)
-    }
-}
-// the rows of the pairs [p0, p1): h[key] holds the next row of each key and is moved on
-static __device__ __forceinline__ void ex_wave_place(const void *ids, int32_t wide, int64_t p0, int64_t p1, int E, int bits, int lane,
-                                                     int32_t *h, int32_t k, int32_t *__restrict__ rows, int32_t *__restrict__ pos) {
-    for (int64_t p = p0; p < p1; p += 64) {
-        const bool in = p + lane < p1;
-        const int key = in ? ex_key(ids, wide, p + lane, E) : E;
-        const uint64_t m = ex_peers(key, in, bits);
-        int base = 0;
-        if (in && (m & ex_below(lane)) == 0) base = atomicAdd(&h[key], __popcll(m));
-        const int first = in ? __ffsll((unsigned long long)m) - 1 : lane;
-        base = __shfl(base, first);
-        if (in) {
-            const int row = base + __popcll(m & ex_below(lane));
-            pos[p + lane] = key < E ? row : ~row;
-            rows[row] = key < E ? (int32_t)((p + lane) / k) : -1;
-        }
-    }
-}
-// exclusive prefix sums over keys [0, E] of tot[], in place, by the whole block (nt threads, scr: nt / 64 ints)
+// exclusive prefix sums of tot[0 .. n) in place, by the whole workgroup (scr: an int for each wave)
 static __device__ __forceinline__ void ex_block_scan(int32_t *tot, int n, int32_t *scr) {
-    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
     int carry = 0;
-    for (int b = 0; b < n; b += nt) {
+    for (int b = 0; b < n; b += blockDim.x) {
         const int i = b + tid;
         const int v = i < n ? tot[i] : 0;
         int s = v;
@@ -105,169 +81,242 @@ static __device__ __forceinline__ void ex_block_scan(int32_t *tot, int n, int32_
         if (lane == 63) scr[wave] = s;
         __syncthreads();
         int before = carry, all = 0;
-        for (int w = 0; w < (nt >> 6); w++) { if (w < wave) before += scr[w]; all += scr[w]; }
+        for (int w = 0; w < nw; w++) { const int c = scr[w]; if (w < wave) before += c; all += c; }
         if (i < n) tot[i] = before + s - v;
         carry += all;
         __syncthreads();
     }
 }
 
-// up to EX_ONE pairs: everything in one workgroup of 16 waves
-#define EX_ONE 16384
-__global__ __launch_bounds__(1024) void k_expert_plan_one(const void *__restrict__ ids, int32_t wide, int32_t n, int32_t k, int32_t E,
-                                                          int32_t bits, int32_t *__restrict__ offsets, int32_t *__restrict__ rows,
-                                                          int32_t *__restrict__ pos) {
-    extern __shared__ int32_t ex_sm[];
-    const int nw = blockDim.x >> 6, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int32_t *const hist = ex_sm, *const tot = ex_sm + nw * (E + 1), *const scr = tot + (E + 1);
-    for (int i = tid; i < nw * (E + 1); i += blockDim.x) hist[i] = 0;
-    __syncthreads();
-    const int per = ((n + nw - 1) / nw + 63) & ~63;
-    const int p0 = min(n, wave * per), p1 = min(n, p0 + per);
-    ex_wave_count(ids, wide, p0, p1, E, bits, lane, hist + wave * (E + 1));
-    __syncthreads();
-    for (int e = tid; e <= E; e += blockDim.x) {
-        int s = 0;
-        for (int w = 0; w < nw; w++) { const int c = hist[w * (E + 1) + e]; hist[w * (E + 1) + e] = s; s += c; }
-        tot[e] = s;
+// A chunk of blockDim * EX_STEPS pairs belongs to a workgroup: wave w takes the EX_STEPS * 64 pairs behind w of those, all its ids in
+// flight at once.  Chunks of one workgroup follow each other, so that any number of pairs needs at most EX_BLOCKS workgroups.
+// ex_chunk_ranks: counts of the keys in the wave's row h[0 .. E] of LDS and each pair's rank in the wave.
+static __device__ __forceinline__ void ex_chunk_keys(const void *ids, int32_t wide, int64_t p, int64_t n, int E, int (&key)[EX_STEPS]) {
+#pragma unroll
+    for (int i = 0; i < EX_STEPS; i++) {
+        const int64_t q = p + i * 64;
+        key[i] = ex_key(ids, wide, q < n ? q : n - 1, E);
     }
-    __syncthreads();
-    ex_block_scan(tot, E + 1, scr);
-    for (int e = tid; e <= E; e += blockDim.x) {
-        offsets[e] = tot[e];                             // tot[E]: the first row without a pair = the number of rows
-        for (int w = 0; w < nw; w++) hist[w * (E + 1) + e] += tot[e];
+}
+static __device__ __forceinline__ void ex_chunk_ranks(const int (&key)[EX_STEPS], int64_t p, int64_t n, int bits, int lane, int32_t *h,
+                                                      int (&rank)[EX_STEPS]) {
+#pragma unroll
+    for (int i = 0; i < EX_STEPS; i++) {
+        const bool in = p + i * 64 < n;
+        if (!__any(in)) break;
+        const uint64_t m = ex_peers(key[i], in, bits);
+        int base = 0;
+        if (in && (m & ex_below(lane)) == 0) base = atomicAdd(&h[key[i]], __popcll(m));      // (the first of its peers)
+        base = __shfl(base, in ? __ffsll((unsigned long long)m) - 1 : lane);
+        rank[i] = base + __popcll(m & ex_below(lane));
     }
-    __syncthreads();
-    ex_wave_place(ids, wide, p0, p1, E, bits, lane, hist + wave * (E + 1), k, rows, pos);
+}
+static __device__ __forceinline__ void ex_chunk_count(const int (&key)[EX_STEPS], int64_t p, int64_t n, int bits, int lane, int32_t *h) {
+#pragma unroll
+    for (int i = 0; i < EX_STEPS; i++) {
+        const bool in = p + i * 64 < n;
+        if (!__any(in)) break;
+        const uint64_t m = ex_peers(key[i], in, bits);
+        if (in && (m & ex_below(lane)) == 0) atomicAdd(&h[key[i]], __popcll(m));             // (whole numbers: any order)
+    }
 }
 
-// more pairs: workgroup b owns the pairs [b * per_block, (b + 1) * per_block); counts [nblk][E + 1] go through memory, and every
-// workgroup of the second launch adds up the columns it needs itself (at most EX_BLOCKS rows)
-#define EX_BLOCKS 256
-__global__ __launch_bounds__(256) void k_expert_plan_count(const void *__restrict__ ids, int32_t wide, int64_t n, int32_t E, int32_t bits,
-                                                           int64_t per_wave, int32_t *__restrict__ counts) {
+// more than one workgroup: counts [nblk][W4] of the workgroups' pairs go through memory (W4: E + 1 up to a multiple of 4)
+__global__ __launch_bounds__(EX_THREADS) void k_expert_plan_count(const void *__restrict__ ids, int32_t wide, int64_t n, int32_t E,
+                                                                  int32_t bits, int32_t chunks, int32_t *__restrict__ counts) {
     extern __shared__ int32_t ex_sm[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i <= E; i += 256) ex_sm[i] = 0;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, W4 = (E + 4) & ~3;
+    const int64_t p = (int64_t)blockIdx.x * chunks * EX_CHUNK + wave * (EX_STEPS * 64) + lane;
+    int key[EX_STEPS];
+    ex_chunk_keys(ids, wide, p, n, E, key);
+    for (int i = tid; i < W4; i += EX_THREADS) ex_sm[i] = 0;
     __syncthreads();
-    const int64_t p0 = min(n, ((int64_t)blockIdx.x * 4 + wave) * per_wave), p1 = min(n, p0 + per_wave);
-    ex_wave_count(ids, wide, p0, p1, E, bits, lane, ex_sm);       // (one row for the workgroup: whole numbers add up in any order)
+    ex_chunk_count(key, p, n, bits, lane, ex_sm);
+    for (int c = 1; c < chunks; c++) {
+        ex_chunk_keys(ids, wide, p + (int64_t)c * EX_CHUNK, n, E, key);
+        ex_chunk_count(key, p + (int64_t)c * EX_CHUNK, n, bits, lane, ex_sm);
+    }
     __syncthreads();
-    for (int i = tid; i <= E; i += 256) counts[(int64_t)blockIdx.x * (E + 1) + i] = ex_sm[i];
+    for (int i = tid; i < W4; i += EX_THREADS) counts[(int64_t)blockIdx.x * W4 + i] = ex_sm[i];
 }
-__global__ __launch_bounds__(256) void k_expert_plan_place(const void *__restrict__ ids, int32_t wide, int64_t n, int32_t k, int32_t E,
-                                                           int32_t bits, int64_t per_wave, const int32_t *__restrict__ counts,
-                                                           int32_t *__restrict__ offsets, int32_t *__restrict__ rows,
-                                                           int32_t *__restrict__ pos) {
+// The first row of each key for this workgroup, from the counts of all of them (the workgroup adds the at most EX_BLOCKS rows up
+// itself, four columns of a thread at a time), or from its own pairs when it is the only one; then chunk by chunk the rows of the pairs.
+__global__ __launch_bounds__(EX_THREADS) void k_expert_plan_place(const void *__restrict__ ids, int32_t wide, int64_t n, int32_t k,
+                                                                  int32_t E, int32_t bits, int32_t chunks, const int32_t *__restrict__ counts,
+                                                                  int32_t *__restrict__ offsets, int32_t *__restrict__ rows,
+                                                                  int32_t *__restrict__ pairs, int32_t *__restrict__ pos) {
     extern __shared__ int32_t ex_sm[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nblk = gridDim.x, me = blockIdx.x;
-    int32_t *const hist = ex_sm, *const tot = ex_sm + 4 * (E + 1), *const mine = tot + (E + 1), *const scr = mine + (E + 1);
-    for (int i = tid; i < 4 * (E + 1); i += 256) hist[i] = 0;
-    for (int e = tid; e <= E; e += 256) {
-        int all = 0, before = 0;
-        for (int b = 0; b < nblk; b++) { const int c = counts[(int64_t)b * (E + 1) + e]; all += c; before += b < me ? c : 0; }
-        tot[e] = all;
-        mine[e] = before;
+    const int tid = threadIdx.x, nt = blockDim.x, nw = nt >> 6, lane = tid & 63, wave = tid >> 6, nblk = gridDim.x, me = blockIdx.x;
+    const int W4 = (E + 4) & ~3, W = E + 1;
+    int32_t *const hist = ex_sm, *const tot = ex_sm + nw * W4, *const next = tot + W4, *const scr = next + W4;
+    const int64_t chunk = (int64_t)nt * EX_STEPS;
+    const int64_t p0 = (int64_t)me * chunks * chunk + wave * (EX_STEPS * 64) + lane;
+    int key[EX_STEPS], rank[EX_STEPS];
+    if (n > 0) ex_chunk_keys(ids, wide, p0, n, E, key);              // (the first chunk's ids travel while the counts are added up)
+    for (int i = tid; i < (nw + 2) * W4; i += nt) ex_sm[i] = 0;
+    __syncthreads();
+    if (counts) {
+        const int nv = W4 >> 2;
+        int width = 1;
+        while (width < nv && width < nt) width <<= 1;
+        const int part = tid / width, parts = nt / width;
+        for (int v = tid & (width - 1); v < nv; v += width) {
+            int4 all = make_int4(0, 0, 0, 0), before = all;
+#pragma unroll 4
+            for (int b = part; b < nblk; b += parts) {
+                const int4 c = *reinterpret_cast<const int4 *>(counts + (int64_t)b * W4 + v * 4);
+                all.x += c.x; all.y += c.y; all.z += c.z; all.w += c.w;
+                if (b < me) { before.x += c.x; before.y += c.y; before.z += c.z; before.w += c.w; }
+            }
+            atomicAdd(&tot[v * 4], all.x); atomicAdd(&tot[v * 4 + 1], all.y); atomicAdd(&tot[v * 4 + 2], all.z); atomicAdd(&tot[v * 4 + 3], all.w);
+            atomicAdd(&next[v * 4], before.x); atomicAdd(&next[v * 4 + 1], before.y); atomicAdd(&next[v * 4 + 2], before.z); atomicAdd(&next[v * 4 + 3], before.w);
+        }
+    } else if (chunks > 1)                                           // the only workgroup, several chunks: counted first
+        for (int c = 0; c < chunks; c++) {
+            int later[EX_STEPS];
+            ex_chunk_keys(ids, wide, p0 + c * chunk, n, E, later);
+            ex_chunk_count(later, p0 + c * chunk, n, bits, lane, tot);
+        }
+    if (n > 0) ex_chunk_ranks(key, p0, n, bits, lane, hist + wave * W4, rank);
+    __syncthreads();
+    if (!counts && chunks == 1) {
+        for (int e = tid; e < W; e += nt) {
+            int s = 0;
+            for (int w = 0; w < nw; w++) s += hist[w * W4 + e];
+            tot[e] = s;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    const int64_t p0 = min(n, ((int64_t)me * 4 + wave) * per_wave), p1 = min(n, p0 + per_wave);
-    ex_wave_count(ids, wide, p0, p1, E, bits, lane, hist + wave * (E + 1));
-    ex_block_scan(tot, E + 1, scr);                      // (starts and ends with barriers of its own for scr; tot is complete above)
-    __syncthreads();
-    for (int e = tid; e <= E; e += 256) {
-        if (me == 0) offsets[e] = tot[e];
-        int s = tot[e] + mine[e];
-        for (int w = 0; w < 4; w++) { const int c = hist[w * (E + 1) + e]; hist[w * (E + 1) + e] = s; s += c; }
+    ex_block_scan(tot, W, scr);
+    for (int e = tid; e < W; e += nt) {
+        if (me == 0) offsets[e] = tot[e];                            // (tot[E]: the first row without a pair = the number of rows)
+        next[e] += tot[e];
     }
-    __syncthreads();
-    ex_wave_place(ids, wide, p0, p1, E, bits, lane, hist + wave * (E + 1), k, rows, pos);
+    for (int c = 0; c < chunks; c++) {
+        const int64_t p = p0 + c * chunk;
+        if (c > 0) {
+            ex_chunk_keys(ids, wide, p, n, E, key);
+            __syncthreads();                                         // (the rows of hist have been read by everyone)
+            for (int i = lane; i < W; i += 64) hist[wave * W4 + i] = 0;
+            ex_chunk_ranks(key, p, n, bits, lane, hist + wave * W4, rank);
+            __syncthreads();
+        }
+        for (int e = tid; e < W; e += nt) {
+            int at = next[e];
+            for (int w = 0; w < nw; w++) { const int q = hist[w * W4 + e]; hist[w * W4 + e] = at; at += q; }
+            next[e] = at;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < EX_STEPS; i++) {
+            const int64_t q = p + i * 64;
+            if (q < n) {
+                const int row = hist[wave * W4 + key[i]] + rank[i];
+                const bool there = key[i] < E;
+                pos[q] = there ? row : ~row;
+                rows[row] = there ? (int32_t)((uint32_t)q / (uint32_t)k) : -1;
+                pairs[row] = there ? (int32_t)q : ~(int32_t)q;
+            }
+        }
+    }
 }
 
-static int64_t ex_blocks(int64_t n) { return n <= EX_ONE ? 0 : (cg3d_divup(n, 4 * 512) < EX_BLOCKS ? cg3d_divup(n, 4 * 512) : EX_BLOCKS); }
+// chunks of a workgroup and workgroups for n pairs
+static int32_t ex_chunks(int64_t n) { return n <= 2 * EX_CHUNK ? (n <= EX_CHUNK ? 1 : 2) : (int32_t)cg3d_divup(cg3d_divup(n, EX_CHUNK), EX_BLOCKS); }
+static int64_t ex_blocks(int64_t n) { const int64_t b = cg3d_divup(n, (int64_t)ex_chunks(n) * EX_CHUNK); return b > 1 ? b : 1; }
 
 extern "C" int64_t cg3d_expert_plan_ws_bytes(int64_t n_tokens, int32_t k, int32_t n_experts) {
     if (n_tokens < 0 || k < 1 || n_experts < 1 || n_experts > EX_MAX_EXPERTS || n_tokens > 0x7fffffffll / k) return CG3D_ERR_ARG;
-    return ex_blocks(n_tokens * k) * (n_experts + 1) * (int64_t)sizeof(int32_t);
+    const int64_t nblk = ex_blocks(n_tokens * k);
+    return nblk == 1 ? 0 : nblk * ((n_experts + 4) & ~3) * (int64_t)sizeof(int32_t);
 }
 extern "C" int cg3d_expert_plan(const void *experts, int32_t wide, int64_t n_tokens, int32_t k, int32_t n_experts, int32_t *offsets,
-                                int32_t *rows, int32_t *pos, void *ws, cg3d_stream_t stream) {
-    if (cg3d_expert_plan_ws_bytes(n_tokens, k, n_experts) < 0 || (wide != 0 && wide != 1) || !offsets) return CG3D_ERR_ARG;
+                                int32_t *rows, int32_t *pairs, int32_t *pos, void *ws, cg3d_stream_t stream) {
+    const int64_t need = cg3d_expert_plan_ws_bytes(n_tokens, k, n_experts);
+    if (need < 0 || (wide != 0 && wide != 1) || !offsets) return CG3D_ERR_ARG;
     const int64_t n = n_tokens * k;
-    if (n > 0 && (!experts || !rows || !pos || ((uintptr_t)experts & (wide ? 7 : 3)))) return CG3D_ERR_ARG;
+    if (n > 0 && (!experts || !rows || !pairs || !pos || ((uintptr_t)experts & (wide ? 7 : 3)))) return CG3D_ERR_ARG;
+    if (need > 0 && (!ws || ((uintptr_t)ws & 15))) return CG3D_ERR_ARG;
     const int64_t nblk = ex_blocks(n);
-    if (nblk > 0 && !ws) return CG3D_ERR_ARG;
+    const int32_t chunks = ex_chunks(n);
     int bits = 1;
     while ((n_experts >> bits) != 0) bits++;
     hipStream_t s = cg3d_hs(stream);
-    if (nblk == 0) {
-        int nt = n <= 64 ? 64 : n >= 1024 ? 1024 : (int)((n + 63) & ~63ll);
-        const size_t lds = ((size_t)(nt / 64 + 1) * (n_experts + 1) + 16) * sizeof(int32_t);
-        if (lds > 64 * 1024) {
-            if (hipFuncSetAttribute(reinterpret_cast<const void *>(&k_expert_plan_one), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
-                return CG3D_ERR_LAUNCH;
-        }
-        hipLaunchKernelGGL(k_expert_plan_one, dim3(1), dim3(nt), lds, s, experts, wide, (int32_t)n, k, n_experts, bits, offsets, rows, pos);
+    const int W4 = (n_experts + 4) & ~3;
+    const int nt = n >= EX_THREADS ? EX_THREADS : n <= 64 ? 64 : (int)((n + 63) & ~63ll);
+    const int lds = ((nt / 64 + 2) * W4 + nt / 64) * (int)sizeof(int32_t);          // (at most 41 KB)
+    int32_t *counts = need > 0 ? reinterpret_cast<int32_t *>(ws) : nullptr;
+    if (counts) {
+        hipLaunchKernelGGL(k_expert_plan_count, dim3((unsigned)nblk), dim3(EX_THREADS), W4 * sizeof(int32_t), s, experts, wide, n,
+                           n_experts, bits, chunks, counts);
         CG3D_CHECK_LAUNCH();
-        return CG3D_OK;
     }
-    const int64_t per_wave = (cg3d_divup(n, nblk * 4) + 63) & ~63ll;
-    int32_t *counts = reinterpret_cast<int32_t *>(ws);
-    hipLaunchKernelGGL(k_expert_plan_count, dim3((unsigned)nblk), dim3(256), (n_experts + 1) * sizeof(int32_t), s, experts, wide, n,
-                       n_experts, bits, per_wave, counts);
-    CG3D_CHECK_LAUNCH();
-    hipLaunchKernelGGL(k_expert_plan_place, dim3((unsigned)nblk), dim3(256), (6 * (n_experts + 1) + 4) * sizeof(int32_t), s, experts, wide,
-                       n, k, n_experts, bits, per_wave, counts, offsets, rows, pos);
+    hipLaunchKernelGGL(k_expert_plan_place, dim3((unsigned)nblk), dim3(nt), lds, s, experts, wide, n, k, n_experts, bits, chunks, counts,
+                       offsets, rows, pairs, pos);
     CG3D_CHECK_LAUNCH();
     return CG3D_OK;
 }
 
 // ---------------------------------------------------------------- rows
-static __device__ __forceinline__ int64_t ex_div(int64_t i, int32_t d) {
-    return (i >> 32) ? i / d : (int64_t)((uint32_t)i / (uint32_t)d);
-}
 // A thread owns V elements (16 bytes) of one token's row; the last vector of a row whose width V does not divide is moved back to
-// end with the row (its first elements are then computed twice, with the same result).  Rows shorter than a vector: V = 1.
+// end with the row (its first elements are then computed twice, with the same result).  Rows shorter than a vector: V = 1.  The
+// combination takes a token's slots EX_SLOTS at a time: their rows are looked up, and then read, together.
+#define EX_SLOTS 4
+// i / nv by a multiplication: magic = ceil(2^64 / nv), exact while i * nv < 2^64 (i counts 16-byte pieces of memory)
+static __device__ __forceinline__ int64_t ex_div(int64_t i, int32_t nv, uint64_t magic) {
+    return nv == 1 ? i : (int64_t)__umul64hi((uint64_t)i, magic);
+}
 template <typename T, int V>
-__global__ __launch_bounds__(256) void k_expert_gather(const T *__restrict__ x, const int32_t *__restrict__ pos, int64_t n_tokens,
-                                                       int32_t k, int32_t c, int32_t nv, T *__restrict__ out) {
+__global__ __launch_bounds__(256) void k_expert_gather(const T *__restrict__ x, const int32_t *__restrict__ rows, int64_t n_tokens,
+                                                       int64_t P, int32_t c, int32_t nv, uint64_t magic, T *__restrict__ out) {
     typedef ex_vec<T, V> vec;
-    const int64_t P = n_tokens * k;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n_tokens * nv; i += gridDim.x * 256ll) {
-        const int64_t t = ex_div(i, nv);
-        int a = (int)(i - t * nv) * V;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < P * nv; i += gridDim.x * 256ll) {
+        const int64_t j = ex_div(i, nv, magic);
+        int a = (int)(i - j * nv) * V;
         if (a + V > c) a = c - V;
-        const vec v = *reinterpret_cast<const vec *>(x + t * c + a);
-        vec z;
+        const int32_t t = rows[j];
+        vec v;
+        if (t >= 0 && t < n_tokens) v = *reinterpret_cast<const vec *>(x + (int64_t)t * c + a);
+        else {
 #pragma unroll
-        for (int j = 0; j < V; j++) z.e[j] = T::from(0.f);
-        for (int s = 0; s < k; s++) {
-            const int32_t r = pos[t * k + s];
-            const int64_t j = r < 0 ? ~r : r;
-            if (j < P) *reinterpret_cast<vec *>(out + j * c + a) = r < 0 ? z : v;
+            for (int u = 0; u < V; u++) v.e[u] = T::from(0.f);
         }
+        *reinterpret_cast<vec *>(out + j * c + a) = v;
     }
 }
 
 template <typename T, int V>
 __global__ __launch_bounds__(256) void k_expert_combine(const T *__restrict__ y, const int32_t *__restrict__ pos, const void *__restrict__ w,
-                                                        int32_t wtype, int64_t n_tokens, int32_t k, int32_t c, int32_t nv,
+                                                        int32_t wtype, int64_t n_tokens, int32_t k, int32_t c, int32_t nv, uint64_t magic,
                                                         T *__restrict__ out) {
     typedef ex_vec<T, V> vec;
     const int64_t P = n_tokens * k;
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n_tokens * nv; i += gridDim.x * 256ll) {
-        const int64_t t = ex_div(i, nv);
+        const int64_t t = ex_div(i, nv, magic);
         int a = (int)(i - t * nv) * V;
         if (a + V > c) a = c - V;
         float acc[V];
 #pragma unroll
         for (int j = 0; j < V; j++) acc[j] = 0.f;
-        for (int s = 0; s < k; s++) {
-            const int32_t r = pos[t * k + s];
-            if (r < 0 || r >= P) continue;
-            const float ws = ex_weight(w, wtype, t * k + s);
-            const vec v = *reinterpret_cast<const vec *>(y + (int64_t)r * c + a);
+        for (int s0 = 0; s0 < k; s0 += EX_SLOTS) {
+            int32_t r[EX_SLOTS];
+            float ws[EX_SLOTS];
+            vec v[EX_SLOTS];
 #pragma unroll
-            for (int j = 0; j < V; j++) acc[j] += ws * T::to(v.e[j]);
+            for (int s = 0; s < EX_SLOTS; s++) {
+                const bool in = s0 + s < k;
+                r[s] = in ? pos[t * k + s0 + s] : -1;
+                ws[s] = in ? ex_weight(w, wtype, t * k + s0 + s) : 0.f;
+            }
+#pragma unroll
+            for (int s = 0; s < EX_SLOTS; s++)
+                if (r[s] >= 0 && r[s] < P) v[s] = *reinterpret_cast<const vec *>(y + (int64_t)r[s] * c + a);
+#pragma unroll
+            for (int s = 0; s < EX_SLOTS; s++)
+                if (r[s] >= 0 && r[s] < P) {
+#pragma unroll
+                    for (int j = 0; j < V; j++) acc[j] += ws[s] * T::to(v[s].e[j]);
+                }
         }
         vec o;
 #pragma unroll
@@ -276,45 +325,43 @@ __global__ __launch_bounds__(256) void k_expert_combine(const T *__restrict__ y,
     }
 }
 
-// L lanes (a power of two, at most a wave) own one token: slot by slot dy = w do and the lanes' shares of <do, y>, joined by shuffles
+// L lanes (a power of two, at most a wave) own one row: dy = w do and the lanes' shares of <do, y>, joined by shuffles.  Row by row
+// and not token by token: y and dy are then streamed and only do is looked up (whose k uses the caches serve).
 template <typename T, int V>
-__global__ __launch_bounds__(256) void k_expert_combine_bwd(const T *__restrict__ dout, const T *__restrict__ y, const int32_t *__restrict__ pos,
-                                                            const void *__restrict__ w, int32_t wtype, int64_t n_tokens, int32_t k,
-                                                            int32_t c, int32_t nv, int32_t lshift, T *__restrict__ dy, void *__restrict__ dw) {
+__global__ __launch_bounds__(256) void k_expert_combine_bwd(const T *__restrict__ dout, const T *__restrict__ y, const int32_t *__restrict__ pairs,
+                                                            const void *__restrict__ w, int32_t wtype, int64_t P, int32_t k, int32_t c,
+                                                            int32_t nv, int32_t lshift, T *__restrict__ dy, void *__restrict__ dw) {
     typedef ex_vec<T, V> vec;
     const int L = 1 << lshift, lane = threadIdx.x & (L - 1);
-    const int64_t P = n_tokens * k;
-    // (whole groups of L lanes take a token and leave together)
-    for (int64_t t = (blockIdx.x * 256ll + threadIdx.x) >> lshift; t < n_tokens; t += (gridDim.x * 256ll) >> lshift)
-    for (int s = 0; s < k; s++) {
-        const int32_t r = pos[t * k + s];
-        const int64_t j = r < 0 ? ~(int64_t)r : (int64_t)r;
-        const bool there = r >= 0 && j < P;
-        const float ws = there ? ex_weight(w, wtype, t * k + s) : 0.f;
+    // (whole groups of L lanes take a row and leave together)
+    for (int64_t j = (blockIdx.x * 256ll + threadIdx.x) >> lshift; j < P; j += (gridDim.x * 256ll) >> lshift) {
+        const int32_t pr = pairs[j];
+        const bool there = pr >= 0 && pr < P;
+        const int32_t p = there ? pr : pr < 0 ? ~pr : 0x7fffffff;
+        const int64_t t = there ? (int64_t)((uint32_t)p / (uint32_t)k) : 0;
+        const float ws = there ? ex_weight(w, wtype, p) : 0.f;
         float dot = 0.f;
-        if (j < P) {
-            for (int q = lane; q < nv; q += L) {
-                const int a0 = q * V, a = a0 + V > c ? c - V : a0;
-                vec g, o;
-                if (there) g = *reinterpret_cast<const vec *>(dout + t * c + a);
-                if (dw && there) {
-                    const vec v = *reinterpret_cast<const vec *>(y + j * c + a);
+        for (int q = lane; q < nv; q += L) {
+            const int a0 = q * V, a = a0 + V > c ? c - V : a0;
+            vec g, v, o;
+            if (there) g = *reinterpret_cast<const vec *>(dout + t * c + a);
+            if (there && dw) {
+                v = *reinterpret_cast<const vec *>(y + j * c + a);
 #pragma unroll
-                    for (int u = 0; u < V; u++) dot += a + u >= a0 ? T::to(g.e[u]) * T::to(v.e[u]) : 0.f;
-                }
-                if (dy) {
+                for (int u = 0; u < V; u++) dot += a + u >= a0 ? T::to(g.e[u]) * T::to(v.e[u]) : 0.f;
+            }
+            if (dy) {
 #pragma unroll
-                    for (int u = 0; u < V; u++) o.e[u] = T::from(there ? ws * T::to(g.e[u]) : 0.f);
-                    *reinterpret_cast<vec *>(dy + j * c + a) = o;
-                }
+                for (int u = 0; u < V; u++) o.e[u] = T::from(there ? ws * T::to(g.e[u]) : 0.f);
+                *reinterpret_cast<vec *>(dy + j * c + a) = o;
             }
         }
         if (dw) {
             for (int d = L >> 1; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
-            if (lane == 0) {
-                if (wtype == CG3D_DT_F32) reinterpret_cast<float *>(dw)[t * k + s] = dot;
-                else if (wtype == CG3D_DT_BF16) reinterpret_cast<ex_bf16 *>(dw)[t * k + s] = ex_bf16::from(dot);
-                else reinterpret_cast<ex_f16 *>(dw)[t * k + s] = ex_f16::from(dot);
+            if (lane == 0 && p < P) {
+                if (wtype == CG3D_DT_F32) reinterpret_cast<float *>(dw)[p] = dot;
+                else if (wtype == CG3D_DT_BF16) reinterpret_cast<ex_bf16 *>(dw)[p] = ex_bf16::from(dot);
+                else reinterpret_cast<ex_f16 *>(dw)[p] = ex_f16::from(dot);
             }
         }
     }
@@ -326,6 +373,7 @@ static bool ex_bad(int32_t dtype, int32_t wtype, int64_t n_tokens, int32_t k, in
 }
 static bool ex_odd(const void *p, int32_t dtype) { return ((uintptr_t)p & (dtype == CG3D_DT_F32 ? 3 : 1)) != 0; }
 
+static uint64_t ex_magic(int32_t nv) { return nv > 1 ? ~0ull / (uint64_t)nv + 1 : 0; }      // (nv > 1 does not divide 2^64 - 1 + 1 evenly unless a power of two: then exact too)
 static int64_t ex_grid(int64_t nb) { return nb < (1 << 22) ? nb : (1 << 22); }      // (fewer than 2^32 threads; the kernels loop)
 
 #define EX_DISPATCH(LAUNCH)                                                                                        \
@@ -335,18 +383,18 @@ static int64_t ex_grid(int64_t nb) { return nb < (1 << 22) ? nb : (1 << 22); }  
         else { if (c >= 8) LAUNCH(ex_f16, 8); else LAUNCH(ex_f16, 1); }                                            \
     } while (0)
 
-extern "C" int cg3d_expert_gather(const void *x, int32_t dtype, const int32_t *pos, int64_t n_tokens, int32_t k, int32_t c, void *out,
+extern "C" int cg3d_expert_gather(const void *x, int32_t dtype, const int32_t *rows, int64_t n_tokens, int32_t k, int32_t c, void *out,
                                   cg3d_stream_t stream) {
     if (ex_bad(dtype, CG3D_DT_F32, n_tokens, k, c)) return CG3D_ERR_ARG;
     if (n_tokens == 0) return CG3D_OK;
-    if (!x || !pos || !out || ex_odd(x, dtype) || ex_odd(out, dtype)) return CG3D_ERR_ARG;
+    if (!x || !rows || !out || ex_odd(x, dtype) || ex_odd(out, dtype)) return CG3D_ERR_ARG;
     hipStream_t s = cg3d_hs(stream);
 #define EX_LAUNCH(T, V)                                                                                            \
     do {                                                                                                           \
         const int32_t nv = (int32_t)cg3d_divup(c, V);                                                              \
-        const int64_t nb = ex_grid(cg3d_divup(n_tokens * nv, 256));                                                \
-        hipLaunchKernelGGL((k_expert_gather<T, V>), dim3((unsigned)nb), dim3(256), 0, s, reinterpret_cast<const T *>(x), pos, n_tokens, k, \
-                           c, nv, reinterpret_cast<T *>(out));                                                     \
+        const int64_t nb = ex_grid(cg3d_divup(n_tokens * k * nv, 256));                                                \
+        hipLaunchKernelGGL((k_expert_gather<T, V>), dim3((unsigned)nb), dim3(256), 0, s, reinterpret_cast<const T *>(x), rows, n_tokens, n_tokens * k, \
+                           c, nv, ex_magic(nv), reinterpret_cast<T *>(out));                                                     \
     } while (0)
     EX_DISPATCH(EX_LAUNCH);
 #undef EX_LAUNCH
@@ -365,7 +413,7 @@ extern "C" int cg3d_expert_combine(const void *y, int32_t dtype, const int32_t *
         const int32_t nv = (int32_t)cg3d_divup(c, V);                                                              \
         const int64_t nb = ex_grid(cg3d_divup(n_tokens * nv, 256));                                                \
         hipLaunchKernelGGL((k_expert_combine<T, V>), dim3((unsigned)nb), dim3(256), 0, s, reinterpret_cast<const T *>(y), pos, w, wtype, \
-                           n_tokens, k, c, nv, reinterpret_cast<T *>(out));                                        \
+                           n_tokens, k, c, nv, ex_magic(nv), reinterpret_cast<T *>(out));                                        \
     } while (0)
     EX_DISPATCH(EX_LAUNCH);
 #undef EX_LAUNCH
@@ -373,11 +421,11 @@ extern "C" int cg3d_expert_combine(const void *y, int32_t dtype, const int32_t *
     return CG3D_OK;
 }
 
-extern "C" int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, const int32_t *pos, const void *w, int32_t wtype,
+extern "C" int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, const int32_t *pairs, const void *w, int32_t wtype,
                                        int64_t n_tokens, int32_t k, int32_t c, void *dy, void *dw, cg3d_stream_t stream) {
     if (ex_bad(dtype, wtype, n_tokens, k, c) || (!dy && !dw)) return CG3D_ERR_ARG;
     if (n_tokens == 0) return CG3D_OK;
-    if (!dout || !pos || (dw && (!y || !w)) || ex_odd(dout, dtype) || ex_odd(y, dtype) || ex_odd(dy, dtype) || ex_odd(w, wtype) || ex_odd(dw, wtype))
+    if (!dout || !pairs || (dw && (!y || !w)) || ex_odd(dout, dtype) || ex_odd(y, dtype) || ex_odd(dy, dtype) || ex_odd(w, wtype) || ex_odd(dw, wtype))
         return CG3D_ERR_ARG;
     hipStream_t s = cg3d_hs(stream);
 #define EX_LAUNCH(T, V)                                                                                            \
@@ -385,9 +433,9 @@ extern "C" int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t 
         const int32_t nv = (int32_t)cg3d_divup(c, V);                                                              \
         int32_t ls = 0;                                                                                            \
         while ((1 << ls) < nv && ls < 6) ls++;                                                                     \
-        const int64_t nb = ex_grid(cg3d_divup(n_tokens << ls, 256));                                               \
+        const int64_t nb = ex_grid(cg3d_divup(n_tokens * k << ls, 256));                                           \
         hipLaunchKernelGGL((k_expert_combine_bwd<T, V>), dim3((unsigned)nb), dim3(256), 0, s, reinterpret_cast<const T *>(dout),   \
-                           reinterpret_cast<const T *>(y), pos, w, wtype, n_tokens, k, c, nv, ls, reinterpret_cast<T *>(dy), dw);  \
+                           reinterpret_cast<const T *>(y), pairs, w, wtype, n_tokens * k, k, c, nv, ls, reinterpret_cast<T *>(dy), dw);  \
     } while (0)
     EX_DISPATCH(EX_LAUNCH);
 #undef EX_LAUNCH

@@ -37,12 +37,13 @@ def need(ok, message, *args):
 
 class ExpertPlan:
     """Where the rows of a routing go.  offsets int32 [n_experts + 1], rows int32 [T * k] (the token of each row, -1 behind the
-    last), pos int32 [T, k] (the row of each pair; negative: the pair has none)."""
+    last), pairs int32 [T * k] (the pair t * k + s of each row, negative behind the last), pos int32 [T, k] (the row of each pair;
+    negative: the pair has none)."""
 
-    __slots__ = ("offsets", "rows", "pos", "n_tokens", "k", "n_experts")
+    __slots__ = ("offsets", "rows", "pairs", "pos", "n_tokens", "k", "n_experts")
 
-    def __init__(self, offsets, rows, pos, n_experts):
-        self.offsets, self.rows, self.pos, self.n_experts = offsets, rows, pos, n_experts
+    def __init__(self, offsets, rows, pairs, pos, n_experts):
+        self.offsets, self.rows, self.pairs, self.pos, self.n_experts = offsets, rows, pairs, pos, n_experts
         self.n_tokens, self.k = pos.shape
 
     @property
@@ -65,12 +66,14 @@ def expert_plan(experts, n_experts):
     with on_device(ids):
         ws_bytes = int(lib.raw("cg3d_expert_plan_ws_bytes")(t, k, n_experts))
         n = t * k
-        out = torch.empty(2 * n + n_experts + 1 + ws_bytes // 4, dtype=torch.int32, device=ids.device)     # rows | pos | offsets | workspace
-        rows, pos, offsets = out[:n], out[n:2 * n].view(t, k), out[2 * n:2 * n + n_experts + 1]
-        ws = out.data_ptr() + 4 * (2 * n + n_experts + 1) if ws_bytes else None
+        n_ws = ws_bytes // 4
+        out = torch.empty(n_ws + 3 * n + n_experts + 1, dtype=torch.int32, device=ids.device)
+        _, rows, pairs, pos, offsets = out.split((n_ws, n, n, n, n_experts + 1))
+        pos = pos.view(t, k)
+        ws = ptr(out) if n_ws else None
         lib.call("cg3d_expert_plan", ptr(ids), c_int32(ids.dtype == torch.int64), c_int64(t), c_int32(k), c_int32(n_experts), ptr(offsets),
-                 ptr(rows), ptr(pos), ws, lib.stream())
-    return ExpertPlan(offsets, rows, pos, n_experts)
+                 ptr(rows), ptr(pairs), ptr(pos), ws, lib.stream())
+    return ExpertPlan(offsets, rows, pairs, pos, n_experts)
 
 
 def _check_rows(who, x, n, plan, what):
@@ -89,16 +92,16 @@ def _combine(lib, y, pos, w, t, k):
 
 class _Gather(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, pos):
+    def forward(ctx, x, pos, rows):
         lib = _lib.get()
         x = x.contiguous()
-        lib.check(x, pos)
+        lib.check(x, rows)
         t, k = pos.shape
         ctx.save_for_backward(pos)
         ctx.set_materialize_grads(False)
         with on_device(x):
             out = torch.empty((t * k, x.shape[1]), dtype=x.dtype, device=x.device)
-            lib.call("cg3d_expert_gather", ptr(x), c_int32(DTYPES[x.dtype]), ptr(pos), c_int64(t), c_int32(k), c_int32(x.shape[1]), ptr(out),
+            lib.call("cg3d_expert_gather", ptr(x), c_int32(DTYPES[x.dtype]), ptr(rows), c_int64(t), c_int32(k), c_int32(x.shape[1]), ptr(out),
                      lib.stream())
         return out
 
@@ -106,20 +109,21 @@ class _Gather(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         if dout is None:
-            return None, None
+            return None, None, None
         (pos,) = ctx.saved_tensors
         dout = dout.contiguous()
         with on_device(dout):
-            return _combine(_lib.get(), dout, pos, None, *pos.shape), None
+            return _combine(_lib.get(), dout, pos, None, *pos.shape), None, None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, pos, w):
+    def forward(ctx, y, pos, pairs, w):
         lib = _lib.get()
         y, w = y.contiguous(), None if w is None else w.contiguous()
         lib.check(y, pos, w)
-        ctx.save_for_backward(y if ctx.needs_input_grad[2] else None, pos, w)
+        ctx.save_for_backward(y if ctx.needs_input_grad[3] else None, pairs, w)
+        ctx.shape = pos.shape
         ctx.set_materialize_grads(False)
         with on_device(y):
             return _combine(lib, y, pos, w, *pos.shape)
@@ -128,23 +132,23 @@ class _Combine(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         if dout is None:
-            return None, None, None
-        y, pos, w = ctx.saved_tensors
-        t, k = pos.shape
+            return None, None, None, None
+        y, pairs, w = ctx.saved_tensors
+        t, k = ctx.shape
         lib = _lib.get()
         dout = dout.contiguous()
         with on_device(dout):
             dy = torch.empty((t * k, dout.shape[1]), dtype=dout.dtype, device=dout.device) if ctx.needs_input_grad[0] else None
-            dw = torch.empty_like(w) if ctx.needs_input_grad[2] else None
-            lib.call("cg3d_expert_combine_bwd", ptr(dout), ptr(y), c_int32(DTYPES[dout.dtype]), ptr(pos), ptr(w),
+            dw = torch.empty_like(w) if ctx.needs_input_grad[3] else None
+            lib.call("cg3d_expert_combine_bwd", ptr(dout), ptr(y), c_int32(DTYPES[dout.dtype]), ptr(pairs), ptr(w),
                      c_int32(0 if w is None else DTYPES[w.dtype]), c_int64(t), c_int32(k), c_int32(dout.shape[1]), ptr(dy), ptr(dw), lib.stream())
-        return dy, None, dw
+        return dy, None, None, dw
 
 
 def expert_gather(x, plan):
     """x [T, C] float32 / bfloat16 / float16 -> [T * k, C], the tokens' rows in the plan's order (differentiable in x)."""
     _check_rows("expert_gather", x, getattr(plan, "n_tokens", 0), plan, "x")
-    return _Gather.apply(x, plan.pos)
+    return _Gather.apply(x, plan.pos, plan.rows)
 
 
 def expert_combine(rows, plan, weights=None):
@@ -159,4 +163,4 @@ def expert_combine(rows, plan, weights=None):
         need(tuple(weights.shape) == (plan.n_tokens, plan.k), "expert_combine: weights must be [%d, %d], got %s", plan.n_tokens, plan.k,
              tuple(weights.shape))
         need(weights.device == rows.device, "expert_combine: weights are on %s, rows on %s", weights.device, rows.device)
-    return _Combine.apply(rows, plan.pos, weights)
+    return _Combine.apply(rows, plan.pos, plan.pairs, weights)

@@ -584,14 +584,17 @@ int cg3d_adamw_step(const int64_t *table, const int32_t *pid, int64_t nrows, con
  *   plan: P = n_tokens * k pairs p = t * k + s sorted by id, pairs of one id in ascending order:
  *     offsets int32 [n_experts + 1]  rows of expert e are [offsets[e], offsets[e + 1])
  *     rows    int32 [P]              the token of each row; -1 behind offsets[n_experts]
+ *     pairs   int32 [P]              the pair of each row; behind offsets[n_experts] ~p of a pair p without a row, each once
  *     pos     int32 [P]              the row of each pair; negative: none (~pos is one of the rows behind the last, which the
  *                                    passes that write rows clear)
- *   1 <= n_experts <= 1024, k >= 1, P < 2^31; ws: cg3d_expert_plan_ws_bytes bytes (may be NULL where that is 0).
+ *   1 <= n_experts <= 1024, k >= 1, P < 2^31; ws: cg3d_expert_plan_ws_bytes bytes, 16-byte aligned (may be NULL where
+ *   that is 0).
  * Element types `dtype` of rows, `wtype` of weights: CG3D_DT_F32 / _BF16 / _F16.  Rows are contiguous [*, c] of any width.
- *   gather:       out[pos] = x[t]              (out [P, c]; rows without a pair are zeros)
+ *   gather:       out[j] = x[rows[j]]           (out [P, c]; rows without a pair are zeros)
  *   combine:      out[t] = sum_s w[t, s] * y[pos[t, s]]   (w NULL: all ones -- also the gather's gradient); fp32 sums in slot
  *                 order, rounded once; a token without rows gives zeros
- *   combine_bwd:  dy[pos] = w[t, s] * dout[t] (rows without a pair: zeros), dw[t, s] = <dout[t], y[pos]> (0 without a row);
+ *   combine_bwd:  for row j of pair (t, s): dy[j] = w[t, s] * dout[t] (rows without a pair: zeros), dw[t, s] = <dout[t], y[j]>
+ *                 (0 without a row);
  *                 dy or dw may be NULL (not both); y may be NULL without dw */
 #define CG3D_DT_F32 0
 #define CG3D_DT_BF16 1
@@ -599,12 +602,12 @@ int cg3d_adamw_step(const int64_t *table, const int32_t *pid, int64_t nrows, con
 #define CG3D_DT_I8 3
 int64_t cg3d_expert_plan_ws_bytes(int64_t n_tokens, int32_t k, int32_t n_experts);
 int cg3d_expert_plan(const void *experts, int32_t wide, int64_t n_tokens, int32_t k, int32_t n_experts, int32_t *offsets, int32_t *rows,
-                     int32_t *pos, void *ws, cg3d_stream_t stream);
-int cg3d_expert_gather(const void *x, int32_t dtype, const int32_t *pos, int64_t n_tokens, int32_t k, int32_t c, void *out,
+                     int32_t *pairs, int32_t *pos, void *ws, cg3d_stream_t stream);
+int cg3d_expert_gather(const void *x, int32_t dtype, const int32_t *rows, int64_t n_tokens, int32_t k, int32_t c, void *out,
                        cg3d_stream_t stream);
 int cg3d_expert_combine(const void *y, int32_t dtype, const int32_t *pos, const void *w, int32_t wtype, int64_t n_tokens, int32_t k,
                         int32_t c, void *out, cg3d_stream_t stream);
-int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, const int32_t *pos, const void *w, int32_t wtype,
+int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, const int32_t *pairs, const void *w, int32_t wtype,
                             int64_t n_tokens, int32_t k, int32_t c, void *dy, void *dw, cg3d_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------

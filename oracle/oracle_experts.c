@@ -57,11 +57,11 @@ int64_t cg3d_expert_plan_ws_bytes(int64_t n_tokens, int32_t k, int32_t n_experts
     return 0;
 }
 int cg3d_expert_plan(const void *experts, int32_t wide, int64_t n_tokens, int32_t k, int32_t n_experts, int32_t *offsets, int32_t *rows,
-                     int32_t *pos, void *ws, cg3d_stream_t stream) {
+                     int32_t *pairs, int32_t *pos, void *ws, cg3d_stream_t stream) {
     (void)ws; (void)stream;
     if (cg3d_expert_plan_ws_bytes(n_tokens, k, n_experts) < 0 || (wide != 0 && wide != 1) || !offsets) return CG3D_ERR_ARG;
     const int64_t n = n_tokens * k;
-    if (n > 0 && (!experts || !rows || !pos || ((uintptr_t)experts & (wide ? 7 : 3)))) return CG3D_ERR_ARG;
+    if (n > 0 && (!experts || !rows || !pairs || !pos || ((uintptr_t)experts & (wide ? 7 : 3)))) return CG3D_ERR_ARG;
     int64_t next[1025];
     memset(next, 0, sizeof next);
 #define KEY(p) ({ const int64_t v = wide ? ((const int64_t *)experts)[p] : ((const int32_t *)experts)[p]; v < 0 || v >= n_experts ? n_experts : v; })
@@ -77,6 +77,7 @@ int cg3d_expert_plan(const void *experts, int32_t wide, int64_t n_tokens, int32_
         const int64_t e = KEY(p);
         const int32_t row = (int32_t)next[e]++;
         rows[row] = e < n_experts ? (int32_t)(p / k) : -1;
+        pairs[row] = e < n_experts ? (int32_t)p : ~(int32_t)p;
         pos[p] = e < n_experts ? row : ~row;
     }
     return CG3D_OK;
@@ -84,18 +85,16 @@ int cg3d_expert_plan(const void *experts, int32_t wide, int64_t n_tokens, int32_
 static int bad(int32_t dt, int32_t wt, int64_t n, int32_t k, int32_t c) {
     return !fl(dt) || !fl(wt) || n < 0 || k < 1 || c < 1 || n > 0x7fffffffll / k;
 }
-int cg3d_expert_gather(const void *x, int32_t dtype, const int32_t *pos, int64_t n_tokens, int32_t k, int32_t c, void *out,
+int cg3d_expert_gather(const void *x, int32_t dtype, const int32_t *rows, int64_t n_tokens, int32_t k, int32_t c, void *out,
                        cg3d_stream_t stream) {
     (void)stream;
     if (bad(dtype, 0, n_tokens, k, c)) return CG3D_ERR_ARG;
     if (n_tokens == 0) return CG3D_OK;
-    if (!x || !pos || !out || odd(x, dtype) || odd(out, dtype)) return CG3D_ERR_ARG;
+    if (!x || !rows || !out || odd(x, dtype) || odd(out, dtype)) return CG3D_ERR_ARG;
     const int64_t w = (int64_t)c * es(dtype), P = n_tokens * k;
-    for (int64_t p = 0; p < P; p++) {
-        const int64_t r = pos[p] < 0 ? ~pos[p] : pos[p];
-        if (r >= P) continue;
-        if (pos[p] < 0) memset((char *)out + r * w, 0, (size_t)w);
-        else memcpy((char *)out + r * w, (const char *)x + p / k * w, (size_t)w);
+    for (int64_t j = 0; j < P; j++) {
+        if (rows[j] < 0 || rows[j] >= n_tokens) memset((char *)out + j * w, 0, (size_t)w);
+        else memcpy((char *)out + j * w, (const char *)x + rows[j] * w, (size_t)w);
     }
     return CG3D_OK;
 }
@@ -116,25 +115,24 @@ int cg3d_expert_combine(const void *y, int32_t dtype, const int32_t *pos, const 
         }
     return CG3D_OK;
 }
-int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, const int32_t *pos, const void *w, int32_t wtype,
+int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, const int32_t *pairs, const void *w, int32_t wtype,
                             int64_t n_tokens, int32_t k, int32_t c, void *dy, void *dw, cg3d_stream_t stream) {
     (void)stream;
     if (bad(dtype, wtype, n_tokens, k, c) || (!dy && !dw)) return CG3D_ERR_ARG;
     if (n_tokens == 0) return CG3D_OK;
-    if (!dout || !pos || (dw && (!y || !w)) || odd(dout, dtype) || odd(y, dtype) || odd(dy, dtype) || odd(w, wtype) || odd(dw, wtype))
+    if (!dout || !pairs || (dw && (!y || !w)) || odd(dout, dtype) || odd(y, dtype) || odd(dy, dtype) || odd(w, wtype) || odd(dw, wtype))
         return CG3D_ERR_ARG;
     const int64_t P = n_tokens * k;
-    for (int64_t p = 0; p < P; p++) {
-        const int there = pos[p] >= 0 && pos[p] < P;
-        const int64_t r = pos[p] < 0 ? ~pos[p] : pos[p], t = p / k;
+    for (int64_t j = 0; j < P; j++) {
+        const int there = pairs[j] >= 0 && pairs[j] < P;
+        const int64_t p = pairs[j] < 0 ? ~pairs[j] : pairs[j], t = p / k;
         double dot = 0;
-        if (r < P)
-            for (int32_t a = 0; a < c; a++) {
-                const double g = there ? ld(dout, dtype, t * c + a) : 0;
-                if (dw && there) dot += g * ld(y, dtype, r * c + a);
-                if (dy) st(dy, dtype, r * c + a, there ? (w ? (double)ld(w, wtype, p) : 1.0) * g : 0);
-            }
-        if (dw) st(dw, wtype, p, dot);
+        for (int32_t a = 0; a < c; a++) {
+            const double g = there ? ld(dout, dtype, t * c + a) : 0;
+            if (dw && there) dot += g * ld(y, dtype, j * c + a);
+            if (dy) st(dy, dtype, j * c + a, there ? (w ? (double)ld(w, wtype, p) : 1.0) * g : 0);
+        }
+        if (dw && p < P) st(dw, wtype, p, dot);
     }
     return CG3D_OK;
 }

@@ -58,6 +58,8 @@ def check_plan(ids, n_experts):
     got = plan.pos.cpu()
     assert torch.equal(torch.where(got >= 0, got, -1), pos)
     behind = torch.sort(~got[got < 0])[0]                    # the pairs without a row own the rows behind the last, once each
+    flat, pairs = got.view(-1).long(), plan.pairs.cpu()
+    assert torch.equal(pairs[torch.where(flat >= 0, flat, ~flat)], torch.where(flat >= 0, 1, -1).int() * torch.arange(ids.numel(), dtype=torch.int32) - (flat < 0).int())
     assert torch.equal(behind, torch.arange(int(offsets[-1]), ids.numel(), dtype=torch.int32))
     return plan, offsets, rows, pos
 
@@ -166,8 +168,8 @@ def test_entry_points_refuse(oracle):
         ok = dict(p=i.data_ptr(), x=f.data_ptr())
         for bad in ((ok["p"], 2, 4, 2, 3), (ok["p"], 0, -1, 2, 3), (ok["p"], 0, 4, 0, 3), (ok["p"], 0, 4, 2, 0), (ok["p"], 0, 4, 2, 1025),
                     (ok["p"], 0, 2 ** 31, 1, 3), (None, 0, 4, 2, 3), (ok["p"] + 2, 0, 4, 2, 3), (ok["p"] + 4, 1, 4, 2, 3)):
-            assert lib.raw("cg3d_expert_plan")(*bad, ok["p"], ok["p"], ok["p"], None, None) == -1, bad
-        assert lib.raw("cg3d_expert_plan")(ok["p"], 0, 4, 2, 3, None, ok["p"], ok["p"], None, None) == -1
+            assert lib.raw("cg3d_expert_plan")(*bad, ok["p"], ok["p"], ok["p"], ok["p"], None, None) == -1, bad
+        assert lib.raw("cg3d_expert_plan")(ok["p"], 0, 4, 2, 3, None, ok["p"], ok["p"], ok["p"], None, None) == -1
         assert lib.raw("cg3d_expert_plan_ws_bytes")(2 ** 31, 1, 3) == -1
         for dt, t, k, c in ((3, 4, 2, 8), (-1, 4, 2, 8), (0, -1, 2, 8), (0, 4, 0, 8), (0, 4, 2, 0), (0, 2 ** 31, 1, 8)):
             assert lib.raw("cg3d_expert_gather")(ok["x"], dt, ok["p"], t, k, c, ok["x"], None) == -1
@@ -179,7 +181,7 @@ def test_entry_points_refuse(oracle):
         assert lib.raw("cg3d_expert_combine_bwd")(ok["x"], None, 0, ok["p"], ok["x"], 0, 4, 2, 8, ok["x"], ok["x"], None) == -1
         assert lib.raw("cg3d_expert_gather")(None, 0, ok["p"], 4, 2, 8, ok["x"], None) == -1
     if h.raw("cg3d_expert_plan_ws_bytes")(100000, 2, 18) > 0:
-        assert h.raw("cg3d_expert_plan")(i.data_ptr(), 0, 100000, 2, 18, i.data_ptr(), i.data_ptr(), i.data_ptr(), None, None) == -1
+        assert h.raw("cg3d_expert_plan")(i.data_ptr(), 0, 100000, 2, 18, i.data_ptr(), i.data_ptr(), i.data_ptr(), i.data_ptr(), None, None) == -1
 
 
 def test_no_cpu_fallback():
