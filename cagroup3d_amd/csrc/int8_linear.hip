@@ -4,8 +4,11 @@
 //   y[r, n] = (sum_k q[r, k] w[k, n]) * sx[r] * sw[n] + b[n]      the sum is exact: int32, fewer than 2^17 terms of at most 2^14
 //   sx[r]   = max_k |x[r, k]| / 127,   q[r, k] = 127 x[r, k] / max |x[r, .]| rounded to the nearest, ties to even
 //
-// The rounding of q is decided exactly, not up to the error of a reciprocal: t = x * (127 / max) in fp32 is off by less than 2^-15,
-// and where it falls within 2^-13 of a half the two sides 254 |x| and (2 n + 1) max are compared in 64 bits, where both are exact.
+// The rounding of q is decided exactly, not up to the error of a reciprocal.  With c = 127 / max rounded UP to fp32, t' = c x lies
+// between the true t and t (1 + 2^-23), so that a wrong nearest level needs t' on or just above a half (by at most 127 * 2^-23 <
+// 2^-16).  t' enters one fused multiply-add with 1.5 * 2^23 (its low byte is then the level) and is never rounded by itself; only
+// where it falls into that strip the two sides 127 |x| and (n - 1/2) max are compared, each as an fp32 product and its exact error.
+// |x| = max / 2, the one tie that rows of 16-bit floats meet all the time, needs no look: it lands on 64, the even side.
 // A row that holds an infinity or a NaN gets the scale NaN (and so a row of NaN as its result); a row of zeros the scale 0.
 //
 // The weights are the MFMA's A operand and the rows its B operand (v_mfma_i32_16x16x64_i8), i.e. a tile of the product is
@@ -15,11 +18,13 @@
 // 16 g .. 16 g + 15 of the channel (nb / 2) * 32 + (m / 4) * 8 + (nb % 2) * 4 + m % 4 of the panel, so that the results of tiles nb = 0, 1
 // (2, 3) in a lane are 8 consecutive channels.  Channels and contraction steps past the end are zeros.
 #include "cg3d_common.h"
+#pragma clang fp contract(off)      // a result has the same bits on every path
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 #define I8_MAX_CIN 131071            // 2^14 * 131071 < 2^31: -128 * -128 included
 #define I8_MAX_EXPERTS 1024
+#define I8_FUSED_CIN 512
 
 template <typename T, int V> struct __attribute__((packed, aligned(1))) i8_vec { T e[V]; };
 
@@ -30,31 +35,131 @@ static __device__ __forceinline__ float i8_f(i8_bf16 a) { return __uint_as_float
 static __device__ __forceinline__ float i8_f(i8_f16 a) { return (float)__builtin_bit_cast(_Float16, a.v); }
 static __device__ __forceinline__ uint32_t i8_abs(float f) { return __float_as_uint(f) & 0x7fffffffu; }   // ordered like |f|; infinity and NaN on top
 
-// what a row's largest magnitude (bits of |.|) makes of its elements: q = level(x), scale
+// 16 neighbouring elements of a row as they lie in memory, in whole registers (a row may start at any multiple of its element)
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+template <typename T> struct i8_raw {
+    u32x4 w[sizeof(T)];
+    __device__ __forceinline__ float operator[](int j) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[j >> 2][j & 3]);
+        else {
+            const uint32_t d = w[j >> 3][(j >> 1) & 3];
+            if constexpr (__is_same(T, i8_bf16)) return __uint_as_float(j & 1 ? d & 0xffff0000u : d << 16);
+            else return (float)__builtin_bit_cast(_Float16, (uint16_t)(j & 1 ? d >> 16 : d));
+        }
+    }
+};
+// elements k0 .. k0 + 15 of a row of cin, zeros behind its end
+template <typename T>
+static __device__ __forceinline__ i8_raw<T> i8_get16(const T *__restrict__ xr, int k0, int cin) {
+    i8_raw<T> v;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); i++) v.w[i] = u32x4{0, 0, 0, 0};
+    if (k0 + 16 <= cin) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); i++) v.w[i] = reinterpret_cast<const u32x4_any *>(xr + k0)[i];
+    } else if (k0 < cin) {
+        constexpr int PER = 4 / sizeof(T);               // elements of a register
+#pragma unroll
+        for (int j = 0; j < 15; j++)
+            if (k0 + j < cin) {
+                uint32_t d = 0;
+                __builtin_memcpy(&d, xr + k0 + j, sizeof(T));
+                v.w[j / (4 * PER)][(j / PER) & 3] |= d << (j % PER * 8 * (int)sizeof(T));
+            }
+    }
+    return v;
+}
+// the running maximum of |.|: fp32 bits, or for 16-bit floats two at a time (their bits are ordered like their magnitudes too)
+template <typename T> struct i8_max {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    uint32_t v = 0;
+    __device__ __forceinline__ void add(const i8_raw<T> &r) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if constexpr (sizeof(T) == 4) v = max(v, r.w[i][j] & 0x7fffffffu);
+                else v = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, v), __builtin_bit_cast(u16x2, r.w[i][j] & 0x7fff7fffu)));
+            }
+    }
+    __device__ __forceinline__ uint32_t bits() const {    // of the fp32 value
+        if constexpr (sizeof(T) == 4) return v;
+        else {
+            T t;
+            t.v = (uint16_t)max(v & 0xffffu, v >> 16);
+            return i8_abs(i8_f(t));
+        }
+    }
+};
+
+// What a row's largest magnitude (its bits) makes of the row's elements.  Rows whose largest is below 2^-96 or from 2^112 on are
+// shifted by a power of two first (`shift`, exact for every element that is not level 0), so that no product here leaves the range.
 struct i8_level {
-    float amax, inv, up, scale;
+    float amax, c, half, shift, scale;
+    uint32_t keep;                                       // 0: the row has no levels
     __device__ __forceinline__ explicit i8_level(uint32_t top) {
         const float a = __uint_as_float(top);
         const bool fine = top < 0x7f800000u;
-        up = a < 0x1p-96f ? 0x1p96f : 1.f;               // (an exact shift of the whole row, so that 127 / max stays finite)
-        amax = fine ? a * up : 0.f;
-        inv = amax > 0.f ? 127.f / amax : 0.f;
+        shift = a < 0x1p-96f ? 0x1p96f : fine && a >= 0x1p112f ? 0x1p-16f : 1.f;
+        keep = fine && top ? ~0u : 0u;
+        amax = keep ? a * shift : 1.f;
+        half = 0.5f * amax;
+        c = 127.f / amax;
+        if (__builtin_fmaf(c, amax, -127.f) < 0.f) c = __uint_as_float(__float_as_uint(c) + 1);
         scale = fine ? a / 127.f : __uint_as_float(0x7fc00000u);
-        if (!fine) up = 0.f;
     }
-    __device__ __forceinline__ int operator()(float x) const {
-        if (amax == 0.f) return 0;
-        const float t = x * up * inv;
-        const float n = rintf(t);
-        if (__builtin_expect(fabsf(t - n) > 0.5f - 0x1p-13f, 0)) {
-            const int lo = (int)floorf(fabsf(t));
-            const double a = fabs((double)x * (double)up) * 254.0, b = (double)(2 * lo + 1) * (double)amax;
-            const int m = a > b || (a == b && (lo & 1)) ? lo + 1 : lo;
-            return t < 0.f ? -m : m;
-        }
-        return (int)n;
-    }
+    __device__ __forceinline__ bool shifted() const { return shift != 1.f; }
 };
+#define I8_MAGIC 12582912.f          // 1.5 * 2^23
+// r = the fma's result for x whose t' is in the strip: the level one nearer to zero where that is the nearest, ties to even
+static __device__ __forceinline__ float i8_decide(const i8_level &v, float x, float r) {
+    const float n = fabsf(r - I8_MAGIC), h = n - 0.5f, ax = fabsf(x);
+    const float s = ax * 127.f, b = h * v.amax;
+    const float es = __builtin_fmaf(ax, 127.f, -s), eb = __builtin_fmaf(h, v.amax, -b);
+    const bool less = s < b || (s == b && es < eb), same = s == b && es == eb;
+    const bool down = less || (same && ((int)n & 1));
+    return down ? r - copysignf(1.f, r - I8_MAGIC) : r;
+}
+// 16 elements (shifted) of one row -> 16 levels.  SHORT: the elements were 16-bit floats
+template <bool SHORT>
+static __device__ __forceinline__ i32x4 i8_quant16(const i8_level &v, const float (&x)[16]) {
+    float r[16];
+    bool look = false;
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        r[j] = __builtin_fmaf(x[j], v.c, I8_MAGIC);
+        const float d = __builtin_fmaf(x[j], v.c, -(r[j] - I8_MAGIC));
+        look |= fabsf(d) > 0.5f - 0x1p-16f && (!SHORT || fabsf(x[j]) != v.half);
+    }
+    if (__builtin_expect(__any(look), 0)) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float n = r[j] - I8_MAGIC, d = __builtin_fmaf(x[j], v.c, -n);
+            if (d * n < 0.f && fabsf(d) > 0.5f - 0x1p-16f) r[j] = i8_decide(v, x[j], r[j]);     // (n = 0 is nearest from either side)
+        }
+    }
+    i32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(r[4 * i + 1]), __float_as_uint(r[4 * i]), 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(r[4 * i + 3]), __float_as_uint(r[4 * i + 2]), 0x04000c0cu);
+        o[i] = (int)((lo | hi) & v.keep);
+    }
+    return o;
+}
+
+template <typename T>
+static __device__ __forceinline__ i32x4 i8_levels16(const i8_level &lev, bool far, const i8_raw<T> &v) {
+    float f[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) f[j] = v[j];
+    if (far) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) f[j] *= lev.shift;
+    }
+    return i8_quant16<sizeof(T) == 2>(lev, f);
+}
 
 // ---------------------------------------------------------------- weights (once per model)
 // w [E][cin][cout]: a thread owns a channel, reads along the contraction are rows of the matrix
@@ -80,18 +185,16 @@ __global__ __launch_bounds__(256) void k_i8_weight_pack(const T *__restrict__ w,
         const int64_t u = i >> 8;
         const int c = (int)(u % chunks), p = (int)((u / chunks) % panels), e = (int)(u / chunks / panels);
         const int n = p * 64 + i8_channel(nb, lane & 15), k0 = c * 64 + (lane >> 4) * 16;
+        const bool there = n < cout;
+        const T *src = w + (int64_t)e * cin * cout + (there ? n : 0);
         union { int8_t b[16]; i32x4 v; } o;
-        o.v = i32x4{0, 0, 0, 0};
-        if (n < cout) {
-            const T *src = w + (int64_t)e * cin * cout + n;
-            if constexpr (sizeof(T) == 1) {
-                for (int j = 0; j < 16; j++)
-                    if (k0 + j < cin) o.b[j] = (int8_t)src[(int64_t)(k0 + j) * cout];
-            } else {
-                const i8_level q(top[(int64_t)e * cout + n]);
-                for (int j = 0; j < 16; j++)
-                    if (k0 + j < cin) o.b[j] = (int8_t)q(i8_f(src[(int64_t)(k0 + j) * cout]));
-            }
+        if constexpr (sizeof(T) == 1) {
+            for (int j = 0; j < 16; j++) o.b[j] = there && k0 + j < cin ? (int8_t)src[(int64_t)(k0 + j) * cout] : 0;
+        } else {
+            const i8_level lev(there ? top[(int64_t)e * cout + n] : 0);
+            float f[16];
+            for (int j = 0; j < 16; j++) f[j] = there && k0 + j < cin ? i8_f(src[(int64_t)(k0 + j) * cout]) * lev.shift : 0.f;
+            o.v = i8_quant16<sizeof(T) == 2>(lev, f);
         }
         reinterpret_cast<i32x4 *>(out)[i] = o.v;
     }
@@ -138,17 +241,6 @@ extern "C" int cg3d_int8_weight(const void *w, int32_t dtype, int32_t n_experts,
 // ---------------------------------------------------------------- rows
 // A group of L lanes (a power of two) owns one row, 16 elements of a lane at a time; the row is read a second time (from the
 // caches) for its levels.  Bytes [cin, pitch) are zeros.
-template <typename T>
-static __device__ __forceinline__ void i8_load16(const T *__restrict__ p, int left, float (&f)[16]) {   // left: elements before the row's end
-    if (left >= 16) {
-        const i8_vec<T, 16> v = *reinterpret_cast<const i8_vec<T, 16> *>(p);
-#pragma unroll
-        for (int j = 0; j < 16; j++) f[j] = i8_f(v.e[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; j++) f[j] = j < left ? i8_f(p[j]) : 0.f;
-    }
-}
 template <typename T, int B>
 __global__ __launch_bounds__(B) void k_i8_rows(const T *__restrict__ x, int64_t n, int32_t cin, int64_t pitch, int32_t lshift,
                                                int8_t *__restrict__ q, float *__restrict__ scale) {
@@ -157,13 +249,9 @@ __global__ __launch_bounds__(B) void k_i8_rows(const T *__restrict__ x, int64_t 
     const int nv = (cin + 15) >> 4;
     for (int64_t r = (blockIdx.x * (int64_t)B + threadIdx.x) >> lshift; r < n; r += ((int64_t)gridDim.x * B) >> lshift) {
         const T *row = x + r * cin;
-        uint32_t top = 0;
-        float f[16];
-        for (int v = lane; v < nv; v += L) {
-            i8_load16(row + v * 16, cin - v * 16, f);
-#pragma unroll
-            for (int j = 0; j < 16; j++) top = max(top, i8_abs(f[j]));
-        }
+        i8_max<T> most;
+        for (int v = lane; v < nv; v += L) most.add(i8_get16<T>(row, v * 16, cin));
+        uint32_t top = most.bits();
         for (int d = (L < 64 ? L : 64) >> 1; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
         if (L > 64) {                                     // (L == B: the workgroup owns the row)
             if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
@@ -176,10 +264,8 @@ __global__ __launch_bounds__(B) void k_i8_rows(const T *__restrict__ x, int64_t 
         if (lane == 0) scale[r] = lev.scale;
         int8_t *dst = q + r * pitch;
         for (int v = lane; v < nv; v += L) {
-            i8_load16(row + v * 16, cin - v * 16, f);
-            i8_vec<int8_t, 16> o;
-#pragma unroll
-            for (int j = 0; j < 16; j++) o.e[j] = (int8_t)lev(f[j]);
+            const i32x4 lv = i8_levels16<T>(lev, lev.shifted(), i8_get16<T>(row, v * 16, cin));
+            const i8_vec<int8_t, 16> o = __builtin_bit_cast(i8_vec<int8_t, 16>, lv);
             if (v * 16 + 16 <= pitch) *reinterpret_cast<i8_vec<int8_t, 16> *>(dst + v * 16) = o;
             else
                 for (int j = 0; j < 16; j++)
@@ -259,43 +345,58 @@ static int64_t i8_tiles(const i8_args &a, int bm) { return a.offsets ? a.n_rows 
 
 // a lane's results of one panel, acc[nb][i]: channels i8_channel(nb, 4 g + i) of row `row`; live = 0: rows behind the last
 static __device__ __forceinline__ void i8_store(const i8_args &a, int e, int panel, int64_t row, float sx, bool live, const i32x4 (&acc)[4]) {
+    typedef i8_vec<float, 8> f8;
+    typedef i8_vec<uint16_t, 8> h8;
     const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const int c0 = panel * 64 + h * 32 + g * 8;
-        if (c0 >= a.cout) continue;
-        const bool whole = c0 + 8 <= a.cout;
-        float v[8];
+        const int c0 = panel * 64 + h * 32 + g * 8, n = min(8, a.cout - c0);
+        if (n <= 0) continue;
+        f8 v;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int c = whole || c0 + j < a.cout ? c0 + j : a.cout - 1;
-            v[j] = 0.f;
-            if (live) {
-                v[j] = (float)acc[2 * h + (j >> 2)][j & 3] * sx * a.sw[(int64_t)e * a.cout + c];
-                if (a.bias) v[j] += a.bias[(int64_t)e * a.bias_step + c];
+        for (int j = 0; j < 8; j++) v.e[j] = 0.f;
+        if (live) {
+            const float *sw = a.sw + (int64_t)e * a.cout + c0, *bias = a.bias + (int64_t)e * a.bias_step + c0;
+            if (n == 8) {
+                const f8 s = *reinterpret_cast<const f8 *>(sw);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v.e[j] = (float)acc[2 * h + (j >> 2)][j & 3] * sx * s.e[j];
+                if (a.bias) {
+                    const f8 b = *reinterpret_cast<const f8 *>(bias);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v.e[j] += b.e[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (j < n) v.e[j] = (float)acc[2 * h + (j >> 2)][j & 3] * sx * sw[j] + (a.bias ? bias[j] : 0.f);
             }
         }
         if (a.out_dtype == CG3D_DT_F32) {
             float *y = reinterpret_cast<float *>(a.y) + row * a.cout + c0;
-            if (whole) {
-                i8_vec<float, 8> o;
-#pragma unroll
-                for (int j = 0; j < 8; j++) o.e[j] = v[j];
-                *reinterpret_cast<i8_vec<float, 8> *>(y) = o;
+            if (n == 8) {
+                struct two { u32x4 q[2]; };
+                const two o = __builtin_bit_cast(two, v);
+                __builtin_nontemporal_store(o.q[0], reinterpret_cast<u32x4_any *>(y));
+                __builtin_nontemporal_store(o.q[1], reinterpret_cast<u32x4_any *>(y + 4));
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; j++) if (c0 + j < a.cout) y[j] = v[j];
+                for (int j = 0; j < 8; j++) if (j < n) y[j] = v.e[j];
             }
         } else {
             uint16_t *y = reinterpret_cast<uint16_t *>(a.y) + row * a.cout + c0;
-            i8_vec<uint16_t, 8> o;
+            h8 o;
+            if (a.out_dtype == CG3D_DT_BF16) {
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                o.e[j] = a.out_dtype == CG3D_DT_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)v[j]) : __builtin_bit_cast(uint16_t, (_Float16)v[j]);
-            if (whole) *reinterpret_cast<i8_vec<uint16_t, 8> *>(y) = o;
+                for (int j = 0; j < 8; j++) o.e[j] = __builtin_bit_cast(uint16_t, (__bf16)v.e[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) o.e[j] = __builtin_bit_cast(uint16_t, (_Float16)v.e[j]);
+            }
+            if (n == 8) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o), reinterpret_cast<u32x4_any *>(y));
             else {
 #pragma unroll
-                for (int j = 0; j < 8; j++) if (c0 + j < a.cout) y[j] = o.e[j];
+                for (int j = 0; j < 8; j++) if (j < n) y[j] = o.e[j];
             }
         }
     }
@@ -303,13 +404,6 @@ static __device__ __forceinline__ void i8_store(const i8_args &a, int e, int pan
 
 // The plainest form: a wave owns 16 rows x 64 channels, operands straight from memory (the fragments of the weights are whole
 // kilobytes, a row's 64 bytes of a chunk belong to four lanes).
-static __device__ __forceinline__ i32x4 i8_row16(const int8_t *__restrict__ p, int left) {
-    if (left >= 16) return __builtin_bit_cast(i32x4, *reinterpret_cast<const i8_vec<int8_t, 16> *>(p));
-    i8_vec<int8_t, 16> o;
-#pragma unroll
-    for (int j = 0; j < 16; j++) o.e[j] = j < left ? p[j] : 0;
-    return __builtin_bit_cast(i32x4, o);
-}
 __global__ __launch_bounds__(256) void k_i8_wave(i8_args a, const int8_t *__restrict__ q, int64_t pitch) {
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int panels = (a.cout + 63) >> 6, chunks = (a.cin + 63) >> 6;
@@ -333,7 +427,7 @@ __global__ __launch_bounds__(256) void k_i8_wave(i8_args a, const int8_t *__rest
         const i32x4 *wf = reinterpret_cast<const i32x4 *>(a.w) + ((int64_t)e * panels + panel) * chunks * 256 + lane;
         for (int c = 0; c < chunks; c++) {
             const int k0 = c * 64 + g * 16;
-            const i32x4 b = k0 < a.cin ? i8_row16(xr + k0, a.cin - k0) : i32x4{0, 0, 0, 0};
+            const i32x4 b = __builtin_bit_cast(i32x4, i8_get16<int8_t>(xr, k0, a.cin).w[0]);
 #pragma unroll
             for (int nb = 0; nb < 4; nb++) acc[nb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[(int64_t)(c * 4 + nb) * 64], b, acc[nb], 0, 0, 0);
         }
@@ -341,12 +435,110 @@ __global__ __launch_bounds__(256) void k_i8_wave(i8_args a, const int8_t *__rest
     if (mine) i8_store(a, e, panel, row0 + m, sx, live, acc);
 }
 
+static __device__ __forceinline__ int64_t i8_source(const i8_args &a, int64_t row) {
+    int64_t src = a.rows ? (int64_t)a.rows[row] : row;
+    return (uint64_t)src < (uint64_t)a.n_x ? src : 0;
+}
+
+// Rows of at most I8_FUSED_CIN columns: one pass over them.  A workgroup of 4 waves owns 64 rows; each wave brings 16 of them in, in the
+// layout of the MFMA's B operand -- lane (g, m) has elements 64 c + 16 g .. + 15 of row m for every chunk c -- so that a row's maximum
+// is a maximum over the lane and two exchanges, and the levels go to LDS as whole fragments (contiguous, no conflicts).  Then wave
+// (wm, wn) multiplies RG of the 4 row groups by panels wn, wn + RG, ... of the part blockIdx.y of the channels: the weights stream
+// past from the caches one chunk ahead, every fragment used RG times.  RG = 4 / 2 / 1 for at least 4 / 2 / 1 panels a part.
+template <typename T, int RG>
+__global__ __launch_bounds__(256, 4) void k_i8_fused(i8_args a, const T *__restrict__ x) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t i8_sm[];
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int panels = (a.cout + 63) >> 6, chunks = (a.cin + 63) >> 6;
+    const int p_lo = (int)((int64_t)panels * blockIdx.y / gridDim.y), p_hi = (int)((int64_t)panels * (blockIdx.y + 1) / gridDim.y);
+    i32x4 *const frag = reinterpret_cast<i32x4 *>(i8_sm);                          // [4 groups][chunks][64 lanes]
+    float *const scales = reinterpret_cast<float *>(i8_sm + chunks * 4096);        // [64]
+    int e, rows;
+    int64_t row0;
+    if (!i8_tile<64>(a, blockIdx.x, e, row0, rows)) return;                        // (the whole workgroup)
+    const bool live = e < a.n_experts;
+    if (live && wave * 16 < rows) {
+        const int64_t src = i8_source(a, row0 + min(wave * 16 + m, rows - 1));
+        const T *xr = x + src * a.cin;
+        i32x4 *const mine = frag + wave * chunks * 64 + lane;
+        if constexpr (sizeof(T) == 1) {
+            if (g == 0) scales[wave * 16 + m] = a.sx[src];
+#pragma unroll 8
+            for (int c = 0; c < chunks; c++) mine[c * 64] = __builtin_bit_cast(i32x4, i8_get16<T>(xr, c * 64 + g * 16, a.cin).w[0]);
+        } else {
+            constexpr int KEEP = sizeof(T) == 2 ? 8 : 4;                           // chunks held in registers (64 of them)
+            i8_raw<T> v[KEEP];
+            i8_max<T> most;
+            for (int c0 = 0; c0 < chunks; c0 += KEEP) {
+#pragma unroll
+                for (int c = 0; c < KEEP; c++)
+                    if (c0 + c < chunks) v[c] = i8_get16<T>(xr, (c0 + c) * 64 + g * 16, a.cin);
+#pragma unroll
+                for (int c = 0; c < KEEP; c++)
+                    if (c0 + c < chunks) most.add(v[c]);
+            }
+            uint32_t top = most.bits();
+            top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+            top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+            const i8_level lev(top);
+            const bool far = __any(lev.shifted());
+            if (g == 0) scales[wave * 16 + m] = lev.scale;
+            for (int c0 = 0; c0 < chunks; c0 += KEEP) {
+                if (chunks > KEEP) {                                               // (longer rows are read again, from the caches)
+#pragma unroll
+                    for (int c = 0; c < KEEP; c++)
+                        if (c0 + c < chunks) v[c] = i8_get16<T>(xr, (c0 + c) * 64 + g * 16, a.cin);
+                }
+#pragma unroll
+                for (int c = 0; c < KEEP; c++)
+                    if (c0 + c < chunks) mine[(c0 + c) * 64] = i8_levels16<T>(lev, far, v[c]);
+            }
+        }
+    }
+    __syncthreads();
+    const int wn = wave % RG, wm = wave / RG;
+    if (wm * RG * 16 >= rows) return;
+    const i32x4 *const bq = frag + wm * RG * chunks * 64 + lane;
+    for (int p = p_lo + wn; p < p_hi; p += RG) {
+        i32x4 acc[RG][4];
+#pragma unroll
+        for (int h = 0; h < RG; h++)
+#pragma unroll
+            for (int nb = 0; nb < 4; nb++) acc[h][nb] = i32x4{0, 0, 0, 0};
+        if (live) {
+            const i32x4 *wf = reinterpret_cast<const i32x4 *>(a.w) + ((int64_t)e * panels + p) * (chunks * 256) + lane;
+            i32x4 cur[4];
+#pragma unroll
+            for (int nb = 0; nb < 4; nb++) cur[nb] = wf[nb * 64];
+            for (int c = 0; c < chunks; c++) {
+                i32x4 nxt[4];
+                wf += c + 1 < chunks ? 256 : 0;
+#pragma unroll
+                for (int nb = 0; nb < 4; nb++) nxt[nb] = wf[nb * 64];
+#pragma unroll
+                for (int h = 0; h < RG; h++) {
+                    const i32x4 q = bq[(h * chunks + c) * 64];                     // (a group without rows: old bytes, never stored)
+#pragma unroll
+                    for (int nb = 0; nb < 4; nb++) acc[h][nb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur[nb], q, acc[h][nb], 0, 0, 0);
+                }
+#pragma unroll
+                for (int nb = 0; nb < 4; nb++) cur[nb] = nxt[nb];
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < RG; h++) {
+            const int r = (wm * RG + h) * 16 + m;
+            if (r < rows) i8_store(a, e, p, row0 + r, scales[r], live, acc[h]);
+        }
+    }
+}
+
 static int64_t i8_pitch(int32_t cin) { return i8_chunks(cin) * 64; }
 extern "C" int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts) {
     if (dtype < CG3D_DT_F32 || dtype > CG3D_DT_I8 || i8_bad_shape(n_experts, cin, cout) || n_x < 0 || n_x > 0x7fffffffll || n_rows < 0 ||
         n_rows > 0x7fffffffll)
         return CG3D_ERR_ARG;
-    return dtype == CG3D_DT_I8 ? 0 : ((n_x * 4 + 255) & ~255ll) + n_x * i8_pitch(cin);
+    return dtype == CG3D_DT_I8 || cin <= I8_FUSED_CIN ? 0 : ((n_x * 4 + 255) & ~255ll) + n_x * i8_pitch(cin);
 }
 extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, int64_t n_x, int32_t cin, const int8_t *w, const float *sw,
                                 const float *bias, int32_t bias_per_expert, const int32_t *offsets, const int32_t *rows, void *y,
@@ -361,6 +553,29 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
         return CG3D_ERR_ARG;
     hipStream_t s = cg3d_hs(stream);
     i8_args a = {sx, w, sw, bias, offsets, rows, y, n_rows, n_x, cin, cout, n_experts, out_dtype, bias_per_expert ? cout : 0};
+    if (cin <= I8_FUSED_CIN) {
+        // enough workgroups for the chip: the panels of a row tile are shared out where there are fewer than 1024 tiles
+        const int64_t tiles = i8_tiles(a, 64), panels = i8_panels(cout);
+        const int32_t parts = (int32_t)(cg3d_divup(1024, tiles) < panels ? cg3d_divup(1024, tiles) : panels);
+        const int32_t each = (int32_t)cg3d_divup(panels, parts);
+        const int lds = (int)i8_chunks(cin) * 4096 + 256;
+        if (tiles > (1ll << 23)) return CG3D_ERR_ARG;
+#define I8_F(T, RG)                                                                                                                 \
+    do {                                                                                                                            \
+        if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(&k_i8_fused<T, RG>), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) \
+            return CG3D_ERR_LAUNCH;                                                                                                 \
+        hipLaunchKernelGGL((k_i8_fused<T, RG>), dim3((unsigned)tiles, (unsigned)parts), dim3(256), lds, s, a, reinterpret_cast<const T *>(x)); \
+    } while (0)
+#define I8_FC(T) do { if (each >= 4) I8_F(T, 4); else if (each >= 2) I8_F(T, 2); else I8_F(T, 1); } while (0)
+        if (dtype == CG3D_DT_F32) I8_FC(float);
+        else if (dtype == CG3D_DT_BF16) I8_FC(i8_bf16);
+        else if (dtype == CG3D_DT_F16) I8_FC(i8_f16);
+        else I8_FC(int8_t);
+#undef I8_FC
+#undef I8_F
+        CG3D_CHECK_LAUNCH();
+        return CG3D_OK;
+    }
     const int8_t *q = reinterpret_cast<const int8_t *>(x);
     int64_t pitch = cin;
     if (dtype != CG3D_DT_I8) {
