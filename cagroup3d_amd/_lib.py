@@ -106,7 +106,7 @@ _SIGNATURES = {
     "cg3d_int8_weight_bytes": (c_int64, [c_int32, c_int32, c_int32]),
     "cg3d_int8_weight": (c_int32, [P, c_int32, c_int32, c_int32, c_int32, P, P, P, P]),
     "cg3d_int8_quantize_rows": (c_int32, [P, c_int32, c_int64, c_int32, c_int64, P, P, P]),
-    "cg3d_int8_linear_ws_bytes": (c_int64, [c_int32, c_int64, c_int32, c_int64, c_int32, c_int32]),
+    "cg3d_int8_linear_ws_bytes": (c_int64, [c_int32, c_int64, c_int32, c_int64, c_int32, c_int32, c_int32]),
     "cg3d_int8_linear": (c_int32, [P, c_int32, P, c_int64, c_int32, P, P, P, c_int32, P, P, P, c_int32, c_int64, c_int32, c_int32, P, P]),
     # include/cagroup3d_stages.h
     "cg3d_roi_match": (c_int32, [P, P, P, c_int32, c_int32, c_float, P, c_int32, c_int32, P, P, P, P]),

@@ -343,100 +343,71 @@ static __device__ __forceinline__ bool i8_tile(const i8_args &a, int64_t u, int 
 }
 static int64_t i8_tiles(const i8_args &a, int bm) { return a.offsets ? a.n_rows / bm + a.n_experts + 1 : cg3d_divup(a.n_rows, bm); }
 
-// a lane's results of one panel, acc[nb][i]: channels i8_channel(nb, 4 g + i) of row `row`; live = 0: rows behind the last
-static __device__ __forceinline__ void i8_store(const i8_args &a, int e, int panel, int64_t row, float sx, bool live, const i32x4 (&acc)[4]) {
+// a lane's 8 neighbouring results c0 .. c0 + 7 of one row; live = 0: a row behind the last
+static __device__ __forceinline__ void i8_store8(const i8_args &a, int e, int c0, int64_t row, float sx, bool live, const i32x4 &lo, const i32x4 &hi) {
     typedef i8_vec<float, 8> f8;
     typedef i8_vec<uint16_t, 8> h8;
-    const int g = (threadIdx.x & 63) >> 4;
+    const int n = min(8, a.cout - c0);
+    if (n <= 0) return;
+    f8 v;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int c0 = panel * 64 + h * 32 + g * 8, n = min(8, a.cout - c0);
-        if (n <= 0) continue;
-        f8 v;
+    for (int j = 0; j < 8; j++) v.e[j] = 0.f;
+    if (live) {
+        const float *sw = a.sw + (int64_t)e * a.cout + c0, *bias = a.bias + (int64_t)e * a.bias_step + c0;
+        if (n == 8) {
+            const f8 s = *reinterpret_cast<const f8 *>(sw);
 #pragma unroll
-        for (int j = 0; j < 8; j++) v.e[j] = 0.f;
-        if (live) {
-            const float *sw = a.sw + (int64_t)e * a.cout + c0, *bias = a.bias + (int64_t)e * a.bias_step + c0;
-            if (n == 8) {
-                const f8 s = *reinterpret_cast<const f8 *>(sw);
+            for (int j = 0; j < 8; j++) v.e[j] = (float)(j < 4 ? lo[j & 3] : hi[j & 3]) * sx * s.e[j];
+            if (a.bias) {
+                const f8 b = *reinterpret_cast<const f8 *>(bias);
 #pragma unroll
-                for (int j = 0; j < 8; j++) v.e[j] = (float)acc[2 * h + (j >> 2)][j & 3] * sx * s.e[j];
-                if (a.bias) {
-                    const f8 b = *reinterpret_cast<const f8 *>(bias);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v.e[j] += b.e[j];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (j < n) v.e[j] = (float)acc[2 * h + (j >> 2)][j & 3] * sx * sw[j] + (a.bias ? bias[j] : 0.f);
-            }
-        }
-        if (a.out_dtype == CG3D_DT_F32) {
-            float *y = reinterpret_cast<float *>(a.y) + row * a.cout + c0;
-            if (n == 8) {
-                struct two { u32x4 q[2]; };
-                const two o = __builtin_bit_cast(two, v);
-                __builtin_nontemporal_store(o.q[0], reinterpret_cast<u32x4_any *>(y));
-                __builtin_nontemporal_store(o.q[1], reinterpret_cast<u32x4_any *>(y + 4));
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) if (j < n) y[j] = v.e[j];
+                for (int j = 0; j < 8; j++) v.e[j] += b.e[j];
             }
         } else {
-            uint16_t *y = reinterpret_cast<uint16_t *>(a.y) + row * a.cout + c0;
-            h8 o;
-            if (a.out_dtype == CG3D_DT_BF16) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) o.e[j] = __builtin_bit_cast(uint16_t, (__bf16)v.e[j]);
-            } else {
+            for (int j = 0; j < 8; j++)
+                if (j < n) {
+                    v.e[j] = (float)(j < 4 ? lo[j & 3] : hi[j & 3]) * sx * sw[j];
+                    if (a.bias) v.e[j] += bias[j];
+                }
+        }
+    }
+    if (a.out_dtype == CG3D_DT_F32) {
+        float *y = reinterpret_cast<float *>(a.y) + row * a.cout + c0;
+        if (n == 8) {
+            struct two { u32x4 q[2]; };
+            const two o = __builtin_bit_cast(two, v);
+            __builtin_nontemporal_store(o.q[0], reinterpret_cast<u32x4_any *>(y));
+            __builtin_nontemporal_store(o.q[1], reinterpret_cast<u32x4_any *>(y + 4));
+        } else {
 #pragma unroll
-                for (int j = 0; j < 8; j++) o.e[j] = __builtin_bit_cast(uint16_t, (_Float16)v.e[j]);
-            }
-            if (n == 8) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o), reinterpret_cast<u32x4_any *>(y));
-            else {
+            for (int j = 0; j < 8; j++) if (j < n) y[j] = v.e[j];
+        }
+    } else {
+        uint16_t *y = reinterpret_cast<uint16_t *>(a.y) + row * a.cout + c0;
+        h8 o;
+        if (a.out_dtype == CG3D_DT_BF16) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) if (j < n) y[j] = o.e[j];
-            }
+            for (int j = 0; j < 8; j++) o.e[j] = __builtin_bit_cast(uint16_t, (__bf16)v.e[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) o.e[j] = __builtin_bit_cast(uint16_t, (_Float16)v.e[j]);
+        }
+        if (n == 8) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o), reinterpret_cast<u32x4_any *>(y));
+        else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) if (j < n) y[j] = o.e[j];
         }
     }
 }
-
-// The plainest form: a wave owns 16 rows x 64 channels, operands straight from memory (the fragments of the weights are whole
-// kilobytes, a row's 64 bytes of a chunk belong to four lanes).
-__global__ __launch_bounds__(256) void k_i8_wave(i8_args a, const int8_t *__restrict__ q, int64_t pitch) {
-    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-    const int panels = (a.cout + 63) >> 6, chunks = (a.cin + 63) >> 6;
-    const int64_t u = blockIdx.x * 4ll + (threadIdx.x >> 6);
-    const int panel = (int)(u % panels);
-    int e, rows;
-    int64_t row0;
-    if (!i8_tile<16>(a, u / panels, e, row0, rows)) return;
-    const bool live = e < a.n_experts;
-    const bool mine = m < rows;
-    i32x4 acc[4];
-#pragma unroll
-    for (int nb = 0; nb < 4; nb++) acc[nb] = i32x4{0, 0, 0, 0};
-    float sx = 0.f;
-    if (live) {
-        int64_t src = row0 + (mine ? m : 0);
-        if (a.rows) src = a.rows[src];
-        if ((uint64_t)src >= (uint64_t)a.n_x) src = 0;
-        sx = a.sx[src];
-        const int8_t *xr = q + src * pitch;
-        const i32x4 *wf = reinterpret_cast<const i32x4 *>(a.w) + ((int64_t)e * panels + panel) * chunks * 256 + lane;
-        for (int c = 0; c < chunks; c++) {
-            const int k0 = c * 64 + g * 16;
-            const i32x4 b = __builtin_bit_cast(i32x4, i8_get16<int8_t>(xr, k0, a.cin).w[0]);
-#pragma unroll
-            for (int nb = 0; nb < 4; nb++) acc[nb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[(int64_t)(c * 4 + nb) * 64], b, acc[nb], 0, 0, 0);
-        }
-    }
-    if (mine) i8_store(a, e, panel, row0 + m, sx, live, acc);
+// a lane's results of one panel, acc[nb][i]: channels i8_channel(nb, 4 g + i)
+static __device__ __forceinline__ void i8_store(const i8_args &a, int e, int panel, int64_t row, float sx, bool live, const i32x4 (&acc)[4]) {
+    const int c0 = panel * 64 + ((threadIdx.x & 63) >> 4) * 8;
+    i8_store8(a, e, c0, row, sx, live, acc[0], acc[1]);
+    i8_store8(a, e, c0 + 32, row, sx, live, acc[2], acc[3]);
 }
-
 static __device__ __forceinline__ int64_t i8_source(const i8_args &a, int64_t row) {
-    int64_t src = a.rows ? (int64_t)a.rows[row] : row;
+    const int64_t src = a.rows ? (int64_t)a.rows[row] : row;
     return (uint64_t)src < (uint64_t)a.n_x ? src : 0;
 }
 
@@ -533,39 +504,332 @@ __global__ __launch_bounds__(256, 4) void k_i8_fused(i8_args a, const T *__restr
     }
 }
 
+// Few rows: a workgroup of 8 waves owns 16 rows x 32 channels and its waves share the contraction (chunk c belongs to wave c % 8), so
+// that every weight is read once, by loads that are all under way before the rows are even looked at.  Rows in floats that fit
+// (I8_FEW chunks of a wave) are quantised here -- each workgroup finds the rows' maxima for itself, through LDS; the waves' sums are
+// joined there too.  grid: (16-row tiles, 32-channel halves of panels).
+template <typename T> struct i8_few { static constexpr int CHUNKS = sizeof(T) == 4 ? 4 : 8; };
+template <typename T>
+__global__ __launch_bounds__(512, 2) void k_i8_few(i8_args a, const T *__restrict__ x, int64_t pitch) {
+    __shared__ i32x4 part[8][2][64];
+    __shared__ uint32_t tops[8][16];
+    constexpr int KEEP = i8_few<T>::CHUNKS;
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int panels = (a.cout + 63) >> 6, chunks = (a.cin + 63) >> 6, panel = blockIdx.y >> 1, half = blockIdx.y & 1;
+    int e, rows;
+    int64_t row0;
+    if (!i8_tile<16>(a, blockIdx.x, e, row0, rows)) return;      // (the whole workgroup)
+    const bool live = e < a.n_experts;
+    const int64_t src = live ? i8_source(a, row0 + min(m, rows - 1)) : 0;
+    const T *xr = x + src * pitch;
+    const i32x4 *wf = reinterpret_cast<const i32x4 *>(a.w) + (((int64_t)(live ? e : 0) * panels + panel) * chunks * 4 + half * 2) * 64 + lane;
+    i32x4 acc[2] = {i32x4{0, 0, 0, 0}, i32x4{0, 0, 0, 0}};
+    float sx = 0.f;
+    if (live) {
+        if constexpr (sizeof(T) == 1) sx = a.sx[src];
+        for (int c0 = 0; c0 < chunks; c0 += 8 * KEEP) {          // (rows in floats: once)
+            i32x4 w[KEEP][2];
+            i8_raw<T> v[KEEP];
+#pragma unroll
+            for (int i = 0; i < KEEP; i++) {
+                const int c = c0 + i * 8 + wave;
+                if (c < chunks) {
+                    v[i] = i8_get16<T>(xr, c * 64 + g * 16, a.cin);
+                    w[i][0] = wf[(int64_t)c * 256];
+                    w[i][1] = wf[(int64_t)c * 256 + 64];
+                }
+            }
+            i8_level lev(0);
+            bool far = false;
+            if constexpr (sizeof(T) != 1) {
+                i8_max<T> most;
+#pragma unroll
+                for (int i = 0; i < KEEP; i++)
+                    if (i * 8 + wave < chunks) most.add(v[i]);
+                uint32_t top = most.bits();
+                top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+                top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+                if (g == 0) tops[wave][m] = top;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = max(top, tops[i][m]);
+                lev = i8_level(top);
+                far = __any(lev.shifted());
+                sx = lev.scale;
+            }
+#pragma unroll
+            for (int i = 0; i < KEEP; i++)
+                if (c0 + i * 8 + wave < chunks) {
+                    i32x4 q;
+                    if constexpr (sizeof(T) == 1) q = __builtin_bit_cast(i32x4, v[i].w[0]);
+                    else q = i8_levels16<T>(lev, far, v[i]);
+                    acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i][0], q, acc[0], 0, 0, 0);
+                    acc[1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i][1], q, acc[1], 0, 0, 0);
+                }
+        }
+    }
+    part[wave][0][lane] = acc[0];
+    part[wave][1][lane] = acc[1];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        acc[0] += part[i][0][lane];
+        acc[1] += part[i][1][lane];
+    }
+    if (m < rows) i8_store8(a, e, panel * 64 + half * 32 + g * 8, row0 + m, sx, live, acc[0], acc[1]);
+}
+
+// Many rows and a long contraction, rows in 8 bits (pitch and address multiples of 16): tiles of WR * RG * 16 rows x WC * 64 channels
+// of WR * WC waves.  Both operands reach LDS by direct loads, three chunks of 64 contraction steps ahead of their use; a wave's
+// fragments of the next chunk are read from LDS while it multiplies those of this one.  The weights' fragments are whole kilobytes
+// in memory and in LDS.  16 rows' pieces of a chunk are another, piece p of row r in place r * 4 + (p ^ (r / 4)): four lanes fetch a
+// row's 64 bytes and the reads of a fragment touch every bank once.  blockIdx.z: a range of chunks; with more than one the sums go to
+// `part` (one i32x4 of a lane after the other, as the tile holds them) and k_i8_join adds them up.
+// The direct loads and their waits are written out, since the compiler waits for ALL of them before any read of LDS: a wave has
+// issued the NL loads of each chunk in order, so vmcnt(NL) leaves only the newest chunk's in flight.
+// 16 bytes of each lane to lds + 16 lane.  (M0 holds the address; the compiler uses it for nothing in a kernel without other such loads.)
+static __device__ __forceinline__ void i8_dma(const void *src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"((uint64_t)(uintptr_t)src), "s"(lds) : "memory");
+}
+template <int RG, int WR, int WC>
+__global__ __launch_bounds__(WR * WC * 64, 2) void k_i8_tile(i8_args a, const int8_t *__restrict__ q, int64_t pitch, int32_t ny, i32x4 *__restrict__ part) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t i8_sm[];
+    constexpr int NW = WR * WC, BM = WR * RG * 16, NA = WC * 4, NB = WR * RG, NL = (NA + NB) / NW, STAGE = (NA + NB) * 1024, NBUF = 4;
+    static_assert((NA + NB) % NW == 0 && NA % NL == 0, "a wave's loads are of one operand");
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave % WR, wc = wave / WR;
+    const int panels = (a.cout + 63) >> 6, chunks = (a.cin + 63) >> 6;
+    // tiles of one XCD (workgroup index mod 8) are neighbours: they share rows and weights in its L2
+    const int total = gridDim.x, per = total >> 3, left = total & 7, xcd = blockIdx.x & 7;
+    const int id = xcd * per + min(xcd, left) + (blockIdx.x >> 3);
+    const int by = id % ny;
+    int e, rows;
+    int64_t row0;
+    if (!i8_tile<BM>(a, id / ny, e, row0, rows)) return;            // (the whole workgroup)
+    const bool live = e < a.n_experts;
+    const int c_lo = (int)((int64_t)chunks * blockIdx.z / gridDim.z), nc = (int)((int64_t)chunks * (blockIdx.z + 1) / gridDim.z) - c_lo;
+    i32x4 acc[RG][4];
+#pragma unroll
+    for (int h = 0; h < RG; h++)
+#pragma unroll
+        for (int nb = 0; nb < 4; nb++) acc[h][nb] = i32x4{0, 0, 0, 0};
+    if (live && nc > 0) {
+        // this wave's loads of a chunk: fragments [wave * NL, + NL) of the stage, the weights' first
+        const uint8_t *src[NL];
+        const bool of_a = wave * NL < NA;
+        const int piece = (lane & 3) ^ (lane >> 4);
+        const int last = (int)((a.cin + 15) & ~15) - 16;            // (no piece starts behind this one; what is read twice meets zeros)
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int f = wave * NL + i;
+            if (of_a) {
+                const int panel = min(by * WC + (f >> 2), panels - 1);
+                src[i] = reinterpret_cast<const uint8_t *>(a.w) + ((((int64_t)e * panels + panel) * chunks + c_lo) * 4 + (f & 3)) * 1024 + lane * 16;
+            } else {
+                const int r = (f - NA) * 16 + (lane >> 2);
+                src[i] = reinterpret_cast<const uint8_t *>(q) + i8_source(a, row0 + min(r, rows - 1)) * pitch;
+            }
+        }
+        const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)i8_sm;
+        // chunk min(k, nc - 1) into buffer k % NBUF: three more chunks are always under way than have been multiplied, past the end
+        // the last one again, into a buffer that nobody reads
+        auto issue = [&](int k) {
+            const uint32_t to = base + (uint32_t)(k % NBUF) * STAGE + wave * NL * 1024;
+            const int c = min(k, nc - 1);
+#pragma unroll
+            for (int i = 0; i < NL; i++)
+                i8_dma(of_a ? src[i] + (int64_t)c * 4096 : src[i] + min((c_lo + c) * 64 + piece * 16, last), to + i * 1024);
+        };
+        const uint8_t *const la = i8_sm + wc * 4096 + lane * 16, *const lb = i8_sm + NA * 1024 + wr * RG * 1024 + m * 64 + ((g ^ (m >> 2)) << 4);
+        i32x4 fa[2][4], fb[2][RG];
+        auto fetch = [&](int k, i32x4 (&A)[4], i32x4 (&B)[RG]) {
+            const int at = (k % NBUF) * STAGE;
+#pragma unroll
+            for (int nb = 0; nb < 4; nb++) A[nb] = *reinterpret_cast<const i32x4 *>(la + at + nb * 1024);
+#pragma unroll
+            for (int h = 0; h < RG; h++) B[h] = *reinterpret_cast<const i32x4 *>(lb + at + h * 1024);
+        };
+        auto multiply = [&](const i32x4 (&A)[4], const i32x4 (&B)[RG]) {
+#pragma unroll
+            for (int h = 0; h < RG; h++)
+#pragma unroll
+                for (int nb = 0; nb < 4; nb++) acc[h][nb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[nb], B[h], acc[h][nb], 0, 0, 0);
+        };
+        auto step = [&](int k, i32x4 (&A)[4], i32x4 (&B)[RG], i32x4 (&nA)[4], i32x4 (&nB)[RG]) {
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(NL) : "memory");      // chunk k + 1 is in LDS, for every wave
+            fetch(k + 1, nA, nB);
+            issue(k + 3);                                           // (its buffer held chunk k - 1: read by every wave before this barrier)
+            multiply(A, B);
+        };
+        issue(0);
+        issue(1);
+        issue(2);
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"(2 * NL) : "memory");
+        fetch(0, fa[0], fb[0]);
+        for (int k = 0; k < nc; k += 2) {
+            step(k, fa[0], fb[0], fa[1], fb[1]);
+            if (k + 1 < nc) step(k + 1, fa[1], fb[1], fa[0], fb[0]);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");          // (nothing may land in LDS after the workgroup has ended)
+    }
+    if (gridDim.z > 1) {
+        i32x4 *to = part + ((((int64_t)blockIdx.z * total + id) * NW + wave) * (RG * 4)) * 64 + lane;
+#pragma unroll
+        for (int h = 0; h < RG; h++)
+#pragma unroll
+            for (int nb = 0; nb < 4; nb++) to[(h * 4 + nb) * 64] = acc[h][nb];
+        return;
+    }
+    const int panel = by * WC + wc;
+    if (panel >= panels) return;
+#pragma unroll
+    for (int h = 0; h < RG; h++) {
+        const int r = (wr * RG + h) * 16 + m;
+        if (r < rows) i8_store(a, e, panel, row0 + r, live ? a.sx[i8_source(a, row0 + r)] : 0.f, live, acc[h]);
+    }
+}
+// the sums of a tile's ranges of chunks: a wave owns 16 rows x 64 channels of it
+template <int RG, int WR, int WC>
+__global__ __launch_bounds__(256) void k_i8_join(i8_args a, int32_t ny, int32_t total, int32_t splits, const i32x4 *__restrict__ part) {
+    constexpr int NW = WR * WC, BM = WR * RG * 16;
+    const int lane = threadIdx.x & 63, m = lane & 15;
+    const int64_t u = blockIdx.x * 4ll + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = (int)(u % RG), wave = (int)(u / RG % NW), id = (int)(u / (RG * NW));
+    if (id >= total) return;
+    int e, rows;
+    int64_t row0;
+    if (!i8_tile<BM>(a, id / ny, e, row0, rows)) return;
+    const bool live = e < a.n_experts;
+    const int wr = wave % WR, wc = wave / WR, panel = id % ny * WC + wc, r = (wr * RG + h) * 16 + m;
+    if (panel >= (a.cout + 63) >> 6 || (wr * RG + h) * 16 >= rows) return;
+    i32x4 acc[4];
+#pragma unroll
+    for (int nb = 0; nb < 4; nb++) acc[nb] = i32x4{0, 0, 0, 0};
+    const i32x4 *from = part + (((int64_t)id * NW + wave) * (RG * 4) + h * 4) * 64 + lane;
+    const int64_t next = (int64_t)total * NW * (RG * 4) * 64;
+#pragma unroll 4
+    for (int z = 0; z < splits; z++, from += next)
+#pragma unroll
+        for (int nb = 0; nb < 4; nb++) acc[nb] += from[nb * 64];
+    if (r < rows) i8_store(a, e, panel, row0 + r, live ? a.sx[i8_source(a, row0 + r)] : 0.f, live, acc);
+}
+
+// rows of 8 bits whose pitch or address 16 does not divide: a copy with pitch i8_pitch
+__global__ __launch_bounds__(256) void k_i8_pad(const int8_t *__restrict__ x, int64_t n, int32_t cin, int64_t pitch, int8_t *__restrict__ out) {
+    const int nv = (int)(pitch >> 4);
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n * nv; i += gridDim.x * 256ll) {
+        const int64_t r = i / nv;
+        const int k0 = (int)(i - r * nv) * 16;
+        *reinterpret_cast<u32x4 *>(out + r * pitch + k0) = i8_get16<int8_t>(x + r * cin, k0, cin).w[0];
+    }
+}
+
+// ---------------------------------------------------------------- which kernel
+struct i8_plan {
+    enum { FUSED, FEW, TILE } kind;
+    bool big;                        // TILE: 256 x 256 tiles, else 128 x 128
+    bool rows8;                      // the rows are in 8 bits, in the workspace
+    int32_t ny, splits;              // TILE: tiles along the channels, ranges of the contraction
+    int64_t tiles, scale_at, part_at, bytes;
+};
 static int64_t i8_pitch(int32_t cin) { return i8_chunks(cin) * 64; }
-extern "C" int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts) {
+static i8_plan i8_choose(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts, bool grouped, bool padded) {
+    i8_plan p = {};
+    const int64_t chunks = i8_chunks(cin), panels = i8_panels(cout);
+    auto tiles = [&](int bm) { return grouped ? n_rows / bm + n_experts + 1 : cg3d_divup(n_rows, bm); };
+    const int64_t each = grouped ? n_rows / n_experts : n_rows;      // rows of a matrix, about
+    if (each <= 32) {
+        p.kind = i8_plan::FEW;
+        p.tiles = tiles(16);
+        p.rows8 = dtype != CG3D_DT_I8 && chunks > 8 * (dtype == CG3D_DT_F32 ? i8_few<float>::CHUNKS : i8_few<i8_bf16>::CHUNKS);
+    } else if (cin <= I8_FUSED_CIN) {
+        p.kind = i8_plan::FUSED;
+        p.tiles = tiles(64);
+    } else {
+        p.kind = i8_plan::TILE;
+        p.rows8 = dtype != CG3D_DT_I8 || padded;
+        p.big = tiles(256) * cg3d_divup(panels, 4) >= 200;
+        p.ny = (int32_t)cg3d_divup(panels, p.big ? 4 : 2);
+        p.tiles = tiles(p.big ? 256 : 128);
+        const int64_t total = p.tiles * p.ny;
+        p.splits = 1;
+        if (!p.big && total < 256) {                                 // half the chip's places empty: the contraction is shared out
+            const int64_t want = cg3d_divup(512, total), most = chunks / 8;
+            p.splits = (int32_t)(want < most ? want : most > 1 ? most : 1);
+        }
+    }
+    int64_t at = 0;
+    if (p.rows8) {
+        p.scale_at = n_x * i8_pitch(cin);
+        at = p.scale_at + ((n_x * 4 + 255) & ~255ll);
+    }
+    if (p.kind == i8_plan::TILE && p.splits > 1) {
+        p.part_at = at;
+        at += p.splits * p.tiles * p.ny * (128 * 128 * 4);
+    }
+    p.bytes = at;
+    return p;
+}
+extern "C" int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts, int32_t grouped) {
     if (dtype < CG3D_DT_F32 || dtype > CG3D_DT_I8 || i8_bad_shape(n_experts, cin, cout) || n_x < 0 || n_x > 0x7fffffffll || n_rows < 0 ||
-        n_rows > 0x7fffffffll)
+        n_rows > 0x7fffffffll || (grouped != 0 && grouped != 1))
         return CG3D_ERR_ARG;
-    return dtype == CG3D_DT_I8 || cin <= I8_FUSED_CIN ? 0 : ((n_x * 4 + 255) & ~255ll) + n_x * i8_pitch(cin);
+    return i8_choose(dtype, n_x, cin, n_rows, cout, n_experts, grouped, true).bytes;
 }
 extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, int64_t n_x, int32_t cin, const int8_t *w, const float *sw,
                                 const float *bias, int32_t bias_per_expert, const int32_t *offsets, const int32_t *rows, void *y,
                                 int32_t out_dtype, int64_t n_rows, int32_t cout, int32_t n_experts, void *ws, cg3d_stream_t stream) {
-    const int64_t need = cg3d_int8_linear_ws_bytes(dtype, n_x, cin, n_rows, cout, n_experts);
+    const int64_t need = cg3d_int8_linear_ws_bytes(dtype, n_x, cin, n_rows, cout, n_experts, offsets != nullptr);
     if (need < 0 || out_dtype < CG3D_DT_F32 || out_dtype > CG3D_DT_F16 || (bias_per_expert != 0 && bias_per_expert != 1)) return CG3D_ERR_ARG;
     if (offsets ? (!rows && n_x != n_rows) : (rows || n_x != n_rows || n_experts != 1)) return CG3D_ERR_ARG;
     if (n_rows == 0) return CG3D_OK;
     if (n_x == 0 || !x || !w || !sw || !y || (dtype == CG3D_DT_I8 && !sx) || (need > 0 && !ws)) return CG3D_ERR_ARG;
     if (((uintptr_t)x & (dtype == CG3D_DT_F32 ? 3 : dtype == CG3D_DT_I8 ? 0 : 1)) || ((uintptr_t)w & 15) || ((uintptr_t)y & (out_dtype == CG3D_DT_F32 ? 3 : 1)) ||
-        (((uintptr_t)sx | (uintptr_t)sw | (uintptr_t)bias) & 3) || ((uintptr_t)ws & 15))
+        (((uintptr_t)sx | (uintptr_t)sw | (uintptr_t)bias | (uintptr_t)offsets | (uintptr_t)rows) & 3) || ((uintptr_t)ws & 15))
         return CG3D_ERR_ARG;
     hipStream_t s = cg3d_hs(stream);
+    const bool padded = (cin & 15) || ((uintptr_t)x & 15);
+    const i8_plan p = i8_choose(dtype, n_x, cin, n_rows, cout, n_experts, offsets != nullptr, padded);
+    const int64_t panels = i8_panels(cout);
+    if (p.tiles > (1ll << 23) || (p.kind == i8_plan::TILE && p.tiles * p.ny > (1ll << 22))) return CG3D_ERR_ARG;      // (2^32 threads of a launch)
     i8_args a = {sx, w, sw, bias, offsets, rows, y, n_rows, n_x, cin, cout, n_experts, out_dtype, bias_per_expert ? cout : 0};
-    if (cin <= I8_FUSED_CIN) {
+    const int8_t *q = reinterpret_cast<const int8_t *>(x);
+    int64_t pitch = cin;
+    if (p.rows8) {
+        int8_t *lev = reinterpret_cast<int8_t *>(ws);
+        pitch = i8_pitch(cin);
+        if (dtype == CG3D_DT_I8) {
+            const int64_t nb = cg3d_divup(n_x * (pitch / 16), 256);
+            hipLaunchKernelGGL(k_i8_pad, dim3((unsigned)(nb < (1 << 22) ? nb : (1 << 22))), dim3(256), 0, s, q, n_x, cin, pitch, lev);
+            CG3D_CHECK_LAUNCH();
+        } else {
+            float *scale = reinterpret_cast<float *>(lev + p.scale_at);
+            const int rc = cg3d_int8_quantize_rows(x, dtype, n_x, cin, pitch, lev, scale, stream);
+            if (rc != CG3D_OK) return rc;
+            a.sx = scale;
+            dtype = CG3D_DT_I8;
+        }
+        q = lev;
+        x = lev;
+    }
+    if (p.kind == i8_plan::FEW) {
+        const dim3 grid((unsigned)p.tiles, (unsigned)(panels * 2));
+        if (panels * 2 > 65535) return CG3D_ERR_ARG;
+        if (p.rows8) a.cin = (int32_t)pitch;                         // (zeros behind the row: whole pieces)
+        if (dtype == CG3D_DT_F32) hipLaunchKernelGGL((k_i8_few<float>), grid, dim3(512), 0, s, a, reinterpret_cast<const float *>(x), pitch);
+        else if (dtype == CG3D_DT_BF16) hipLaunchKernelGGL((k_i8_few<i8_bf16>), grid, dim3(512), 0, s, a, reinterpret_cast<const i8_bf16 *>(x), pitch);
+        else if (dtype == CG3D_DT_F16) hipLaunchKernelGGL((k_i8_few<i8_f16>), grid, dim3(512), 0, s, a, reinterpret_cast<const i8_f16 *>(x), pitch);
+        else hipLaunchKernelGGL((k_i8_few<int8_t>), grid, dim3(512), 0, s, a, q, pitch);
+        CG3D_CHECK_LAUNCH();
+        return CG3D_OK;
+    }
+    if (p.kind == i8_plan::FUSED) {
         // enough workgroups for the chip: the panels of a row tile are shared out where there are fewer than 1024 tiles
-        const int64_t tiles = i8_tiles(a, 64), panels = i8_panels(cout);
-        const int32_t parts = (int32_t)(cg3d_divup(1024, tiles) < panels ? cg3d_divup(1024, tiles) : panels);
+        const int32_t parts = (int32_t)(cg3d_divup(1024, p.tiles) < panels ? cg3d_divup(1024, p.tiles) : panels);
         const int32_t each = (int32_t)cg3d_divup(panels, parts);
-        const int lds = (int)i8_chunks(cin) * 4096 + 256;
-        if (tiles > (1ll << 23)) return CG3D_ERR_ARG;
-#define I8_F(T, RG)                                                                                                                 \
-    do {                                                                                                                            \
-        if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(&k_i8_fused<T, RG>), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) \
-            return CG3D_ERR_LAUNCH;                                                                                                 \
-        hipLaunchKernelGGL((k_i8_fused<T, RG>), dim3((unsigned)tiles, (unsigned)parts), dim3(256), lds, s, a, reinterpret_cast<const T *>(x)); \
-    } while (0)
+        const int lds = (int)i8_chunks(cin) * 4096 + 256;           // (at most 32.25 KB)
+#define I8_F(T, RG) hipLaunchKernelGGL((k_i8_fused<T, RG>), dim3((unsigned)p.tiles, (unsigned)parts), dim3(256), lds, s, a, reinterpret_cast<const T *>(x))
 #define I8_FC(T) do { if (each >= 4) I8_F(T, 4); else if (each >= 2) I8_F(T, 2); else I8_F(T, 1); } while (0)
         if (dtype == CG3D_DT_F32) I8_FC(float);
         else if (dtype == CG3D_DT_BF16) I8_FC(i8_bf16);
@@ -576,20 +840,23 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
         CG3D_CHECK_LAUNCH();
         return CG3D_OK;
     }
-    const int8_t *q = reinterpret_cast<const int8_t *>(x);
-    int64_t pitch = cin;
-    if (dtype != CG3D_DT_I8) {
-        float *scale = reinterpret_cast<float *>(ws);
-        int8_t *lev = reinterpret_cast<int8_t *>(ws) + ((n_x * 4 + 255) & ~255ll);
-        pitch = i8_pitch(cin);
-        const int rc = cg3d_int8_quantize_rows(x, dtype, n_x, cin, pitch, lev, scale, stream);
-        if (rc != CG3D_OK) return rc;
-        a.sx = scale;
-        q = lev;
-    }
-    const int64_t nb = cg3d_divup(i8_tiles(a, 16) * i8_panels(cout), 4);
-    if (nb > (1ll << 23)) return CG3D_ERR_ARG;
-    hipLaunchKernelGGL(k_i8_wave, dim3((unsigned)nb), dim3(256), 0, s, a, q, pitch);
-    CG3D_CHECK_LAUNCH();
+    if (p.rows8) a.cin = (int32_t)pitch;
+    i32x4 *part = p.splits > 1 ? reinterpret_cast<i32x4 *>(reinterpret_cast<int8_t *>(ws) + p.part_at) : nullptr;
+    const int32_t total = (int32_t)(p.tiles * p.ny);
+#define I8_T(RG, WR, WC)                                                                                                            \
+    do {                                                                                                                            \
+        constexpr int lds = 4 * (WC * 4 + WR * RG) * 1024;                                                                          \
+        if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(&k_i8_tile<RG, WR, WC>), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) \
+            return CG3D_ERR_LAUNCH;                                                                                                 \
+        hipLaunchKernelGGL((k_i8_tile<RG, WR, WC>), dim3((unsigned)total, 1, (unsigned)p.splits), dim3(WR * WC * 64), lds, s, a, q, pitch, p.ny, part); \
+        CG3D_CHECK_LAUNCH();                                                                                                        \
+        if (part) {                                                                                                                 \
+            hipLaunchKernelGGL((k_i8_join<RG, WR, WC>), dim3((unsigned)cg3d_divup((int64_t)total * (RG * WR * WC), 4)), dim3(256), 0, s, a, p.ny, total, p.splits, part); \
+            CG3D_CHECK_LAUNCH();                                                                                                    \
+        }                                                                                                                           \
+    } while (0)
+    if (p.big) I8_T(8, 2, 4);
+    else I8_T(4, 2, 2);
+#undef I8_T
     return CG3D_OK;
 }

@@ -9,8 +9,6 @@ matrices of their own -- what the class-aware head does with its voxels (ops/hea
 Nothing is read back to the host: the calls can be captured into a graph.  No sum uses an atomic: results and gradients are the
 same from run to run.  Rows behind the last (as many as there are dropped pairs) are zeros in every output of that shape."""
 import contextlib
-from ctypes import c_int32, c_int64
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -71,7 +69,7 @@ def expert_plan(experts, n_experts):
         _, rows, pairs, pos, offsets = out.split((n_ws, n, n, n, n_experts + 1))
         pos = pos.view(t, k)
         ws = ptr(out) if n_ws else None
-        lib.call("cg3d_expert_plan", ptr(ids), c_int32(ids.dtype == torch.int64), c_int64(t), c_int32(k), c_int32(n_experts), ptr(offsets),
+        lib.call("cg3d_expert_plan", ptr(ids), int(ids.dtype == torch.int64), t, k, n_experts, ptr(offsets),
                  ptr(rows), ptr(pairs), ptr(pos), ws, lib.stream())
     return ExpertPlan(offsets, rows, pairs, pos, n_experts)
 
@@ -83,50 +81,49 @@ def _check_rows(who, x, n, plan, what):
     need(x.device == plan.pos.device, "%s: %s is on %s, the plan on %s", who, what, x.device, plan.pos.device)
 
 
-def _combine(lib, y, pos, w, t, k):
-    out = torch.empty((t, y.shape[1]), dtype=y.dtype, device=y.device)
-    lib.call("cg3d_expert_combine", ptr(y), c_int32(DTYPES[y.dtype]), ptr(pos), ptr(w), c_int32(0 if w is None else DTYPES[w.dtype]),
-             c_int64(t), c_int32(k), c_int32(y.shape[1]), ptr(out), lib.stream())
+def _gather(x, pos, rows):
+    lib = _lib.get()
+    x = x.contiguous()
+    lib.check(x, rows)
+    t, k = pos.shape
+    with on_device(x):
+        out = torch.empty((t * k, x.shape[1]), dtype=x.dtype, device=x.device)
+        lib.call("cg3d_expert_gather", ptr(x), DTYPES[x.dtype], ptr(rows), t, k, x.shape[1], ptr(out), lib.stream())
+    return out
+
+
+def _combine(y, pos, w):
+    lib = _lib.get()
+    lib.check(y, pos, w)
+    t, k = pos.shape
+    with on_device(y):
+        out = torch.empty((t, y.shape[1]), dtype=y.dtype, device=y.device)
+        lib.call("cg3d_expert_combine", ptr(y), DTYPES[y.dtype], ptr(pos), ptr(w), 0 if w is None else DTYPES[w.dtype], t, k, y.shape[1],
+                 ptr(out), lib.stream())
     return out
 
 
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, pos, rows):
-        lib = _lib.get()
-        x = x.contiguous()
-        lib.check(x, rows)
-        t, k = pos.shape
         ctx.save_for_backward(pos)
         ctx.set_materialize_grads(False)
-        with on_device(x):
-            out = torch.empty((t * k, x.shape[1]), dtype=x.dtype, device=x.device)
-            lib.call("cg3d_expert_gather", ptr(x), c_int32(DTYPES[x.dtype]), ptr(rows), c_int64(t), c_int32(k), c_int32(x.shape[1]), ptr(out),
-                     lib.stream())
-        return out
+        return _gather(x, pos, rows)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        if dout is None:
-            return None, None, None
-        (pos,) = ctx.saved_tensors
-        dout = dout.contiguous()
-        with on_device(dout):
-            return _combine(_lib.get(), dout, pos, None, *pos.shape), None, None
+        return None if dout is None else _combine(dout.contiguous(), ctx.saved_tensors[0], None), None, None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, pos, pairs, w):
-        lib = _lib.get()
         y, w = y.contiguous(), None if w is None else w.contiguous()
-        lib.check(y, pos, w)
         ctx.save_for_backward(y if ctx.needs_input_grad[3] else None, pairs, w)
         ctx.shape = pos.shape
         ctx.set_materialize_grads(False)
-        with on_device(y):
-            return _combine(lib, y, pos, w, *pos.shape)
+        return _combine(y, pos, w)
 
     @staticmethod
     @once_differentiable
@@ -134,20 +131,23 @@ class _Combine(torch.autograd.Function):
         if dout is None:
             return None, None, None, None
         y, pairs, w = ctx.saved_tensors
-        t, k = ctx.shape
+        (t, k), c = ctx.shape, dout.shape[1]
+        need_dy, _, _, need_dw = ctx.needs_input_grad
         lib = _lib.get()
         dout = dout.contiguous()
         with on_device(dout):
-            dy = torch.empty((t * k, dout.shape[1]), dtype=dout.dtype, device=dout.device) if ctx.needs_input_grad[0] else None
-            dw = torch.empty_like(w) if ctx.needs_input_grad[3] else None
-            lib.call("cg3d_expert_combine_bwd", ptr(dout), ptr(y), c_int32(DTYPES[dout.dtype]), ptr(pairs), ptr(w),
-                     c_int32(0 if w is None else DTYPES[w.dtype]), c_int64(t), c_int32(k), c_int32(dout.shape[1]), ptr(dy), ptr(dw), lib.stream())
+            dy = torch.empty((t * k, c), dtype=dout.dtype, device=dout.device) if need_dy else None
+            dw = torch.empty_like(w) if need_dw else None
+            lib.call("cg3d_expert_combine_bwd", ptr(dout), ptr(y), DTYPES[dout.dtype], ptr(pairs), ptr(w), 0 if w is None else DTYPES[w.dtype], t, k, c,
+                     ptr(dy), ptr(dw), lib.stream())
         return dy, None, None, dw
 
 
 def expert_gather(x, plan):
     """x [T, C] float32 / bfloat16 / float16 -> [T * k, C], the tokens' rows in the plan's order (differentiable in x)."""
     _check_rows("expert_gather", x, getattr(plan, "n_tokens", 0), plan, "x")
+    if not (x.requires_grad and torch.is_grad_enabled()):
+        return _gather(x, plan.pos, plan.rows)
     return _Gather.apply(x, plan.pos, plan.rows)
 
 
@@ -163,4 +163,6 @@ def expert_combine(rows, plan, weights=None):
         need(tuple(weights.shape) == (plan.n_tokens, plan.k), "expert_combine: weights must be [%d, %d], got %s", plan.n_tokens, plan.k,
              tuple(weights.shape))
         need(weights.device == rows.device, "expert_combine: weights are on %s, rows on %s", weights.device, rows.device)
+    if not (torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))):
+        return _combine(rows.contiguous(), plan.pos, None if weights is None else weights.contiguous())
     return _Combine.apply(rows, plan.pos, plan.pairs, weights)

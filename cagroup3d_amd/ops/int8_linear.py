@@ -9,8 +9,6 @@ its own for each expert's rows: the served form of the kernel-size-1 convolution
 
 The integer sums are exact, so results do not depend on how the work is split.  There is no gradient: a call on inputs that require
 one, with gradients enabled, is refused."""
-from ctypes import c_int32, c_int64
-
 import torch
 
 from .. import _lib
@@ -62,7 +60,7 @@ def int8_weight(w, scale=None):
             out, ws = torch.empty((2, e, cout), dtype=torch.float32, device=w.device)
         else:
             out, ws = scale.detach().clone().view(e, cout), None          # (the handle's own: the caller may reuse the memory)
-        lib.call("cg3d_int8_weight", ptr(w), c_int32(DTYPES[w.dtype]), c_int32(e), c_int32(cin), c_int32(cout), ptr(packed),
+        lib.call("cg3d_int8_weight", ptr(w), DTYPES[w.dtype], e, cin, cout, ptr(packed),
                  ptr(out) if ws is not None else None, ptr(ws), lib.stream())
     return Int8Weight(packed, out, e, cin, cout, grouped)
 
@@ -85,7 +83,7 @@ def quantize_rows(x):
     with on_device(x):
         q = torch.empty((n, cin), dtype=torch.int8, device=x.device)
         scale = torch.empty(n, dtype=torch.float32, device=x.device)
-        lib.call("cg3d_int8_quantize_rows", ptr(x), c_int32(DTYPES[x.dtype]), c_int64(n), c_int32(cin), c_int64(cin), ptr(q), ptr(scale),
+        lib.call("cg3d_int8_quantize_rows", ptr(x), DTYPES[x.dtype], n, cin, cin, ptr(q), ptr(scale),
                  lib.stream())
     return q, scale
 
@@ -131,10 +129,11 @@ def int8_linear(x, weight, bias=None, scale=None, out_dtype=None, plan=None, gat
     lib.check(x, bias, scale)
     with on_device(x):
         y = torch.empty((n_rows, weight.cout), dtype=out_dtype, device=x.device)
-        ws_bytes = int(lib.raw("cg3d_int8_linear_ws_bytes")(DTYPES[x.dtype], x.shape[0], weight.cin, n_rows, weight.cout, weight.n_experts))
+        ws_bytes = int(lib.raw("cg3d_int8_linear_ws_bytes")(DTYPES[x.dtype], x.shape[0], weight.cin, n_rows, weight.cout, weight.n_experts,
+                                                            int(plan is not None)))
         ws = torch.empty(ws_bytes, dtype=torch.int8, device=x.device) if ws_bytes > 0 else None
-        lib.call("cg3d_int8_linear", ptr(x), c_int32(DTYPES[x.dtype]), ptr(scale), c_int64(x.shape[0]), c_int32(weight.cin), ptr(weight.packed),
-                 ptr(weight.scale), ptr(bias), c_int32(per_expert), ptr(plan.offsets) if plan else None,
-                 ptr(plan.rows) if plan and gather else None, ptr(y), c_int32(DTYPES[out_dtype]), c_int64(n_rows), c_int32(weight.cout),
-                 c_int32(weight.n_experts), ptr(ws), lib.stream())
+        lib.call("cg3d_int8_linear", ptr(x), DTYPES[x.dtype], ptr(scale), x.shape[0], weight.cin, ptr(weight.packed),
+                 ptr(weight.scale), ptr(bias), int(per_expert), ptr(plan.offsets) if plan else None,
+                 ptr(plan.rows) if plan and gather else None, ptr(y), DTYPES[out_dtype], n_rows, weight.cout,
+                 weight.n_experts, ptr(ws), lib.stream())
     return y

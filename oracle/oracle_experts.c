@@ -209,21 +209,21 @@ int cg3d_int8_quantize_rows(const void *x, int32_t dtype, int64_t n, int32_t cin
     }
     return CG3D_OK;
 }
-int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts) {
+int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts, int32_t grouped) {
     if (dtype < CG3D_DT_F32 || dtype > CG3D_DT_I8 || bad_shape(n_experts, cin, cout) || n_x < 0 || n_x > 0x7fffffffll || n_rows < 0 ||
-        n_rows > 0x7fffffffll)
+        n_rows > 0x7fffffffll || (grouped != 0 && grouped != 1))
         return CG3D_ERR_ARG;
     return dtype == CG3D_DT_I8 ? 0 : n_x * (4 + (int64_t)cin);
 }
 int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, int64_t n_x, int32_t cin, const int8_t *w, const float *sw,
                      const float *bias, int32_t bias_per_expert, const int32_t *offsets, const int32_t *rows, void *y, int32_t out_dtype,
                      int64_t n_rows, int32_t cout, int32_t n_experts, void *ws, cg3d_stream_t stream) {
-    const int64_t need = cg3d_int8_linear_ws_bytes(dtype, n_x, cin, n_rows, cout, n_experts);
+    const int64_t need = cg3d_int8_linear_ws_bytes(dtype, n_x, cin, n_rows, cout, n_experts, offsets != 0);
     if (need < 0 || !fl(out_dtype) || (bias_per_expert != 0 && bias_per_expert != 1)) return CG3D_ERR_ARG;
     if (offsets ? (!rows && n_x != n_rows) : (rows || n_x != n_rows || n_experts != 1)) return CG3D_ERR_ARG;
     if (n_rows == 0) return CG3D_OK;
     if (n_x == 0 || !x || !w || !sw || !y || (dtype == CG3D_DT_I8 && !sx) || (need > 0 && !ws)) return CG3D_ERR_ARG;
-    if (odd(x, dtype) || ((uintptr_t)w & 15) || odd(y, out_dtype) || odd(sx, 0) || odd(sw, 0) || odd(bias, 0) || ((uintptr_t)ws & 15))
+    if (odd(x, dtype) || ((uintptr_t)w & 15) || odd(y, out_dtype) || odd(sx, 0) || odd(sw, 0) || odd(bias, 0) || odd(offsets, 0) || odd(rows, 0) || ((uintptr_t)ws & 15))
         return CG3D_ERR_ARG;
     const int8_t *q = (const int8_t *)x;
     if (dtype != CG3D_DT_I8) {

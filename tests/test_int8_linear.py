@@ -242,11 +242,11 @@ def test_entry_points_refuse(oracle):
         for args in ((a, 3, 4, 8, 8, a, a), (a, 0, -1, 8, 8, a, a), (a, 0, 4, 0, 8, a, a), (a, 0, 4, 8, 7, a, a), (None, 0, 4, 8, 8, a, a),
                      (a, 0, 4, 8, 8, None, a), (a, 0, 4, 8, 8, a, None), (a + 2, 0, 4, 8, 8, a, a), (a, 0, 4, 8, 8, a, a + 2)):
             assert lib.raw("cg3d_int8_quantize_rows")(*args, None) == -1, args
-        good = dict(x=a, dtype=0, sx=None, n_x=4, cin=800, w=a, sw=a, bias=None, bpe=0, offsets=None, rows=None, y=a, out=0, n_rows=4, cout=6, e=1, ws=a)
+        good = dict(x=a, dtype=0, sx=None, n_x=4, cin=8000, w=a, sw=a, bias=None, bpe=0, offsets=None, rows=None, y=a, out=0, n_rows=4, cout=6, e=1, ws=a)
         for change in (dict(dtype=4), dict(dtype=-1), dict(out=3), dict(out=-1), dict(bpe=2), dict(n_x=3), dict(e=2), dict(rows=a), dict(x=None),
                        dict(w=None), dict(sw=None), dict(y=None), dict(ws=None), dict(ws=a + 4), dict(x=a + 2), dict(w=a + 8), dict(y=a + 2),
                        dict(sw=a + 2), dict(bias=a + 1), dict(dtype=3, ws=None), dict(dtype=3, sx=a + 2), dict(n_x=-4, n_rows=-4), dict(cin=0), dict(cout=0),
-                       dict(offsets=a, n_x=3), dict(offsets=a, rows=a, n_x=0), dict(n_rows=1 << 31, n_x=1 << 31)):
+                       dict(offsets=a, n_x=3), dict(offsets=a, rows=a, n_x=0), dict(offsets=a + 2), dict(offsets=a, rows=a + 1), dict(n_rows=1 << 31, n_x=1 << 31)):
             assert lib.raw("cg3d_int8_linear")(*{**good, **change}.values(), None) == -1, change
 
 
