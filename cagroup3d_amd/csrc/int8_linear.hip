@@ -6,9 +6,13 @@
 //
 // The rounding of q is decided exactly, not up to the error of a reciprocal.  With c = 127 / max rounded UP to fp32, t' = c x lies
 // between the true t and t (1 + 2^-23), so that a wrong nearest level needs t' on or just above a half (by at most 127 * 2^-23 <
-// 2^-16).  t' enters one fused multiply-add with 1.5 * 2^23 (its low byte is then the level) and is never rounded by itself; only
-// where it falls into that strip the two sides 127 |x| and (n - 1/2) max are compared, each as an fp32 product and its exact error.
-// |x| = max / 2, the one tie that rows of 16-bit floats meet all the time, needs no look: it lands on 64, the even side.
+// 2^-16).  t' enters one fused multiply-add with 1.5 * 2^23 (its low byte is then the level) and is never rounded by itself.
+//   fp32 rows: where t' falls into that strip the two sides 127 |x| and (n - 1/2) max are compared, each as an fp32 product and its
+//   exact error.
+//   16-bit rows: x = mx 2^i and max = ma 2^(i + s) with whole mx, ma < 2^11, so a t that is no half is off it by 1 / (2 ma 2^s) or more
+//   -- over 2^-12 2^-s, against an error below 2^-15 2^-s: only true halves can go wrong, 254 mx = (2 n + 1) ma 2^s.  127 divides one
+//   side's 2 n + 1 (n = 63: t' lands on 64, the even side, as it should) or ma = 127 k: for k a power of two c is exact and so is the
+//   rounding, and only for the other k (fp16; bf16 has none, ma < 2^8) a row's elements are looked at like those of fp32 rows.
 // A row that holds an infinity or a NaN gets the scale NaN (and so a row of NaN as its result); a row of zeros the scale 0.
 //
 // The weights are the MFMA's A operand and the rows its B operand (v_mfma_i32_16x16x64_i8), i.e. a tile of the product is
@@ -25,6 +29,8 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 #define I8_MAX_CIN 131071            // 2^14 * 131071 < 2^31: -128 * -128 included
 #define I8_MAX_EXPERTS 1024
 #define I8_FUSED_CIN 512
+#define I8_LONG 513
+#define I8_SPLIT 256
 
 template <typename T, int V> struct __attribute__((packed, aligned(1))) i8_vec { T e[V]; };
 
@@ -96,17 +102,19 @@ template <typename T> struct i8_max {
 // What a row's largest magnitude (its bits) makes of the row's elements.  Rows whose largest is below 2^-96 or from 2^112 on are
 // shifted by a power of two first (`shift`, exact for every element that is not level 0), so that no product here leaves the range.
 struct i8_level {
-    float amax, c, half, shift, scale;
+    float amax, c, shift, scale;
     uint32_t keep;                                       // 0: the row has no levels
+    bool fine127;                                        // max / 127 is exact, 127 / max is not
     __device__ __forceinline__ explicit i8_level(uint32_t top) {
         const float a = __uint_as_float(top);
         const bool fine = top < 0x7f800000u;
         shift = a < 0x1p-96f ? 0x1p96f : fine && a >= 0x1p112f ? 0x1p-16f : 1.f;
         keep = fine && top ? ~0u : 0u;
         amax = keep ? a * shift : 1.f;
-        half = 0.5f * amax;
         c = 127.f / amax;
-        if (__builtin_fmaf(c, amax, -127.f) < 0.f) c = __uint_as_float(__float_as_uint(c) + 1);
+        const float off = __builtin_fmaf(c, amax, -127.f), s127 = amax / 127.f;
+        if (off < 0.f) c = __uint_as_float(__float_as_uint(c) + 1);
+        fine127 = off != 0.f && __builtin_fmaf(s127, 127.f, -amax) == 0.f;
         scale = fine ? a / 127.f : __uint_as_float(0x7fc00000u);
     }
     __device__ __forceinline__ bool shifted() const { return shift != 1.f; }
@@ -121,18 +129,20 @@ static __device__ __forceinline__ float i8_decide(const i8_level &v, float x, fl
     const bool down = less || (same && ((int)n & 1));
     return down ? r - copysignf(1.f, r - I8_MAGIC) : r;
 }
-// 16 elements (shifted) of one row -> 16 levels.  SHORT: the elements were 16-bit floats
-template <bool SHORT>
+// 16 elements (shifted) of one row -> 16 levels.  T: what the elements were
+template <typename T>
 static __device__ __forceinline__ i32x4 i8_quant16(const i8_level &v, const float (&x)[16]) {
     float r[16];
     bool look = false;
 #pragma unroll
-    for (int j = 0; j < 16; j++) {
-        r[j] = __builtin_fmaf(x[j], v.c, I8_MAGIC);
-        const float d = __builtin_fmaf(x[j], v.c, -(r[j] - I8_MAGIC));
-        look |= fabsf(d) > 0.5f - 0x1p-16f && (!SHORT || fabsf(x[j]) != v.half);
-    }
-    if (__builtin_expect(__any(look), 0)) {
+    for (int j = 0; j < 16; j++) r[j] = __builtin_fmaf(x[j], v.c, I8_MAGIC);
+    if constexpr (sizeof(T) == 4) {
+        float most = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; j++) most = fmaxf(most, fabsf(__builtin_fmaf(x[j], v.c, I8_MAGIC - r[j])));
+        look = most > 0.5f - 0x1p-16f;
+    } else if constexpr (__is_same(T, i8_f16)) look = v.fine127;
+    if (!__is_same(T, i8_bf16) && __builtin_expect(__any(look), 0)) {
 #pragma unroll
         for (int j = 0; j < 16; j++) {
             const float n = r[j] - I8_MAGIC, d = __builtin_fmaf(x[j], v.c, -n);
@@ -158,7 +168,7 @@ static __device__ __forceinline__ i32x4 i8_levels16(const i8_level &lev, bool fa
 #pragma unroll
         for (int j = 0; j < 16; j++) f[j] *= lev.shift;
     }
-    return i8_quant16<sizeof(T) == 2>(lev, f);
+    return i8_quant16<T>(lev, f);
 }
 
 // ---------------------------------------------------------------- weights (once per model)
@@ -194,7 +204,7 @@ __global__ __launch_bounds__(256) void k_i8_weight_pack(const T *__restrict__ w,
             const i8_level lev(there ? top[(int64_t)e * cout + n] : 0);
             float f[16];
             for (int j = 0; j < 16; j++) f[j] = there && k0 + j < cin ? i8_f(src[(int64_t)(k0 + j) * cout]) * lev.shift : 0.f;
-            o.v = i8_quant16<sizeof(T) == 2>(lev, f);
+            o.v = i8_quant16<T>(lev, f);
         }
         reinterpret_cast<i32x4 *>(out)[i] = o.v;
     }
@@ -274,6 +284,47 @@ __global__ __launch_bounds__(B) void k_i8_rows(const T *__restrict__ x, int64_t 
         for (int64_t a = nv * 16ll + lane; a < pitch; a += L) dst[a] = 0;
     }
 }
+// Long rows, one to a workgroup of B threads, held in registers between the maximum and the levels: KEEP * B * 16 elements at most.
+// (512 rows of 43 904 fp32: ... us with 16 waves and 3 pieces each, 36 with 8 and 6, 31 reading the row twice with 4.)
+template <typename T, int KEEP, int B>
+__global__ __launch_bounds__(B) void k_i8_long_rows(const T *__restrict__ x, int64_t n, int32_t cin, int64_t pitch, int8_t *__restrict__ q,
+                                                      float *__restrict__ scale) {
+    __shared__ uint32_t sh[B / 64];
+    const int tid = threadIdx.x;
+    for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
+        const T *row = x + r * cin;
+        i8_raw<T> v[KEEP];
+        i8_max<T> most;
+#pragma unroll
+        for (int i = 0; i < KEEP; i++) v[i] = i8_get16<T>(row, (i * B + tid) * 16, cin);
+#pragma unroll
+        for (int i = 0; i < KEEP; i++) most.add(v[i]);
+        uint32_t top = most.bits();
+        for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        if ((tid & 63) == 0) sh[tid >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < B / 64; w++) top = max(top, sh[w]);
+        __syncthreads();
+        const i8_level lev(top);
+        if (tid == 0) scale[r] = lev.scale;
+        int8_t *dst = q + r * pitch;
+#pragma unroll
+        for (int i = 0; i < KEEP; i++) {
+            const int64_t k0 = (int64_t)(i * B + tid) * 16;
+            if (k0 >= pitch) break;
+            const i32x4 lv = i8_levels16<T>(lev, lev.shifted(), v[i]);
+            if (k0 + 16 <= pitch) *reinterpret_cast<u32x4_any *>(dst + k0) = __builtin_bit_cast(u32x4, lv);
+            else {
+                const i8_vec<int8_t, 16> o = __builtin_bit_cast(i8_vec<int8_t, 16>, lv);
+#pragma unroll
+                for (int j = 0; j < 15; j++)
+                    if (k0 + j < pitch) dst[k0 + j] = o.e[j];
+            }
+        }
+        for (int64_t a = (int64_t)KEEP * B * 16 + tid; a < pitch; a += B) dst[a] = 0;
+    }
+}
 extern "C" int cg3d_int8_quantize_rows(const void *x, int32_t dtype, int64_t n, int32_t cin, int64_t pitch, int8_t *q, float *scale,
                                        cg3d_stream_t stream) {
     if (dtype < CG3D_DT_F32 || dtype > CG3D_DT_F16 || n < 0 || cin < 1 || cin > I8_MAX_CIN || pitch < cin) return CG3D_ERR_ARG;
@@ -282,6 +333,18 @@ extern "C" int cg3d_int8_quantize_rows(const void *x, int32_t dtype, int64_t n, 
     hipStream_t s = cg3d_hs(stream);
     int32_t ls = 0;
     const int32_t nv = (cin + 15) / 16;
+    if (cin >= I8_LONG && cin <= 3 * 16384) {             // whole rows in a workgroup's registers; beyond that they are read twice
+        const unsigned nb = (unsigned)(n < (1 << 21) ? n : (1 << 21));
+#define I8_L(T, K, B) hipLaunchKernelGGL((k_i8_long_rows<T, K, B>), dim3(nb), dim3(B), 0, s, reinterpret_cast<const T *>(x), n, cin, pitch, q, scale)
+#define I8_LK(T) do { if (cin <= 1024) I8_L(T, 1, 64); else if (cin <= 2048) I8_L(T, 1, 128); else if (cin <= 4096) I8_L(T, 1, 256); else if (cin <= 8192) I8_L(T, 1, 512); else if (cin <= 16384) I8_L(T, 1, 1024); else if (cin <= 2 * 16384) I8_L(T, 2, 1024); else I8_L(T, 3, 1024); } while (0)
+        if (dtype == CG3D_DT_F32) I8_LK(float);
+        else if (dtype == CG3D_DT_BF16) I8_LK(i8_bf16);
+        else I8_LK(i8_f16);
+#undef I8_LK
+#undef I8_L
+        CG3D_CHECK_LAUNCH();
+        return CG3D_OK;
+    }
     while ((1 << ls) < nv && ls < 6) ls++;
     if (nv > 4 * 64) ls = 8;                              // a long row: the whole workgroup
     int64_t nb = cg3d_divup(n << ls, 256);
@@ -416,8 +479,8 @@ static __device__ __forceinline__ int64_t i8_source(const i8_args &a, int64_t ro
 // is a maximum over the lane and two exchanges, and the levels go to LDS as whole fragments (contiguous, no conflicts).  Then wave
 // (wm, wn) multiplies RG of the 4 row groups by panels wn, wn + RG, ... of the part blockIdx.y of the channels: the weights stream
 // past from the caches one chunk ahead, every fragment used RG times.  RG = 4 / 2 / 1 for at least 4 / 2 / 1 panels a part.
-template <typename T, int RG>
-__global__ __launch_bounds__(256, 4) void k_i8_fused(i8_args a, const T *__restrict__ x) {
+template <typename T, int RG, int KEEP>                  // KEEP: chunks of a row held in registers; longer rows are read again, from the caches
+__global__ __launch_bounds__(256, RG == 4 || KEEP * sizeof(T) > 8 ? 4 : RG == 2 ? 5 : 6) void k_i8_fused(i8_args a, const T *__restrict__ x) {
     extern __shared__ __attribute__((aligned(16))) uint8_t i8_sm[];
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int panels = (a.cout + 63) >> 6, chunks = (a.cin + 63) >> 6;
@@ -437,7 +500,6 @@ __global__ __launch_bounds__(256, 4) void k_i8_fused(i8_args a, const T *__restr
 #pragma unroll 8
             for (int c = 0; c < chunks; c++) mine[c * 64] = __builtin_bit_cast(i32x4, i8_get16<T>(xr, c * 64 + g * 16, a.cin).w[0]);
         } else {
-            constexpr int KEEP = sizeof(T) == 2 ? 8 : 4;                           // chunks held in registers (64 of them)
             i8_raw<T> v[KEEP];
             i8_max<T> most;
             for (int c0 = 0; c0 < chunks; c0 += KEEP) {
@@ -455,7 +517,7 @@ __global__ __launch_bounds__(256, 4) void k_i8_fused(i8_args a, const T *__restr
             const bool far = __any(lev.shifted());
             if (g == 0) scales[wave * 16 + m] = lev.scale;
             for (int c0 = 0; c0 < chunks; c0 += KEEP) {
-                if (chunks > KEEP) {                                               // (longer rows are read again, from the caches)
+                if (chunks > KEEP) {
 #pragma unroll
                     for (int c = 0; c < KEEP; c++)
                         if (c0 + c < chunks) v[c] = i8_get16<T>(xr, (c0 + c) * 64 + g * 16, a.cin);
@@ -466,8 +528,13 @@ __global__ __launch_bounds__(256, 4) void k_i8_fused(i8_args a, const T *__restr
             }
         }
     }
-    __syncthreads();
     const int wn = wave % RG, wm = wave / RG;
+    const i32x4 *const w_e = reinterpret_cast<const i32x4 *>(a.w) + (int64_t)(live ? e : 0) * panels * (chunks * 256) + lane;
+    i32x4 cur[4];                                                                  // (the first weights travel over the barrier)
+    if (p_lo + wn < p_hi)
+#pragma unroll
+        for (int nb = 0; nb < 4; nb++) cur[nb] = w_e[(int64_t)(p_lo + wn) * (chunks * 256) + nb * 64];
+    __syncthreads();
     if (wm * RG * 16 >= rows) return;
     const i32x4 *const bq = frag + wm * RG * chunks * 64 + lane;
     for (int p = p_lo + wn; p < p_hi; p += RG) {
@@ -476,25 +543,23 @@ __global__ __launch_bounds__(256, 4) void k_i8_fused(i8_args a, const T *__restr
         for (int h = 0; h < RG; h++)
 #pragma unroll
             for (int nb = 0; nb < 4; nb++) acc[h][nb] = i32x4{0, 0, 0, 0};
-        if (live) {
-            const i32x4 *wf = reinterpret_cast<const i32x4 *>(a.w) + ((int64_t)e * panels + p) * (chunks * 256) + lane;
-            i32x4 cur[4];
+        const i32x4 *wf = w_e + (int64_t)p * (chunks * 256);
+        const i32x4 *const then = w_e + (int64_t)(p + RG < p_hi ? p + RG : p) * (chunks * 256);
+        for (int c = 0; c < chunks; c++) {
+            i32x4 nxt[4];
+            wf = c + 1 < chunks ? wf + 256 : then;                                 // (the next panel's first behind the last)
 #pragma unroll
-            for (int nb = 0; nb < 4; nb++) cur[nb] = wf[nb * 64];
-            for (int c = 0; c < chunks; c++) {
-                i32x4 nxt[4];
-                wf += c + 1 < chunks ? 256 : 0;
-#pragma unroll
-                for (int nb = 0; nb < 4; nb++) nxt[nb] = wf[nb * 64];
+            for (int nb = 0; nb < 4; nb++) nxt[nb] = wf[nb * 64];
+            if (live) {
 #pragma unroll
                 for (int h = 0; h < RG; h++) {
                     const i32x4 q = bq[(h * chunks + c) * 64];                     // (a group without rows: old bytes, never stored)
 #pragma unroll
                     for (int nb = 0; nb < 4; nb++) acc[h][nb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur[nb], q, acc[h][nb], 0, 0, 0);
                 }
-#pragma unroll
-                for (int nb = 0; nb < 4; nb++) cur[nb] = nxt[nb];
             }
+#pragma unroll
+            for (int nb = 0; nb < 4; nb++) cur[nb] = nxt[nb];
         }
 #pragma unroll
         for (int h = 0; h < RG; h++) {
@@ -689,29 +754,37 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void k_i8_tile(i8_args a, const in
         if (r < rows) i8_store(a, e, panel, row0 + r, live ? a.sx[i8_source(a, row0 + r)] : 0.f, live, acc[h]);
     }
 }
-// the sums of a tile's ranges of chunks: a wave owns 16 rows x 64 channels of it
+// The sums of a tile's ranges of chunks: a workgroup owns 16 rows x 64 channels, its 8 waves share the ranges (one wave for all of
+// them: 64 waves on the whole chip for 512 x 128 results, 18.7 us at 85 ranges).
 template <int RG, int WR, int WC>
-__global__ __launch_bounds__(256) void k_i8_join(i8_args a, int32_t ny, int32_t total, int32_t splits, const i32x4 *__restrict__ part) {
+__global__ __launch_bounds__(512) void k_i8_join(i8_args a, int32_t ny, int32_t total, int32_t splits, const i32x4 *__restrict__ part) {
     constexpr int NW = WR * WC, BM = WR * RG * 16;
-    const int lane = threadIdx.x & 63, m = lane & 15;
-    const int64_t u = blockIdx.x * 4ll + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = (int)(u % RG), wave = (int)(u / RG % NW), id = (int)(u / (RG * NW));
-    if (id >= total) return;
+    __shared__ i32x4 sum[8][4][64];
+    const int lane = threadIdx.x & 63, m = lane & 15, me = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = blockIdx.x % RG, wave = blockIdx.x / RG % NW, id = blockIdx.x / (RG * NW);
     int e, rows;
     int64_t row0;
-    if (!i8_tile<BM>(a, id / ny, e, row0, rows)) return;
+    if (!i8_tile<BM>(a, id / ny, e, row0, rows)) return;             // (the whole workgroup)
     const bool live = e < a.n_experts;
     const int wr = wave % WR, wc = wave / WR, panel = id % ny * WC + wc, r = (wr * RG + h) * 16 + m;
     if (panel >= (a.cout + 63) >> 6 || (wr * RG + h) * 16 >= rows) return;
     i32x4 acc[4];
 #pragma unroll
     for (int nb = 0; nb < 4; nb++) acc[nb] = i32x4{0, 0, 0, 0};
-    const i32x4 *from = part + (((int64_t)id * NW + wave) * (RG * 4) + h * 4) * 64 + lane;
     const int64_t next = (int64_t)total * NW * (RG * 4) * 64;
-#pragma unroll 4
-    for (int z = 0; z < splits; z++, from += next)
+    const i32x4 *from = part + (((int64_t)id * NW + wave) * (RG * 4) + h * 4) * 64 + lane;
+#pragma unroll 2
+    for (int z = me; z < splits; z += 8)
 #pragma unroll
-        for (int nb = 0; nb < 4; nb++) acc[nb] += from[nb * 64];
+        for (int nb = 0; nb < 4; nb++) acc[nb] += from[z * next + nb * 64];
+#pragma unroll
+    for (int nb = 0; nb < 4; nb++) sum[me][nb][lane] = acc[nb];
+    __syncthreads();
+    if (me != 0) return;
+#pragma unroll
+    for (int w = 1; w < 8; w++)
+#pragma unroll
+        for (int nb = 0; nb < 4; nb++) acc[nb] += sum[w][nb][lane];
     if (r < rows) i8_store(a, e, panel, row0 + r, live ? a.sx[i8_source(a, row0 + r)] : 0.f, live, acc);
 }
 
@@ -755,7 +828,7 @@ static i8_plan i8_choose(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows
         const int64_t total = p.tiles * p.ny;
         p.splits = 1;
         if (!p.big && total < 256) {                                 // half the chip's places empty: the contraction is shared out
-            const int64_t want = cg3d_divup(512, total), most = chunks / 8;
+            const int64_t want = cg3d_divup(I8_SPLIT, total), most = chunks / 8;
             p.splits = (int32_t)(want < most ? want : most > 1 ? most : 1);
         }
     }
@@ -829,12 +902,17 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
         const int32_t parts = (int32_t)(cg3d_divup(1024, p.tiles) < panels ? cg3d_divup(1024, p.tiles) : panels);
         const int32_t each = (int32_t)cg3d_divup(panels, parts);
         const int lds = (int)i8_chunks(cin) * 4096 + 256;           // (at most 32.25 KB)
-#define I8_F(T, RG) hipLaunchKernelGGL((k_i8_fused<T, RG>), dim3((unsigned)p.tiles, (unsigned)parts), dim3(256), lds, s, a, reinterpret_cast<const T *>(x))
-#define I8_FC(T) do { if (each >= 4) I8_F(T, 4); else if (each >= 2) I8_F(T, 2); else I8_F(T, 1); } while (0)
+#define I8_F(T, RG, KEEP) hipLaunchKernelGGL((k_i8_fused<T, RG, KEEP>), dim3((unsigned)p.tiles, (unsigned)parts), dim3(256), lds, s, a, reinterpret_cast<const T *>(x))
+#define I8_FK(T, RG) do { if (chunks <= 1) I8_F(T, RG, 1); else if (chunks <= 2) I8_F(T, RG, 2); else I8_F(T, RG, (sizeof(T) == 4 ? 4 : 8)); } while (0)
+#define I8_FC(T) do { if (each >= 4) I8_FK(T, 4); else if (each >= 2) I8_FK(T, 2); else I8_FK(T, 1); } while (0)
+        const int64_t chunks = i8_chunks(cin);
         if (dtype == CG3D_DT_F32) I8_FC(float);
         else if (dtype == CG3D_DT_BF16) I8_FC(i8_bf16);
         else if (dtype == CG3D_DT_F16) I8_FC(i8_f16);
-        else I8_FC(int8_t);
+        else if (each >= 4) I8_F(int8_t, 4, 1);
+        else if (each >= 2) I8_F(int8_t, 2, 1);
+        else I8_F(int8_t, 1, 1);
+#undef I8_FK
 #undef I8_FC
 #undef I8_F
         CG3D_CHECK_LAUNCH();
@@ -851,7 +929,7 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
         hipLaunchKernelGGL((k_i8_tile<RG, WR, WC>), dim3((unsigned)total, 1, (unsigned)p.splits), dim3(WR * WC * 64), lds, s, a, q, pitch, p.ny, part); \
         CG3D_CHECK_LAUNCH();                                                                                                        \
         if (part) {                                                                                                                 \
-            hipLaunchKernelGGL((k_i8_join<RG, WR, WC>), dim3((unsigned)cg3d_divup((int64_t)total * (RG * WR * WC), 4)), dim3(256), 0, s, a, p.ny, total, p.splits, part); \
+            hipLaunchKernelGGL((k_i8_join<RG, WR, WC>), dim3((unsigned)(total * (RG * WR * WC))), dim3(512), 0, s, a, p.ny, total, p.splits, part); \
             CG3D_CHECK_LAUNCH();                                                                                                    \
         }                                                                                                                           \
     } while (0)

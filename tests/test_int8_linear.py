@@ -155,6 +155,19 @@ def levels(dev):
         check_levels(v, *quantize_rows(v))
 
 
+def short_levels(dev, dtype):
+    """Every pair of significands of the type, over the octaves where a level is not 0: a row for each largest magnitude."""
+    bits = 8 if dtype == BF16 else 11
+    step = 1 if dev == "cuda" or dtype == BF16 else 37            # (fp16 has 1024 x 1024 pairs an octave)
+    sig = torch.arange(2 ** (bits - 1), 2 ** bits, step).double()
+    if step > 1:                                                  # multiples of 127 are where halves can be met away from 63.5
+        sig = torch.cat([sig, torch.arange(9, 17).double() * 127])
+    x = torch.cat([sig.unsqueeze(1)] + [torch.arange(2 ** (bits - 1), 2 ** bits).double().unsqueeze(0).expand(sig.numel(), -1) * 2.0 ** -s for s in range(1, 9)], 1)
+    x[:, 1::2] *= -1
+    x = (x * 2.0 ** -6).to(dtype).to(dev)                         # (exact: no subnormals of fp16)
+    check_levels(x, *quantize_rows(x))
+
+
 def nonfinite(dev):
     x = torch.randn(6, 40, generator=torch.Generator().manual_seed(5)).to(dev)
     x[1, 7], x[2, 39], x[3, 0], x[4] = float("inf"), float("nan"), float("-inf"), 0.0
@@ -171,6 +184,8 @@ def nonfinite(dev):
 def test_oracle_levels_and_nonfinite(oracle):
     with _lib.use_library(oracle):
         levels("cpu")
+        short_levels("cpu", BF16)
+        short_levels("cpu", F16)
         nonfinite("cpu")
 
 
@@ -262,6 +277,8 @@ def test_no_cpu_fallback():
 @pytest.mark.gpu
 def test_hip_levels_and_nonfinite(hip):
     levels("cuda")
+    short_levels("cuda", BF16)
+    short_levels("cuda", F16)
     nonfinite("cuda")
 
 
