@@ -9,6 +9,7 @@ matrices of their own -- what the class-aware head does with its voxels (ops/hea
 Nothing is read back to the host: the calls can be captured into a graph.  No sum uses an atomic: results and gradients are the
 same from run to run.  Rows behind the last (as many as there are dropped pairs) are zeros in every output of that shape."""
 import contextlib
+import functools
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -25,7 +26,10 @@ def on_device(t):
     the current one."""
     if t.is_cuda and t.device.index != torch.cuda.current_device():
         return torch.cuda.device(t.device)
-    return contextlib.nullcontext()
+    return _HERE
+
+
+_HERE = contextlib.nullcontext()
 
 
 def need(ok, message, *args):
@@ -36,17 +40,34 @@ def need(ok, message, *args):
 class ExpertPlan:
     """Where the rows of a routing go.  offsets int32 [n_experts + 1], rows int32 [T * k] (the token of each row, -1 behind the
     last), pairs int32 [T * k] (the pair t * k + s of each row, negative behind the last), pos int32 [T, k] (the row of each pair;
-    negative: the pair has none)."""
+    negative: the pair has none).  The tables lie in one allocation; the tensors are made when they are asked for."""
 
-    __slots__ = ("offsets", "rows", "pairs", "pos", "n_tokens", "k", "n_experts")
+    __slots__ = ("device", "n_tokens", "k", "n_experts", "n_rows", "_tables", "_at")
 
-    def __init__(self, offsets, rows, pairs, pos, n_experts):
-        self.offsets, self.rows, self.pairs, self.pos, self.n_experts = offsets, rows, pairs, pos, n_experts
-        self.n_tokens, self.k = pos.shape
+    def __init__(self, tables, at, n_tokens, k, n_experts):
+        self.device, self.n_tokens, self.k, self.n_experts, self.n_rows = tables.device, n_tokens, k, n_experts, n_tokens * k
+        self._tables, self._at = tables, at
 
-    @property
-    def n_rows(self):
-        return self.n_tokens * self.k
+    def _slice(self, i, n):
+        at = self._at + i * self.n_rows
+        return self._tables[at:at + n]
+
+    rows = property(lambda self: self._slice(0, self.n_rows))
+    pairs = property(lambda self: self._slice(1, self.n_rows))
+    pos = property(lambda self: self._slice(2, self.n_rows).view(self.n_tokens, self.k))
+    offsets = property(lambda self: self._slice(3, self.n_experts + 1))
+
+    def address(self, i):
+        """Of table i: rows, pairs, pos, offsets."""
+        return self._tables.data_ptr() + 4 * (self._at + i * self.n_rows)
+
+
+ROWS, PAIRS, POS, OFFSETS = range(4)
+
+
+@functools.lru_cache(maxsize=4096)
+def _plan_ws_words(lib, t, k, n_experts):
+    return int(lib.raw("cg3d_expert_plan_ws_bytes")(t, k, n_experts)) // 4
 
 
 def expert_plan(experts, n_experts):
@@ -58,97 +79,95 @@ def expert_plan(experts, n_experts):
     need(1 <= n_experts <= MAX_EXPERTS, "expert_plan: n_experts = %d is not in 1 .. %d", n_experts, MAX_EXPERTS)
     ids = (experts if experts.dim() == 2 else experts.unsqueeze(1)).contiguous()
     t, k = ids.shape
-    need(k >= 1 and t * k < 2 ** 31, "expert_plan: experts of shape %s (k >= 1, fewer than 2^31 pairs)", tuple(experts.shape))
+    need(k >= 1 and t * k < 2 ** 31, "expert_plan: %d x %d pairs (k >= 1, fewer than 2^31 pairs)", t, k)
     lib = _lib.get()
     lib.check(ids)
     with on_device(ids):
-        ws_bytes = int(lib.raw("cg3d_expert_plan_ws_bytes")(t, k, n_experts))
-        n = t * k
-        n_ws = ws_bytes // 4
-        out = torch.empty(n_ws + 3 * n + n_experts + 1, dtype=torch.int32, device=ids.device)
-        _, rows, pairs, pos, offsets = out.split((n_ws, n, n, n, n_experts + 1))
-        pos = pos.view(t, k)
-        ws = ptr(out) if n_ws else None
-        lib.call("cg3d_expert_plan", ptr(ids), int(ids.dtype == torch.int64), t, k, n_experts, ptr(offsets),
-                 ptr(rows), ptr(pairs), ptr(pos), ws, lib.stream())
-    return ExpertPlan(offsets, rows, pairs, pos, n_experts)
+        at = _plan_ws_words(lib, t, k, n_experts)
+        tables = torch.empty(at + 3 * t * k + n_experts + 1, dtype=torch.int32, device=ids.device)      # workspace | the plan's four tables
+        plan = ExpertPlan(tables, at, t, k, n_experts)
+        rows = plan.address(ROWS)
+        lib.call("cg3d_expert_plan", ids.data_ptr(), int(ids.dtype == torch.int64), t, k, n_experts, plan.address(OFFSETS), rows,
+                 plan.address(PAIRS), plan.address(POS), rows - 4 * at if at else None, lib.stream())
+    return plan
 
 
 def _check_rows(who, x, n, plan, what):
-    need(isinstance(plan, ExpertPlan), "%s: plan must come from expert_plan", who)
-    need(isinstance(x, torch.Tensor) and x.dtype in FLOATS, "%s: %s must be float32, bfloat16 or float16", who, what)
-    need(x.dim() == 2 and x.shape[0] == n and x.shape[1] >= 1, "%s: %s must be [%d, C], got %s", who, what, n, tuple(x.shape))
-    need(x.device == plan.pos.device, "%s: %s is on %s, the plan on %s", who, what, x.device, plan.pos.device)
+    if not isinstance(plan, ExpertPlan):
+        raise CG3DError("%s: plan must come from expert_plan" % who)
+    if not (isinstance(x, torch.Tensor) and x.dtype in FLOATS and x.dim() == 2 and x.shape[0] == n and x.shape[1] >= 1):
+        raise CG3DError("%s: %s must be [%d, C] float32, bfloat16 or float16, got %s" % (
+            who, what, n, (x.dtype, tuple(x.shape)) if isinstance(x, torch.Tensor) else type(x)))
+    if x.device != plan.device:
+        raise CG3DError("%s: %s is on %s, the plan on %s" % (who, what, x.device, plan.device))
 
 
-def _gather(x, pos, rows):
+def _gather(x, plan):
     lib = _lib.get()
     x = x.contiguous()
-    lib.check(x, rows)
-    t, k = pos.shape
+    lib.check(x)
     with on_device(x):
-        out = torch.empty((t * k, x.shape[1]), dtype=x.dtype, device=x.device)
-        lib.call("cg3d_expert_gather", ptr(x), DTYPES[x.dtype], ptr(rows), t, k, x.shape[1], ptr(out), lib.stream())
+        out = torch.empty((plan.n_rows, x.shape[1]), dtype=x.dtype, device=x.device)
+        lib.call("cg3d_expert_gather", x.data_ptr(), DTYPES[x.dtype], plan.address(ROWS), plan.n_tokens, plan.k, x.shape[1], out.data_ptr(),
+                 lib.stream())
     return out
 
 
-def _combine(y, pos, w):
+def _combine(y, plan, w):
     lib = _lib.get()
-    lib.check(y, pos, w)
-    t, k = pos.shape
+    lib.check(y, w)
     with on_device(y):
-        out = torch.empty((t, y.shape[1]), dtype=y.dtype, device=y.device)
-        lib.call("cg3d_expert_combine", ptr(y), DTYPES[y.dtype], ptr(pos), ptr(w), 0 if w is None else DTYPES[w.dtype], t, k, y.shape[1],
-                 ptr(out), lib.stream())
+        out = torch.empty((plan.n_tokens, y.shape[1]), dtype=y.dtype, device=y.device)
+        lib.call("cg3d_expert_combine", y.data_ptr(), DTYPES[y.dtype], plan.address(POS), ptr(w), 0 if w is None else DTYPES[w.dtype],
+                 plan.n_tokens, plan.k, y.shape[1], out.data_ptr(), lib.stream())
     return out
 
 
 class _Gather(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, pos, rows):
-        ctx.save_for_backward(pos)
+    def forward(ctx, x, plan):
+        ctx.plan = plan
         ctx.set_materialize_grads(False)
-        return _gather(x, pos, rows)
+        return _gather(x, plan)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        return None if dout is None else _combine(dout.contiguous(), ctx.saved_tensors[0], None), None, None
+        return None if dout is None else _combine(dout.contiguous(), ctx.plan, None), None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, pos, pairs, w):
+    def forward(ctx, y, plan, w):
         y, w = y.contiguous(), None if w is None else w.contiguous()
-        ctx.save_for_backward(y if ctx.needs_input_grad[3] else None, pairs, w)
-        ctx.shape = pos.shape
+        ctx.plan = plan
+        ctx.save_for_backward(y if ctx.needs_input_grad[2] else None, w)
         ctx.set_materialize_grads(False)
-        return _combine(y, pos, w)
+        return _combine(y, plan, w)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         if dout is None:
-            return None, None, None, None
-        y, pairs, w = ctx.saved_tensors
-        (t, k), c = ctx.shape, dout.shape[1]
-        need_dy, _, _, need_dw = ctx.needs_input_grad
+            return None, None, None
+        y, w = ctx.saved_tensors
+        plan, c = ctx.plan, dout.shape[1]
         lib = _lib.get()
         dout = dout.contiguous()
         with on_device(dout):
-            dy = torch.empty((t * k, c), dtype=dout.dtype, device=dout.device) if need_dy else None
-            dw = torch.empty_like(w) if need_dw else None
-            lib.call("cg3d_expert_combine_bwd", ptr(dout), ptr(y), DTYPES[dout.dtype], ptr(pairs), ptr(w), 0 if w is None else DTYPES[w.dtype], t, k, c,
-                     ptr(dy), ptr(dw), lib.stream())
-        return dy, None, None, dw
+            dy = torch.empty((plan.n_rows, c), dtype=dout.dtype, device=dout.device) if ctx.needs_input_grad[0] else None
+            dw = torch.empty_like(w) if ctx.needs_input_grad[2] else None
+            lib.call("cg3d_expert_combine_bwd", dout.data_ptr(), ptr(y), DTYPES[dout.dtype], plan.address(PAIRS), ptr(w),
+                     0 if w is None else DTYPES[w.dtype], plan.n_tokens, plan.k, c, ptr(dy), ptr(dw), lib.stream())
+        return dy, None, dw
 
 
 def expert_gather(x, plan):
     """x [T, C] float32 / bfloat16 / float16 -> [T * k, C], the tokens' rows in the plan's order (differentiable in x)."""
     _check_rows("expert_gather", x, getattr(plan, "n_tokens", 0), plan, "x")
     if not (x.requires_grad and torch.is_grad_enabled()):
-        return _gather(x, plan.pos, plan.rows)
-    return _Gather.apply(x, plan.pos, plan.rows)
+        return _gather(x, plan)
+    return _Gather.apply(x, plan)
 
 
 def expert_combine(rows, plan, weights=None):
@@ -160,9 +179,9 @@ def expert_combine(rows, plan, weights=None):
         need(isinstance(weights, torch.Tensor) and weights.dtype in FLOATS, "expert_combine: weights must be float32, bfloat16 or float16")
         if weights.dim() == 1 and plan.k == 1:
             weights = weights.unsqueeze(1)
-        need(tuple(weights.shape) == (plan.n_tokens, plan.k), "expert_combine: weights must be [%d, %d], got %s", plan.n_tokens, plan.k,
-             tuple(weights.shape))
-        need(weights.device == rows.device, "expert_combine: weights are on %s, rows on %s", weights.device, rows.device)
+        if weights.shape != (plan.n_tokens, plan.k) or weights.device != rows.device:
+            raise CG3DError("expert_combine: weights must be [%d, %d] on %s, got %s on %s" % (plan.n_tokens, plan.k, rows.device,
+                                                                                              tuple(weights.shape), weights.device))
     if not (torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))):
-        return _combine(rows.contiguous(), plan.pos, None if weights is None else weights.contiguous())
-    return _Combine.apply(rows, plan.pos, plan.pairs, weights)
+        return _combine(rows.contiguous(), plan, None if weights is None else weights.contiguous())
+    return _Combine.apply(rows, plan, weights)

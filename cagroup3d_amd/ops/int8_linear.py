@@ -9,12 +9,15 @@ its own for each expert's rows: the served form of the kernel-size-1 convolution
 
 The integer sums are exact, so results do not depend on how the work is split.  There is no gradient: a call on inputs that require
 one, with gradients enabled, is refused."""
+import functools
+
 import torch
 
 from .. import _lib
-from .._lib import ptr
-from .expert_rows import DTYPES, FLOATS, ExpertPlan, need, on_device
+from .._lib import CG3DError, ptr
+from .expert_rows import DTYPES, FLOATS, OFFSETS, ROWS, ExpertPlan, need, on_device
 
+ROWS_IN = tuple(DTYPES)
 MAX_CIN = 131071                  # the int32 sum of so many products of 8-bit values cannot overflow
 
 
@@ -66,9 +69,14 @@ def int8_weight(w, scale=None):
 
 
 def _rows_in(who, x, dtypes):
-    need(isinstance(x, torch.Tensor) and x.dtype in dtypes and x.dim() == 2, "%s: x must be [rows, cin] of %s", who,
-         " / ".join(str(d).replace("torch.", "") for d in dtypes))
-    need(1 <= x.shape[1] <= MAX_CIN and x.shape[0] < 2 ** 31, "%s: x of shape %s (cin in 1 .. %d)", who, tuple(x.shape), MAX_CIN)
+    if not (isinstance(x, torch.Tensor) and x.dtype in dtypes and x.dim() == 2 and 1 <= x.shape[1] <= MAX_CIN and x.shape[0] < 2 ** 31):
+        raise CG3DError("%s: x must be [rows, cin] of %s with cin in 1 .. %d, got %s" % (
+            who, " / ".join(str(d).replace("torch.", "") for d in dtypes), MAX_CIN, (x.dtype, tuple(x.shape)) if isinstance(x, torch.Tensor) else type(x)))
+
+
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(lib, *sizes):
+    return int(lib.raw("cg3d_int8_linear_ws_bytes")(*sizes))
 
 
 def quantize_rows(x):
@@ -96,44 +104,47 @@ def int8_linear(x, weight, bias=None, scale=None, out_dtype=None, plan=None, gat
     plan's rows ([T * k, cin], what expert_gather gives), or with gather=True the tokens ([T, cin]), whose rows are picked in the
     product -- quantised once for a token, not once for a row.  Rows behind the last are zeros."""
     need(isinstance(weight, Int8Weight), "int8_linear: weight must come from int8_weight")
-    _rows_in("int8_linear", x, tuple(DTYPES))
+    _rows_in("int8_linear", x, ROWS_IN)
     need(x.shape[1] == weight.cin, "int8_linear: x has %d columns, weight %d rows", x.shape[1], weight.cin)
-    out_dtype = out_dtype or (torch.float32 if x.dtype == torch.int8 else x.dtype)
+    in8 = x.dtype == torch.int8
+    out_dtype = out_dtype or (torch.float32 if in8 else x.dtype)
     need(out_dtype in FLOATS, "int8_linear: out_dtype must be float32, bfloat16 or float16")
-    if x.dtype == torch.int8:
-        need(isinstance(scale, torch.Tensor) and scale.dtype == torch.float32 and tuple(scale.shape) == (x.shape[0],),
-             "int8_linear: rows in 8 bits need their scale, float32 [%d]", x.shape[0])
+    n_x = n_rows = x.shape[0]
+    if in8:
+        need(isinstance(scale, torch.Tensor) and scale.dtype == torch.float32 and scale.shape == (n_x,),
+             "int8_linear: rows in 8 bits need their scale, float32 [%d]", n_x)
     else:
         need(scale is None, "int8_linear: the scale of rows in floats is computed here")
     if plan is None:
         need(weight.n_experts == 1 and not gather, "int8_linear: %d matrices (or gather) need a plan", weight.n_experts)
-        n_rows = x.shape[0]
     else:
         need(isinstance(plan, ExpertPlan), "int8_linear: plan must come from expert_plan")
         need(weight.n_experts == plan.n_experts, "int8_linear: %d matrices for a plan of %d experts", weight.n_experts, plan.n_experts)
         n_rows = plan.n_rows
-        n_x = plan.n_tokens if gather else n_rows
-        need(x.shape[0] == n_x, "int8_linear: x has %d rows, the plan %d", x.shape[0], n_x)
-    per_expert = bias is not None and bias.dim() == 2
+        need(n_x == (plan.n_tokens if gather else n_rows), "int8_linear: x has %d rows, the plan %d tokens and %d rows", n_x, plan.n_tokens, n_rows)
+    per_expert = 0
     if bias is not None:
-        need(bias.dtype in FLOATS and tuple(bias.shape) in ((weight.cout,), (weight.n_experts, weight.cout) if weight.grouped else ()),
-             "int8_linear: bias must be floats [%d]%s, got %s", weight.cout,
-             " or [%d, %d]" % (weight.n_experts, weight.cout) if weight.grouped else "", tuple(bias.shape))
+        per_expert = int(bias.dim() == 2)
+        if bias.dtype not in FLOATS or not (bias.shape == (weight.cout,) or (weight.grouped and bias.shape == (weight.n_experts, weight.cout))):
+            raise CG3DError("int8_linear: bias must be floats [%d]%s, got %s" % (
+                weight.cout, " or [%d, %d]" % (weight.n_experts, weight.cout) if weight.grouped else "", tuple(bias.shape)))
     _no_grad_for("int8_linear", x, bias, scale)
-    for t in (weight.packed, bias, scale, plan and plan.offsets):
-        need(t is None or t.device == x.device, "int8_linear: x is on %s, another argument on %s", x.device, t is not None and t.device)
+    for t in (weight, bias, scale, plan):
+        if t is not None and t.device != x.device:
+            raise CG3DError("int8_linear: x is on %s, another argument on %s" % (x.device, t.device))
     lib = _lib.get()
-    x = x.detach().contiguous()
-    bias = None if bias is None else bias.detach().to(torch.float32).contiguous()
-    scale = None if scale is None else scale.detach().contiguous()
+    x = x.contiguous()
+    if bias is not None:
+        bias = bias.detach().to(torch.float32).contiguous()
+    if scale is not None:
+        scale = scale.contiguous()
     lib.check(x, bias, scale)
+    code = DTYPES[x.dtype]
     with on_device(x):
+        ws_bytes = _ws_bytes(lib, code, n_x, weight.cin, n_rows, weight.cout, weight.n_experts, int(plan is not None))
         y = torch.empty((n_rows, weight.cout), dtype=out_dtype, device=x.device)
-        ws_bytes = int(lib.raw("cg3d_int8_linear_ws_bytes")(DTYPES[x.dtype], x.shape[0], weight.cin, n_rows, weight.cout, weight.n_experts,
-                                                            int(plan is not None)))
         ws = torch.empty(ws_bytes, dtype=torch.int8, device=x.device) if ws_bytes > 0 else None
-        lib.call("cg3d_int8_linear", ptr(x), DTYPES[x.dtype], ptr(scale), x.shape[0], weight.cin, ptr(weight.packed),
-                 ptr(weight.scale), ptr(bias), int(per_expert), ptr(plan.offsets) if plan else None,
-                 ptr(plan.rows) if plan and gather else None, ptr(y), DTYPES[out_dtype], n_rows, weight.cout,
-                 weight.n_experts, ptr(ws), lib.stream())
+        lib.call("cg3d_int8_linear", x.data_ptr(), code, ptr(scale), n_x, weight.cin, weight.packed.data_ptr(), weight.scale.data_ptr(), ptr(bias),
+                 per_expert, None if plan is None else plan.address(OFFSETS), plan.address(ROWS) if gather else None, y.data_ptr(),
+                 DTYPES[out_dtype], n_rows, weight.cout, weight.n_experts, ptr(ws), lib.stream())
     return y
