@@ -15,22 +15,24 @@
 //   rounding, and only for the other k (fp16; bf16 has none, ma < 2^8) a row's elements are looked at like those of fp32 rows.
 // A row that holds an infinity or a NaN gets the scale NaN (and so a row of NaN as its result); a row of zeros the scale 0.
 //
-// The weights are the MFMA's A operand and the rows its B operand (v_mfma_i32_16x16x64_i8), i.e. a tile of the product is
-// D[channel][row]: a lane then holds neighbouring channels of ONE row, its row scale is one register, and the result leaves in
-// 16-byte stores without a detour through LDS.  Weights are laid out once (cg3d_int8_weight): [expert][panel of 64 channels][chunk
-// of 64 contraction steps][tile nb of 4][lane][16 bytes]; lane (g = lane / 16, m = lane % 16) holds contraction steps
-// 16 g .. 16 g + 15 of the channel (nb / 2) * 32 + (m / 4) * 8 + (nb % 2) * 4 + m % 4 of the panel, so that the results of tiles nb = 0, 1
-// (2, 3) in a lane are 8 consecutive channels.  Channels and contraction steps past the end are zeros.
+// A tile of the product is v_mfma_i32_16x16x64_i8 with the rows as A and the weights as B operand.  The weights are laid out once
+// (cg3d_int8_weight): [expert][panel of 64 channels][chunk of 64 contraction steps][tile nb of 4][lane][16 bytes]; lane (g = lane / 16,
+// m = lane % 16) of tile nb holds contraction steps 16 g .. 16 g + 15 of channel 4 m + nb of the panel, so that a lane's results of
+// the four tiles are 4 neighbouring channels and 16 neighbouring lanes store a whole line of a row.  Channels and contraction steps
+// past the end are zeros.
 #include "cg3d_common.h"
 #pragma clang fp contract(off)      // a result has the same bits on every path
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));      // a row may start at any multiple of its element
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 
 #define I8_MAX_CIN 131071            // 2^14 * 131071 < 2^31: -128 * -128 included
 #define I8_MAX_EXPERTS 1024
 #define I8_FUSED_CIN 512
-#define I8_LONG 513
 #define I8_SPLIT 256
+#define I8_WANT 384
 
 template <typename T, int V> struct __attribute__((packed, aligned(1))) i8_vec { T e[V]; };
 
@@ -41,55 +43,44 @@ static __device__ __forceinline__ float i8_f(i8_bf16 a) { return __uint_as_float
 static __device__ __forceinline__ float i8_f(i8_f16 a) { return (float)__builtin_bit_cast(_Float16, a.v); }
 static __device__ __forceinline__ uint32_t i8_abs(float f) { return __float_as_uint(f) & 0x7fffffffu; }   // ordered like |f|; infinity and NaN on top
 
-// 16 neighbouring elements of a row as they lie in memory, in whole registers (a row may start at any multiple of its element)
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
-template <typename T> struct i8_raw {
-    u32x4 w[sizeof(T)];
-    __device__ __forceinline__ float operator[](int j) const {
-        if constexpr (sizeof(T) == 4) return __uint_as_float(w[j >> 2][j & 3]);
-        else {
-            const uint32_t d = w[j >> 3][(j >> 1) & 3];
-            if constexpr (__is_same(T, i8_bf16)) return __uint_as_float(j & 1 ? d & 0xffff0000u : d << 16);
-            else return (float)__builtin_bit_cast(_Float16, (uint16_t)(j & 1 ? d >> 16 : d));
-        }
+// ---------------------------------------------------------------- pieces of rows: 16 bytes, i8_els<T> elements, in whole registers
+template <typename T> static constexpr int i8_els = 16 / (int)sizeof(T);
+template <typename T> static __device__ __forceinline__ float i8_el(const u32x4 &w, int j) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+    else {
+        const uint32_t d = w[j >> 1];
+        if constexpr (__is_same(T, i8_bf16)) return __uint_as_float(j & 1 ? d & 0xffff0000u : d << 16);
+        else return (float)__builtin_bit_cast(_Float16, (uint16_t)(j & 1 ? d >> 16 : d));
     }
-};
-// elements k0 .. k0 + 15 of a row of cin, zeros behind its end
-template <typename T>
-static __device__ __forceinline__ i8_raw<T> i8_get16(const T *__restrict__ xr, int k0, int cin) {
-    i8_raw<T> v;
+}
+// the piece at element k0 of a row of cin, zeros behind its end
+template <typename T> static __device__ __forceinline__ u32x4 i8_piece(const T *__restrict__ xr, int k0, int cin) {
+    constexpr int N = i8_els<T>, PER = 4 / (int)sizeof(T);           // PER: elements of a register
+    u32x4 w = {0, 0, 0, 0};
+    if (k0 + N <= cin) w = *reinterpret_cast<const u32x4_any *>(xr + k0);
+    else if (k0 < cin) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T); i++) v.w[i] = u32x4{0, 0, 0, 0};
-    if (k0 + 16 <= cin) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T); i++) v.w[i] = reinterpret_cast<const u32x4_any *>(xr + k0)[i];
-    } else if (k0 < cin) {
-        constexpr int PER = 4 / sizeof(T);               // elements of a register
-#pragma unroll
-        for (int j = 0; j < 15; j++)
+        for (int j = 0; j < N - 1; j++)
             if (k0 + j < cin) {
                 uint32_t d = 0;
                 __builtin_memcpy(&d, xr + k0 + j, sizeof(T));
-                v.w[j / (4 * PER)][(j / PER) & 3] |= d << (j % PER * 8 * (int)sizeof(T));
+                w[j / PER] |= d << (j % PER * 8 * (int)sizeof(T));
             }
     }
-    return v;
+    return w;
 }
 // the running maximum of |.|: fp32 bits, or for 16-bit floats two at a time (their bits are ordered like their magnitudes too)
 template <typename T> struct i8_max {
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     uint32_t v = 0;
-    __device__ __forceinline__ void add(const i8_raw<T> &r) {
+    __device__ __forceinline__ void add(const u32x4 &w) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T); i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if constexpr (sizeof(T) == 4) v = max(v, r.w[i][j] & 0x7fffffffu);
-                else v = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, v), __builtin_bit_cast(u16x2, r.w[i][j] & 0x7fff7fffu)));
-            }
+        for (int j = 0; j < 4; j++) {
+            if constexpr (sizeof(T) == 4) v = max(v, w[j] & 0x7fffffffu);
+            else v = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, v), __builtin_bit_cast(u16x2, w[j] & 0x7fff7fffu)));
+        }
     }
-    __device__ __forceinline__ uint32_t bits() const {    // of the fp32 value
+    __device__ __forceinline__ uint32_t bits() const {                // of the fp32 value
         if constexpr (sizeof(T) == 4) return v;
         else {
             T t;
@@ -98,6 +89,21 @@ template <typename T> struct i8_max {
         }
     }
 };
+template <int CTRL> static __device__ __forceinline__ uint32_t i8_dpp(uint32_t v) {      // from another lane of 4, 8 or 16
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+// the maximum over L = 4, 8, 16 or 64 neighbouring lanes, in all of them
+template <int L> static __device__ __forceinline__ uint32_t i8_max_of(uint32_t v) {
+    v = max(v, i8_dpp<0xb1>(v));                                      // quad_perm: lane ^ 1
+    v = max(v, i8_dpp<0x4e>(v));                                      // quad_perm: lane ^ 2
+    if constexpr (L >= 8) v = max(v, i8_dpp<0x141>(v));               // row_half_mirror: 7 - lane of 8
+    if constexpr (L >= 16) v = max(v, i8_dpp<0x140>(v));              // row_mirror: 15 - lane of 16
+    if constexpr (L >= 64) {
+        v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+        v = max(v, (uint32_t)__shfl_xor((int)v, 32));
+    }
+    return v;
+}
 
 // What a row's largest magnitude (its bits) makes of the row's elements.  Rows whose largest is below 2^-96 or from 2^112 on are
 // shifted by a power of two first (`shift`, exact for every element that is not level 0), so that no product here leaves the range.
@@ -105,6 +111,7 @@ struct i8_level {
     float amax, c, shift, scale;
     uint32_t keep;                                       // 0: the row has no levels
     bool fine127;                                        // max / 127 is exact, 127 / max is not
+    i8_level() = default;
     __device__ __forceinline__ explicit i8_level(uint32_t top) {
         const float a = __uint_as_float(top);
         const bool fine = top < 0x7f800000u;
@@ -129,63 +136,76 @@ static __device__ __forceinline__ float i8_decide(const i8_level &v, float x, fl
     const bool down = less || (same && ((int)n & 1));
     return down ? r - copysignf(1.f, r - I8_MAGIC) : r;
 }
-// 16 elements (shifted) of one row -> 16 levels.  T: what the elements were
-template <typename T>
-static __device__ __forceinline__ i32x4 i8_quant16(const i8_level &v, const float (&x)[16]) {
-    float r[16];
+// N elements (shifted) of one row -> N levels, 4 to a word.  T: what the elements were
+template <typename T, int N>
+static __device__ __forceinline__ void i8_quant(const i8_level &v, const float (&x)[N], uint32_t (&out)[N / 4]) {
+    float r[N];
     bool look = false;
 #pragma unroll
-    for (int j = 0; j < 16; j++) r[j] = __builtin_fmaf(x[j], v.c, I8_MAGIC);
+    for (int j = 0; j < N; j++) r[j] = __builtin_fmaf(x[j], v.c, I8_MAGIC);
     if constexpr (sizeof(T) == 4) {
         float most = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; j++) most = fmaxf(most, fabsf(__builtin_fmaf(x[j], v.c, I8_MAGIC - r[j])));
+        for (int j = 0; j < N; j++) most = fmaxf(most, fabsf(__builtin_fmaf(x[j], v.c, I8_MAGIC - r[j])));
         look = most > 0.5f - 0x1p-16f;
     } else if constexpr (__is_same(T, i8_f16)) look = v.fine127;
     if (!__is_same(T, i8_bf16) && __builtin_expect(__any(look), 0)) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
+        for (int j = 0; j < N; j++) {
             const float n = r[j] - I8_MAGIC, d = __builtin_fmaf(x[j], v.c, -n);
             if (d * n < 0.f && fabsf(d) > 0.5f - 0x1p-16f) r[j] = i8_decide(v, x[j], r[j]);     // (n = 0 is nearest from either side)
         }
     }
-    i32x4 o;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < N / 4; i++) {
         const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(r[4 * i + 1]), __float_as_uint(r[4 * i]), 0x0c0c0400u);
         const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(r[4 * i + 3]), __float_as_uint(r[4 * i + 2]), 0x04000c0cu);
-        o[i] = (int)((lo | hi) & v.keep);
+        out[i] = (lo | hi) & v.keep;
+    }
+}
+// the levels of a piece: i8_els<T> bytes
+template <typename T> struct i8_lev { uint32_t w[i8_els<T> / 4]; };
+template <typename T>
+static __device__ __forceinline__ i8_lev<T> i8_levels(const i8_level &lev, bool far, const u32x4 &w) {
+    constexpr int N = i8_els<T>;
+    i8_lev<T> o;
+    if constexpr (sizeof(T) == 1) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) o.w[j] = w[j];
+    } else {
+        float f[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) f[j] = i8_el<T>(w, j);
+        if (far) {
+#pragma unroll
+            for (int j = 0; j < N; j++) f[j] *= lev.shift;
+        }
+        i8_quant<T, N>(lev, f, o.w);
     }
     return o;
 }
 
-template <typename T>
-static __device__ __forceinline__ i32x4 i8_levels16(const i8_level &lev, bool far, const i8_raw<T> &v) {
-    float f[16];
-#pragma unroll
-    for (int j = 0; j < 16; j++) f[j] = v[j];
-    if (far) {
-#pragma unroll
-        for (int j = 0; j < 16; j++) f[j] *= lev.shift;
-    }
-    return i8_quant16<T>(lev, f);
-}
-
 // ---------------------------------------------------------------- weights (once per model)
-// w [E][cin][cout]: a thread owns a channel, reads along the contraction are rows of the matrix
+// w [E][cin][cout]: a thread of 16 to a channel, reads along the contraction are rows of the matrix
 template <typename T>
-__global__ __launch_bounds__(256) void k_i8_weight_scale(const T *__restrict__ w, int32_t cin, int32_t cout, float *__restrict__ scale,
-                                                         uint32_t *__restrict__ top) {
-    const int n = blockIdx.x * 256 + threadIdx.x, e = blockIdx.y;
-    if (n >= cout) return;
-    const T *p = w + (int64_t)e * cin * cout + n;
+__global__ __launch_bounds__(1024) void k_i8_weight_scale(const T *__restrict__ w, int32_t cin, int32_t cout, float *__restrict__ scale,
+                                                          uint32_t *__restrict__ top) {
+    __shared__ uint32_t sh[16][64];
+    const int n = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6, e = blockIdx.y;
     uint32_t m = 0;
-    for (int k = 0; k < cin; k++) m = max(m, i8_abs(i8_f(p[(int64_t)k * cout])));
+    if (n < cout) {
+        const T *p = w + (int64_t)e * cin * cout + n;
+#pragma unroll 4
+        for (int k = part; k < cin; k += 16) m = max(m, i8_abs(i8_f(p[(int64_t)k * cout])));
+    }
+    sh[part][threadIdx.x & 63] = m;
+    __syncthreads();
+    if (part || n >= cout) return;
+#pragma unroll
+    for (int i = 1; i < 16; i++) m = max(m, sh[i][threadIdx.x]);
     scale[(int64_t)e * cout + n] = i8_level(m).scale;
     top[(int64_t)e * cout + n] = m;
 }
-static __device__ __forceinline__ int i8_channel(int nb, int m) { return (nb >> 1) * 32 + (m >> 2) * 8 + (nb & 1) * 4 + (m & 3); }
-
 // a thread writes the 16 bytes of one lane of one fragment (top == NULL: w is in 8 bits already)
 template <typename T>
 __global__ __launch_bounds__(256) void k_i8_weight_pack(const T *__restrict__ w, const uint32_t *__restrict__ top, int32_t cin, int32_t cout,
@@ -194,19 +214,21 @@ __global__ __launch_bounds__(256) void k_i8_weight_pack(const T *__restrict__ w,
         const int lane = (int)(i & 63), nb = (int)((i >> 6) & 3);
         const int64_t u = i >> 8;
         const int c = (int)(u % chunks), p = (int)((u / chunks) % panels), e = (int)(u / chunks / panels);
-        const int n = p * 64 + i8_channel(nb, lane & 15), k0 = c * 64 + (lane >> 4) * 16;
+        const int n = p * 64 + (lane & 15) * 4 + nb, k0 = c * 64 + (lane >> 4) * 16;
         const bool there = n < cout;
         const T *src = w + (int64_t)e * cin * cout + (there ? n : 0);
-        union { int8_t b[16]; i32x4 v; } o;
+        union { int8_t b[16]; uint32_t w[4]; u32x4 v; } o;
         if constexpr (sizeof(T) == 1) {
+#pragma unroll
             for (int j = 0; j < 16; j++) o.b[j] = there && k0 + j < cin ? (int8_t)src[(int64_t)(k0 + j) * cout] : 0;
         } else {
             const i8_level lev(there ? top[(int64_t)e * cout + n] : 0);
             float f[16];
+#pragma unroll
             for (int j = 0; j < 16; j++) f[j] = there && k0 + j < cin ? i8_f(src[(int64_t)(k0 + j) * cout]) * lev.shift : 0.f;
-            o.v = i8_quant16<T>(lev, f);
+            i8_quant<T, 16>(lev, f, o.w);
         }
-        reinterpret_cast<i32x4 *>(out)[i] = o.v;
+        reinterpret_cast<u32x4 *>(out)[i] = o.v;
     }
 }
 
@@ -231,7 +253,7 @@ extern "C" int cg3d_int8_weight(const void *w, int32_t dtype, int32_t n_experts,
     uint32_t *top = reinterpret_cast<uint32_t *>(ws);
 #define I8_W(T)                                                                                                                     \
     do {                                                                                                                            \
-        hipLaunchKernelGGL((k_i8_weight_scale<T>), dim3((unsigned)cg3d_divup(cout, 256), (unsigned)n_experts), dim3(256), 0, s,     \
+        hipLaunchKernelGGL((k_i8_weight_scale<T>), dim3((unsigned)cg3d_divup(cout, 64), (unsigned)n_experts), dim3(1024), 0, s,     \
                            reinterpret_cast<const T *>(w), cin, cout, scale, top);                                                  \
         CG3D_CHECK_LAUNCH();                                                                                                        \
         hipLaunchKernelGGL((k_i8_weight_pack<T>), dim3(nb), dim3(256), 0, s, reinterpret_cast<const T *>(w), top, cin, cout, panels, \
@@ -249,58 +271,64 @@ extern "C" int cg3d_int8_weight(const void *w, int32_t dtype, int32_t n_experts,
 }
 
 // ---------------------------------------------------------------- rows
-// A group of L lanes (a power of two) owns one row, 16 elements of a lane at a time; the row is read a second time (from the
-// caches) for its levels.  Bytes [cin, pitch) are zeros.
-template <typename T, int B>
-__global__ __launch_bounds__(B) void k_i8_rows(const T *__restrict__ x, int64_t n, int32_t cin, int64_t pitch, int32_t lshift,
-                                               int8_t *__restrict__ q, float *__restrict__ scale) {
-    __shared__ uint32_t sh[B / 64];
-    const int L = 1 << lshift, lane = threadIdx.x & (L - 1);
-    const int nv = (cin + 15) >> 4;
-    for (int64_t r = (blockIdx.x * (int64_t)B + threadIdx.x) >> lshift; r < n; r += ((int64_t)gridDim.x * B) >> lshift) {
-        const T *row = x + r * cin;
-        i8_max<T> most;
-        for (int v = lane; v < nv; v += L) most.add(i8_get16<T>(row, v * 16, cin));
-        uint32_t top = most.bits();
-        for (int d = (L < 64 ? L : 64) >> 1; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-        if (L > 64) {                                     // (L == B: the workgroup owns the row)
-            if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
-            __syncthreads();
+template <typename T> static __device__ __forceinline__ void i8_put_levels(int8_t *__restrict__ dst, int64_t k0, int64_t pitch, const i8_lev<T> &o) {
+    constexpr int N = i8_els<T>;
+    if (k0 + N <= pitch) {
+        if constexpr (N == 4) *reinterpret_cast<i8_vec<uint32_t, 1> *>(dst + k0) = __builtin_bit_cast(i8_vec<uint32_t, 1>, o);
+        else *reinterpret_cast<u32x2_any *>(dst + k0) = __builtin_bit_cast(u32x2_any, o);
+    } else {
+        const i8_vec<int8_t, N> b = __builtin_bit_cast(i8_vec<int8_t, N>, o);
 #pragma unroll
-            for (int w = 0; w < B / 64; w++) top = max(top, sh[w]);
-            __syncthreads();
-        }
-        const i8_level lev(top);
-        if (lane == 0) scale[r] = lev.scale;
-        int8_t *dst = q + r * pitch;
-        for (int v = lane; v < nv; v += L) {
-            const i32x4 lv = i8_levels16<T>(lev, lev.shifted(), i8_get16<T>(row, v * 16, cin));
-            const i8_vec<int8_t, 16> o = __builtin_bit_cast(i8_vec<int8_t, 16>, lv);
-            if (v * 16 + 16 <= pitch) *reinterpret_cast<i8_vec<int8_t, 16> *>(dst + v * 16) = o;
-            else
-                for (int j = 0; j < 16; j++)
-                    if (v * 16 + j < pitch) dst[v * 16 + j] = o.e[j];
-        }
-        for (int64_t a = nv * 16ll + lane; a < pitch; a += L) dst[a] = 0;
+        for (int j = 0; j < N - 1; j++)
+            if (k0 + j < pitch) dst[k0 + j] = b.e[j];
     }
 }
-// Long rows, one to a workgroup of B threads, held in registers between the maximum and the levels: KEEP * B * 16 elements at most.
-// (512 rows of 43 904 fp32: ... us with 16 waves and 3 pieces each, 36 with 8 and 6, 31 reading the row twice with 4.)
-template <typename T, int KEEP, int B>
-__global__ __launch_bounds__(B) void k_i8_long_rows(const T *__restrict__ x, int64_t n, int32_t cin, int64_t pitch, int8_t *__restrict__ q,
-                                                      float *__restrict__ scale) {
-    __shared__ uint32_t sh[B / 64];
-    const int tid = threadIdx.x;
-    for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
+// L lanes (a power of two, at most a wave) own one row of at most L * KEEP pieces and hold it in registers: as few lanes as KEEP
+// pieces of each allow (with 64 lanes and one piece 100 000 x 512 bf16 took 39.5 us, with 16 and four 28)
+template <typename T>
+__global__ __launch_bounds__(256) void k_i8_rows(const T *__restrict__ x, int64_t n, int32_t cin, int64_t pitch, int32_t lshift,
+                                                 int8_t *__restrict__ q, float *__restrict__ scale) {
+    constexpr int N = i8_els<T>, KEEP = 4;
+    const int L = 1 << lshift, lane = threadIdx.x & (L - 1);
+    for (int64_t r = (blockIdx.x * 256ll + threadIdx.x) >> lshift; r < n; r += (gridDim.x * 256ll) >> lshift) {
         const T *row = x + r * cin;
-        i8_raw<T> v[KEEP];
+        u32x4 v[KEEP];
         i8_max<T> most;
 #pragma unroll
-        for (int i = 0; i < KEEP; i++) v[i] = i8_get16<T>(row, (i * B + tid) * 16, cin);
+        for (int i = 0; i < KEEP; i++) v[i] = i8_piece<T>(row, (i * L + lane) * N, cin);
 #pragma unroll
         for (int i = 0; i < KEEP; i++) most.add(v[i]);
         uint32_t top = most.bits();
-        for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        for (int d = L >> 1; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        const i8_level lev(top);
+        if (lane == 0) scale[r] = lev.scale;
+        int8_t *dst = q + r * pitch;
+#pragma unroll
+        for (int i = 0; i < KEEP; i++) {
+            const int k0 = (i * L + lane) * N;
+            if (k0 < pitch) i8_put_levels<T>(dst, k0, pitch, i8_levels<T>(lev, lev.shifted(), v[i]));
+        }
+        for (int64_t a = (int64_t)KEEP * L * N + lane; a < pitch; a += L) dst[a] = 0;
+    }
+}
+// longer rows, one to a workgroup of B threads; rows of more than B * KEEP pieces are read again for their levels
+template <typename T, int B, int KEEP>
+__global__ __launch_bounds__(B) void k_i8_long_rows(const T *__restrict__ x, int64_t n, int32_t cin, int64_t pitch, int8_t *__restrict__ q,
+                                                    float *__restrict__ scale) {
+    constexpr int N = i8_els<T>;
+    __shared__ uint32_t sh[B / 64];
+    const int tid = threadIdx.x, step = B * KEEP * N;
+    for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
+        const T *row = x + r * cin;
+        u32x4 v[KEEP];
+        i8_max<T> most;
+        for (int a = 0; a < cin; a += step) {
+#pragma unroll
+            for (int i = 0; i < KEEP; i++) v[i] = i8_piece<T>(row, a + (i * B + tid) * N, cin);
+#pragma unroll
+            for (int i = 0; i < KEEP; i++) most.add(v[i]);
+        }
+        uint32_t top = i8_max_of<64>(most.bits());
         if ((tid & 63) == 0) sh[tid >> 6] = top;
         __syncthreads();
 #pragma unroll
@@ -309,49 +337,43 @@ __global__ __launch_bounds__(B) void k_i8_long_rows(const T *__restrict__ x, int
         const i8_level lev(top);
         if (tid == 0) scale[r] = lev.scale;
         int8_t *dst = q + r * pitch;
+        for (int64_t a = 0; a < pitch; a += step) {
+            if (cin > step) {
 #pragma unroll
-        for (int i = 0; i < KEEP; i++) {
-            const int64_t k0 = (int64_t)(i * B + tid) * 16;
-            if (k0 >= pitch) break;
-            const i32x4 lv = i8_levels16<T>(lev, lev.shifted(), v[i]);
-            if (k0 + 16 <= pitch) *reinterpret_cast<u32x4_any *>(dst + k0) = __builtin_bit_cast(u32x4, lv);
-            else {
-                const i8_vec<int8_t, 16> o = __builtin_bit_cast(i8_vec<int8_t, 16>, lv);
+                for (int i = 0; i < KEEP; i++) v[i] = i8_piece<T>(row, (int)a + (i * B + tid) * N, cin);
+            }
 #pragma unroll
-                for (int j = 0; j < 15; j++)
-                    if (k0 + j < pitch) dst[k0 + j] = o.e[j];
+            for (int i = 0; i < KEEP; i++) {
+                const int64_t k0 = a + (i * B + tid) * N;
+                if (k0 < pitch) i8_put_levels<T>(dst, k0, pitch, i8_levels<T>(lev, lev.shifted(), a < cin ? v[i] : u32x4{0, 0, 0, 0}));
             }
         }
-        for (int64_t a = (int64_t)KEEP * B * 16 + tid; a < pitch; a += B) dst[a] = 0;
     }
+}
+template <typename T>
+static void i8_launch_rows(const T *x, int64_t n, int32_t cin, int64_t pitch, int8_t *q, float *scale, hipStream_t s) {
+    constexpr int N = i8_els<T>, F = (int)sizeof(T) / 2;             // F: an fp32 row has twice the pieces
+    const int32_t np = (cin + N - 1) / N;
+    int32_t ls = 0;
+    while ((4 << ls) < np && ls < 6) ls++;
+    const int64_t waves = cg3d_divup(n << ls, 256);
+    const dim3 gw((unsigned)(waves < (1 << 22) ? waves : (1 << 22))), gb((unsigned)(n < (1 << 20) ? n : (1 << 20)));
+    if (np <= 256) hipLaunchKernelGGL((k_i8_rows<T>), gw, dim3(256), 0, s, x, n, cin, pitch, ls, q, scale);
+    else if (cin <= 2048) hipLaunchKernelGGL((k_i8_long_rows<T, 128, 2 * F>), gb, dim3(128), 0, s, x, n, cin, pitch, q, scale);
+    else if (cin <= 4096) hipLaunchKernelGGL((k_i8_long_rows<T, 256, 2 * F>), gb, dim3(256), 0, s, x, n, cin, pitch, q, scale);
+    else if (cin <= 8192) hipLaunchKernelGGL((k_i8_long_rows<T, 512, 2 * F>), gb, dim3(512), 0, s, x, n, cin, pitch, q, scale);
+    else if (cin <= 16384) hipLaunchKernelGGL((k_i8_long_rows<T, 1024, 2 * F>), gb, dim3(1024), 0, s, x, n, cin, pitch, q, scale);
+    else hipLaunchKernelGGL((k_i8_long_rows<T, 1024, 6 * F>), gb, dim3(1024), 0, s, x, n, cin, pitch, q, scale);
 }
 extern "C" int cg3d_int8_quantize_rows(const void *x, int32_t dtype, int64_t n, int32_t cin, int64_t pitch, int8_t *q, float *scale,
                                        cg3d_stream_t stream) {
-    if (dtype < CG3D_DT_F32 || dtype > CG3D_DT_F16 || n < 0 || cin < 1 || cin > I8_MAX_CIN || pitch < cin) return CG3D_ERR_ARG;
+    if (dtype < CG3D_DT_F32 || dtype > CG3D_DT_F16 || n < 0 || cin < 1 || cin > I8_MAX_CIN || pitch < cin || pitch > (1 << 30)) return CG3D_ERR_ARG;
     if (n == 0) return CG3D_OK;
     if (!x || !q || !scale || ((uintptr_t)x & (dtype == CG3D_DT_F32 ? 3 : 1)) || ((uintptr_t)scale & 3)) return CG3D_ERR_ARG;
     hipStream_t s = cg3d_hs(stream);
-    int32_t ls = 0;
-    const int32_t nv = (cin + 15) / 16;
-    if (cin >= I8_LONG && cin <= 3 * 16384) {             // whole rows in a workgroup's registers; beyond that they are read twice
-        const unsigned nb = (unsigned)(n < (1 << 21) ? n : (1 << 21));
-#define I8_L(T, K, B) hipLaunchKernelGGL((k_i8_long_rows<T, K, B>), dim3(nb), dim3(B), 0, s, reinterpret_cast<const T *>(x), n, cin, pitch, q, scale)
-#define I8_LK(T) do { if (cin <= 1024) I8_L(T, 1, 64); else if (cin <= 2048) I8_L(T, 1, 128); else if (cin <= 4096) I8_L(T, 1, 256); else if (cin <= 8192) I8_L(T, 1, 512); else if (cin <= 16384) I8_L(T, 1, 1024); else if (cin <= 2 * 16384) I8_L(T, 2, 1024); else I8_L(T, 3, 1024); } while (0)
-        if (dtype == CG3D_DT_F32) I8_LK(float);
-        else if (dtype == CG3D_DT_BF16) I8_LK(i8_bf16);
-        else I8_LK(i8_f16);
-#undef I8_LK
-#undef I8_L
-        CG3D_CHECK_LAUNCH();
-        return CG3D_OK;
-    }
-    while ((1 << ls) < nv && ls < 6) ls++;
-    if (nv > 4 * 64) ls = 8;                              // a long row: the whole workgroup
-    int64_t nb = cg3d_divup(n << ls, 256);
-    if (nb > (1 << 22)) nb = 1 << 22;
-    if (dtype == CG3D_DT_F32) hipLaunchKernelGGL((k_i8_rows<float, 256>), dim3((unsigned)nb), dim3(256), 0, s, reinterpret_cast<const float *>(x), n, cin, pitch, ls, q, scale);
-    else if (dtype == CG3D_DT_BF16) hipLaunchKernelGGL((k_i8_rows<i8_bf16, 256>), dim3((unsigned)nb), dim3(256), 0, s, reinterpret_cast<const i8_bf16 *>(x), n, cin, pitch, ls, q, scale);
-    else hipLaunchKernelGGL((k_i8_rows<i8_f16, 256>), dim3((unsigned)nb), dim3(256), 0, s, reinterpret_cast<const i8_f16 *>(x), n, cin, pitch, ls, q, scale);
+    if (dtype == CG3D_DT_F32) i8_launch_rows(reinterpret_cast<const float *>(x), n, cin, pitch, q, scale, s);
+    else if (dtype == CG3D_DT_BF16) i8_launch_rows(reinterpret_cast<const i8_bf16 *>(x), n, cin, pitch, q, scale, s);
+    else i8_launch_rows(reinterpret_cast<const i8_f16 *>(x), n, cin, pitch, q, scale, s);
     CG3D_CHECK_LAUNCH();
     return CG3D_OK;
 }
@@ -386,231 +408,291 @@ static __device__ __forceinline__ bool i8_tile(const i8_args &a, int64_t u, int 
             lo = min(max((int64_t)a.offsets[g], (int64_t)0), a.n_rows);
             hi = g < a.n_experts ? min(max((int64_t)a.offsets[g + 1], lo), a.n_rows) : a.n_rows;
         }
-        const int tiles = (int)((hi - lo + BM - 1) / BM);
+        const int tiles = (int)(((uint32_t)(hi - lo) + (uint32_t)BM - 1) / (uint32_t)BM);
         int s = tiles;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(s, d); if (lane >= d) s += o; }
         const uint64_t hit = __ballot(u < before + s);
         if (hit) {
-            const int l = __ffsll((unsigned long long)hit) - 1;
-            const int64_t first = before + __shfl(s - tiles, l);
-            const int64_t base = (int64_t)__shfl((int)lo, l), end = (int64_t)__shfl((int)hi, l);
+            const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)hit) - 1);      // (uniform, and so is all that follows)
+            const int64_t first = before + __builtin_amdgcn_readlane(s - tiles, l);
+            const int64_t base = (int64_t)__builtin_amdgcn_readlane((int)lo, l), end = (int64_t)__builtin_amdgcn_readlane((int)hi, l);
             e = b + l;
             row0 = base + (u - first) * BM;
             rows = (int)min((int64_t)BM, end - row0);
             return true;
         }
-        before += __shfl(s, 63);
+        before += __builtin_amdgcn_readlane(s, 63);
     }
     return false;
-}
-static int64_t i8_tiles(const i8_args &a, int bm) { return a.offsets ? a.n_rows / bm + a.n_experts + 1 : cg3d_divup(a.n_rows, bm); }
-
-// a lane's 8 neighbouring results c0 .. c0 + 7 of one row; live = 0: a row behind the last
-static __device__ __forceinline__ void i8_store8(const i8_args &a, int e, int c0, int64_t row, float sx, bool live, const i32x4 &lo, const i32x4 &hi) {
-    typedef i8_vec<float, 8> f8;
-    typedef i8_vec<uint16_t, 8> h8;
-    const int n = min(8, a.cout - c0);
-    if (n <= 0) return;
-    f8 v;
-#pragma unroll
-    for (int j = 0; j < 8; j++) v.e[j] = 0.f;
-    if (live) {
-        const float *sw = a.sw + (int64_t)e * a.cout + c0, *bias = a.bias + (int64_t)e * a.bias_step + c0;
-        if (n == 8) {
-            const f8 s = *reinterpret_cast<const f8 *>(sw);
-#pragma unroll
-            for (int j = 0; j < 8; j++) v.e[j] = (float)(j < 4 ? lo[j & 3] : hi[j & 3]) * sx * s.e[j];
-            if (a.bias) {
-                const f8 b = *reinterpret_cast<const f8 *>(bias);
-#pragma unroll
-                for (int j = 0; j < 8; j++) v.e[j] += b.e[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j < n) {
-                    v.e[j] = (float)(j < 4 ? lo[j & 3] : hi[j & 3]) * sx * sw[j];
-                    if (a.bias) v.e[j] += bias[j];
-                }
-        }
-    }
-    if (a.out_dtype == CG3D_DT_F32) {
-        float *y = reinterpret_cast<float *>(a.y) + row * a.cout + c0;
-        if (n == 8) {
-            struct two { u32x4 q[2]; };
-            const two o = __builtin_bit_cast(two, v);
-            __builtin_nontemporal_store(o.q[0], reinterpret_cast<u32x4_any *>(y));
-            __builtin_nontemporal_store(o.q[1], reinterpret_cast<u32x4_any *>(y + 4));
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) if (j < n) y[j] = v.e[j];
-        }
-    } else {
-        uint16_t *y = reinterpret_cast<uint16_t *>(a.y) + row * a.cout + c0;
-        h8 o;
-        if (a.out_dtype == CG3D_DT_BF16) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) o.e[j] = __builtin_bit_cast(uint16_t, (__bf16)v.e[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) o.e[j] = __builtin_bit_cast(uint16_t, (_Float16)v.e[j]);
-        }
-        if (n == 8) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o), reinterpret_cast<u32x4_any *>(y));
-        else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) if (j < n) y[j] = o.e[j];
-        }
-    }
-}
-// a lane's results of one panel, acc[nb][i]: channels i8_channel(nb, 4 g + i)
-static __device__ __forceinline__ void i8_store(const i8_args &a, int e, int panel, int64_t row, float sx, bool live, const i32x4 (&acc)[4]) {
-    const int c0 = panel * 64 + ((threadIdx.x & 63) >> 4) * 8;
-    i8_store8(a, e, c0, row, sx, live, acc[0], acc[1]);
-    i8_store8(a, e, c0 + 32, row, sx, live, acc[2], acc[3]);
 }
 static __device__ __forceinline__ int64_t i8_source(const i8_args &a, int64_t row) {
     const int64_t src = a.rows ? (int64_t)a.rows[row] : row;
     return (uint64_t)src < (uint64_t)a.n_x ? src : 0;
 }
+// N neighbouring channels from c0 of one expert: their scales and biases (zeros behind the last channel)
+template <int N> struct i8_chan {
+    i8_vec<float, N> s, b;
+    __device__ __forceinline__ i8_chan(const i8_args &a, int e, int c0) : s{}, b{} {
+        const float *sw = a.sw + (int64_t)e * a.cout + c0, *bias = a.bias + (int64_t)e * a.bias_step + c0;
+        if (c0 + N <= a.cout) {
+            s = *reinterpret_cast<const i8_vec<float, N> *>(sw);
+            if (a.bias) b = *reinterpret_cast<const i8_vec<float, N> *>(bias);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N - 1; j++)
+                if (c0 + j < a.cout) {
+                    s.e[j] = sw[j];
+                    if (a.bias) b.e[j] = bias[j];
+                }
+        }
+    }
+};
+// a lane's N sums of one row, scaled, as many of them as there are channels left (n); live = 0: a row behind the last.  to: where the
+// workgroup's first lane would store (the same for all lanes), at: this lane's elements behind it
+template <int N>
+static __device__ __forceinline__ void i8_store(const i8_args &a, int64_t to, uint32_t at, int n, float sx, bool live, const i8_chan<N> &ch, const int (&sum)[N]) {
+    i8_vec<float, N> v;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        v.e[j] = (float)sum[j] * sx * ch.s.e[j];
+        if (a.bias) v.e[j] += ch.b.e[j];
+        if (!live) v.e[j] = 0.f;
+    }
+    // (streamed past the caches like the rows of expert_rows.hip)
+    if (a.out_dtype == CG3D_DT_F32) {
+        float *y = reinterpret_cast<float *>(a.y) + to + at;
+        if (n >= N) {
+            if constexpr (N == 4) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4_any *>(y));
+            else *reinterpret_cast<i8_vec<float, N> *>(y) = v;
+        } else {
+#pragma unroll
+            for (int j = 0; j < N - 1; j++) if (j < n) y[j] = v.e[j];
+        }
+    } else {
+        uint16_t *y = reinterpret_cast<uint16_t *>(a.y) + to + at;
+        i8_vec<uint16_t, N> o;
+        if (a.out_dtype == CG3D_DT_BF16) {
+#pragma unroll
+            for (int j = 0; j < N; j++) o.e[j] = __builtin_bit_cast(uint16_t, (__bf16)v.e[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) o.e[j] = __builtin_bit_cast(uint16_t, (_Float16)v.e[j]);
+        }
+        if (n >= N) {
+            if constexpr (N == 4) __builtin_nontemporal_store(__builtin_bit_cast(u32x2_any, o), reinterpret_cast<u32x2_any *>(y));
+            else *reinterpret_cast<i8_vec<uint16_t, N> *>(y) = o;
+        } else {
+#pragma unroll
+            for (int j = 0; j < N - 1; j++) if (j < n) y[j] = o.e[j];
+        }
+    }
+}
+// a wave's results of 16 rows x one panel: acc[nb][i] of lane (g, m) is row 4 g + i, channel 4 m + nb; sx: of the lane's four rows
+static __device__ __forceinline__ void i8_store_panel(const i8_args &a, int e, int panel, int64_t row0, int rows, const float (&sx)[4], bool live,
+                                                      const i32x4 (&acc)[4]) {
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, c0 = panel * 64 + m * 4, n = a.cout - c0;
+    if (n <= 0) return;
+    const i8_chan<4> ch(a, live ? e : 0, c0);
+    const uint32_t at = (uint32_t)(g * 4) * (uint32_t)a.cout + m * 4;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (g * 4 + i < rows) {
+            const int sum[4] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+            i8_store<4>(a, (row0 + i) * a.cout + panel * 64, at, n, sx[i], live, ch, sum);
+        }
+}
+// the scales of the lane's four rows of 16
+static __device__ __forceinline__ void i8_scales(const i8_args &a, int64_t row0, int rows, bool live, float (&sx)[4]) {
+    const int g = (threadIdx.x & 63) >> 4;
+    if (live && !a.rows && g * 4 + 4 <= rows) {
+        const i8_vec<float, 4> s = *reinterpret_cast<const i8_vec<float, 4> *>(a.sx + row0 + g * 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) sx[i] = s.e[i];
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) sx[i] = live && g * 4 + i < rows ? a.sx[i8_source(a, row0 + g * 4 + i)] : 0.f;
+}
+// where piece p (16 bytes) of row r lies in a fragment of 16 rows x 64 bytes of LDS: whole rows to write, and the 16 lanes that read
+// one piece of every row touch every bank once
+static __device__ __forceinline__ int i8_place(int r, int p) { return r * 64 + ((p ^ (r >> 2)) << 4); }
 
-// Rows of at most I8_FUSED_CIN columns: one pass over them.  A workgroup of 4 waves owns 64 rows; each wave brings 16 of them in, in the
-// layout of the MFMA's B operand -- lane (g, m) has elements 64 c + 16 g .. + 15 of row m for every chunk c -- so that a row's maximum
-// is a maximum over the lane and two exchanges, and the levels go to LDS as whole fragments (contiguous, no conflicts).  Then wave
-// (wm, wn) multiplies RG of the 4 row groups by panels wn, wn + RG, ... of the part blockIdx.y of the channels: the weights stream
-// past from the caches one chunk ahead, every fragment used RG times.  RG = 4 / 2 / 1 for at least 4 / 2 / 1 panels a part.
+// Rows of at most I8_FUSED_CIN columns: one pass over them.  A workgroup of 4 waves owns 64 rows; each wave brings 16 of them in,
+// neighbouring lanes neighbouring pieces (a chunk of a row is 4, 8 or 16 lanes, so a load of the wave is whole lines), finds their
+// maxima over those lanes, and leaves their levels in LDS in the order of the MFMA's operand.  A level's divisions are done once for a
+// row: of the NI rows that a lane has pieces of, lane l sees to row l % NI and its neighbours get the factor from it.  Then wave
+// (wm, wn) multiplies RG of the 4 row groups by panels wn, wn + RG, ... of the part blockIdx.y of the channels, the weights streaming
+// past from the caches, every fragment used RG times.  RG = 4 / 2 / 1 for at least 4 / 2 / 1 panels a part.
 template <typename T, int RG, int KEEP>                  // KEEP: chunks of a row held in registers; longer rows are read again, from the caches
 __global__ __launch_bounds__(256, RG == 4 || KEEP * sizeof(T) > 8 ? 4 : RG == 2 ? 5 : 6) void k_i8_fused(i8_args a, const T *__restrict__ x) {
     extern __shared__ __attribute__((aligned(16))) uint8_t i8_sm[];
+    constexpr int NI = sizeof(T), LPR = 4 * NI, RPI = 64 / LPR, N = i8_els<T>;     // lanes of a row's chunk, rows of a load, elements of a piece
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int panels = (a.cout + 63) >> 6, chunks = (a.cin + 63) >> 6;
     const int p_lo = (int)((int64_t)panels * blockIdx.y / gridDim.y), p_hi = (int)((int64_t)panels * (blockIdx.y + 1) / gridDim.y);
-    i32x4 *const frag = reinterpret_cast<i32x4 *>(i8_sm);                          // [4 groups][chunks][64 lanes]
-    float *const scales = reinterpret_cast<float *>(i8_sm + chunks * 4096);        // [64]
+    float *const scales = reinterpret_cast<float *>(i8_sm + chunks * 4096);        // [64], behind [4 groups][chunks][1 KB]
     int e, rows;
     int64_t row0;
     if (!i8_tile<64>(a, blockIdx.x, e, row0, rows)) return;                        // (the whole workgroup)
     const bool live = e < a.n_experts;
     if (live && wave * 16 < rows) {
-        const int64_t src = i8_source(a, row0 + min(wave * 16 + m, rows - 1));
-        const T *xr = x + src * a.cin;
-        i32x4 *const mine = frag + wave * chunks * 64 + lane;
-        if constexpr (sizeof(T) == 1) {
-            if (g == 0) scales[wave * 16 + m] = a.sx[src];
+        const int rl = lane / LPR, k0 = (lane % LPR) * N;
+        const T *xr[NI];
+        uint8_t *to[NI];
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int r = i * RPI + rl;
+            const int64_t src = i8_source(a, row0 + min(wave * 16 + r, rows - 1));
+            xr[i] = x + src * a.cin;
+            to[i] = i8_sm + wave * chunks * 1024 + i8_place(r, k0 >> 4) + (k0 & 15);
+            if constexpr (NI == 1) {
+                if (lane % LPR == 0) scales[wave * 16 + r] = a.sx[src];
+            }
+        }
+        if constexpr (NI == 1) {
 #pragma unroll 8
-            for (int c = 0; c < chunks; c++) mine[c * 64] = __builtin_bit_cast(i32x4, i8_get16<T>(xr, c * 64 + g * 16, a.cin).w[0]);
+            for (int c = 0; c < chunks; c++) *reinterpret_cast<u32x4 *>(to[0] + c * 1024) = i8_piece<T>(xr[0], c * 64 + k0, a.cin);
         } else {
-            i8_raw<T> v[KEEP];
-            i8_max<T> most;
+            u32x4 v[KEEP][NI];
+            i8_max<T> most[NI];
             for (int c0 = 0; c0 < chunks; c0 += KEEP) {
 #pragma unroll
                 for (int c = 0; c < KEEP; c++)
-                    if (c0 + c < chunks) v[c] = i8_get16<T>(xr, (c0 + c) * 64 + g * 16, a.cin);
+                    if (c0 + c < chunks)
+#pragma unroll
+                        for (int i = 0; i < NI; i++) v[c][i] = i8_piece<T>(xr[i], (c0 + c) * 64 + k0, a.cin);
 #pragma unroll
                 for (int c = 0; c < KEEP; c++)
-                    if (c0 + c < chunks) most.add(v[c]);
+                    if (c0 + c < chunks)
+#pragma unroll
+                        for (int i = 0; i < NI; i++) most[i].add(v[c][i]);
             }
-            uint32_t top = most.bits();
-            top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-            top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-            const i8_level lev(top);
-            const bool far = __any(lev.shifted());
-            if (g == 0) scales[wave * 16 + m] = lev.scale;
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const uint32_t t = i8_max_of<LPR>(most[i].bits());
+                top = lane % NI == i ? t : top;
+            }
+            const i8_level mine(top);
+            const bool far = __any(mine.shifted());
+            if (lane % LPR < NI) scales[wave * 16 + (lane % NI) * RPI + rl] = mine.scale;
+            i8_level lev[NI];
+#pragma unroll
+            for (int i = 0; i < NI; i++) {                                         // (lane i of each NI neighbours)
+                lev[i] = mine;
+                constexpr int ALL[4] = {NI == 2 ? 0xa0 : 0x00, NI == 2 ? 0xf5 : 0x55, 0xaa, 0xff};
+                auto from = [&](uint32_t w) {
+                    return i == 0 ? i8_dpp<ALL[0]>(w) : i == 1 ? i8_dpp<ALL[1]>(w) : i == 2 ? i8_dpp<ALL[2]>(w) : i8_dpp<ALL[3]>(w);
+                };
+                lev[i].c = __uint_as_float(from(__float_as_uint(mine.c)));
+                lev[i].amax = __uint_as_float(from(__float_as_uint(mine.amax)));
+                lev[i].shift = __uint_as_float(from(__float_as_uint(mine.shift)));
+                lev[i].keep = from(mine.keep);
+                lev[i].fine127 = from(mine.fine127) != 0;
+            }
             for (int c0 = 0; c0 < chunks; c0 += KEEP) {
                 if (chunks > KEEP) {
 #pragma unroll
                     for (int c = 0; c < KEEP; c++)
-                        if (c0 + c < chunks) v[c] = i8_get16<T>(xr, (c0 + c) * 64 + g * 16, a.cin);
+                        if (c0 + c < chunks)
+#pragma unroll
+                            for (int i = 0; i < NI; i++) v[c][i] = i8_piece<T>(xr[i], (c0 + c) * 64 + k0, a.cin);
                 }
 #pragma unroll
                 for (int c = 0; c < KEEP; c++)
-                    if (c0 + c < chunks) mine[(c0 + c) * 64] = i8_levels16<T>(lev, far, v[c]);
+                    if (c0 + c < chunks)
+#pragma unroll
+                        for (int i = 0; i < NI; i++)
+                            *reinterpret_cast<i8_lev<T> *>(to[i] + (c0 + c) * 1024) = i8_levels<T>(lev[i], far, v[c][i]);
             }
         }
     }
     const int wn = wave % RG, wm = wave / RG;
-    const i32x4 *const w_e = reinterpret_cast<const i32x4 *>(a.w) + (int64_t)(live ? e : 0) * panels * (chunks * 256) + lane;
-    i32x4 cur[4];                                                                  // (the first weights travel over the barrier)
-    if (p_lo + wn < p_hi)
+    // the weights' fragments of the next chunk are asked for as soon as those of this one are used (two or four chunks ahead: no gain)
+    const int8_t *const w_e = a.w + (int64_t)(live ? e : 0) * panels * (chunks * 4096);             // (uniform: an address for all lanes)
+    i32x4 wq[4];
+    if (p_lo + wn < p_hi)                                                          // (the first ones travel over the barrier)
 #pragma unroll
-        for (int nb = 0; nb < 4; nb++) cur[nb] = w_e[(int64_t)(p_lo + wn) * (chunks * 256) + nb * 64];
+        for (int nb = 0; nb < 4; nb++) wq[nb] = reinterpret_cast<const i32x4 *>(w_e + (int64_t)(p_lo + wn) * chunks * 4096 + nb * 1024)[lane];
     __syncthreads();
     if (wm * RG * 16 >= rows) return;
-    const i32x4 *const bq = frag + wm * RG * chunks * 64 + lane;
+    const uint8_t *const bq = i8_sm + wm * RG * chunks * 1024 + i8_place(m, g);
     for (int p = p_lo + wn; p < p_hi; p += RG) {
         i32x4 acc[RG][4];
 #pragma unroll
         for (int h = 0; h < RG; h++)
 #pragma unroll
             for (int nb = 0; nb < 4; nb++) acc[h][nb] = i32x4{0, 0, 0, 0};
-        const i32x4 *wf = w_e + (int64_t)p * (chunks * 256);
-        const i32x4 *const then = w_e + (int64_t)(p + RG < p_hi ? p + RG : p) * (chunks * 256);
+        const int here = p * chunks, then = (p + RG < p_hi ? p + RG : p) * chunks;
         for (int c = 0; c < chunks; c++) {
-            i32x4 nxt[4];
-            wf = c + 1 < chunks ? wf + 256 : then;                                 // (the next panel's first behind the last)
-#pragma unroll
-            for (int nb = 0; nb < 4; nb++) nxt[nb] = wf[nb * 64];
             if (live) {
 #pragma unroll
                 for (int h = 0; h < RG; h++) {
-                    const i32x4 q = bq[(h * chunks + c) * 64];                     // (a group without rows: old bytes, never stored)
+                    const i32x4 q = *reinterpret_cast<const i32x4 *>(bq + (h * chunks + c) * 1024);     // (a group without rows: old bytes, never stored)
 #pragma unroll
-                    for (int nb = 0; nb < 4; nb++) acc[h][nb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur[nb], q, acc[h][nb], 0, 0, 0);
+                    for (int nb = 0; nb < 4; nb++) acc[h][nb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(q, wq[nb], acc[h][nb], 0, 0, 0);
                 }
             }
+            const int8_t *const wf = w_e + (int64_t)(c + 1 < chunks ? here + c + 1 : then) * 4096;
 #pragma unroll
-            for (int nb = 0; nb < 4; nb++) cur[nb] = nxt[nb];
+            for (int nb = 0; nb < 4; nb++) wq[nb] = reinterpret_cast<const i32x4 *>(wf + nb * 1024)[lane];
         }
 #pragma unroll
         for (int h = 0; h < RG; h++) {
-            const int r = (wm * RG + h) * 16 + m;
-            if (r < rows) i8_store(a, e, p, row0 + r, scales[r], live, acc[h]);
+            const int r = (wm * RG + h) * 16;
+            const i8_vec<float, 4> sx = *reinterpret_cast<const i8_vec<float, 4> *>(scales + r + g * 4);
+            i8_store_panel(a, e, p, row0 + r, rows - r, sx.e, live, acc[h]);
         }
     }
 }
 
-// Few rows: a workgroup of 8 waves owns 16 rows x 32 channels and its waves share the contraction (chunk c belongs to wave c % 8), so
-// that every weight is read once, by loads that are all under way before the rows are even looked at.  Rows in floats that fit
-// (I8_FEW chunks of a wave) are quantised here -- each workgroup finds the rows' maxima for itself, through LDS; the waves' sums are
-// joined there too.  grid: (16-row tiles, 32-channel halves of panels).
+// Few rows: a workgroup of 8 waves owns 16 rows x 32 channels (tiles nb of a pair) and its waves share the contraction (chunk c belongs
+// to wave c % 8), so that every weight is read once, by loads that are all under way before the rows are even looked at.  Rows in
+// floats that fit (CHUNKS chunks of a wave) are quantised here, in the operand's own layout -- each workgroup finds the rows' maxima for
+// itself, through LDS; the waves' sums are joined there too.  grid: (16-row tiles, pairs of tiles).
 template <typename T> struct i8_few { static constexpr int CHUNKS = sizeof(T) == 4 ? 4 : 8; };
 template <typename T>
 __global__ __launch_bounds__(512, 2) void k_i8_few(i8_args a, const T *__restrict__ x, int64_t pitch) {
     __shared__ i32x4 part[8][2][64];
     __shared__ uint32_t tops[8][16];
-    constexpr int KEEP = i8_few<T>::CHUNKS;
+    __shared__ float scales[16];
+    constexpr int KEEP = i8_few<T>::CHUNKS, NI = sizeof(T), N = i8_els<T>;
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int panels = (a.cout + 63) >> 6, chunks = (a.cin + 63) >> 6, panel = blockIdx.y >> 1, half = blockIdx.y & 1;
+    const int panels = (a.cout + 63) >> 6, chunks = (a.cin + 63) >> 6, panel = blockIdx.y >> 1, pair = blockIdx.y & 1;
     int e, rows;
     int64_t row0;
     if (!i8_tile<16>(a, blockIdx.x, e, row0, rows)) return;      // (the whole workgroup)
     const bool live = e < a.n_experts;
     const int64_t src = live ? i8_source(a, row0 + min(m, rows - 1)) : 0;
     const T *xr = x + src * pitch;
-    const i32x4 *wf = reinterpret_cast<const i32x4 *>(a.w) + (((int64_t)(live ? e : 0) * panels + panel) * chunks * 4 + half * 2) * 64 + lane;
+    const i32x4 *wf = reinterpret_cast<const i32x4 *>(a.w) + (((int64_t)(live ? e : 0) * panels + panel) * chunks * 4 + pair * 2) * 64 + lane;
     i32x4 acc[2] = {i32x4{0, 0, 0, 0}, i32x4{0, 0, 0, 0}};
     float sx = 0.f;
     if (live) {
-        if constexpr (sizeof(T) == 1) sx = a.sx[src];
+        if constexpr (NI == 1) sx = a.sx[src];
         for (int c0 = 0; c0 < chunks; c0 += 8 * KEEP) {          // (rows in floats: once)
             i32x4 w[KEEP][2];
-            i8_raw<T> v[KEEP];
+            u32x4 v[KEEP][NI];
 #pragma unroll
             for (int i = 0; i < KEEP; i++) {
                 const int c = c0 + i * 8 + wave;
                 if (c < chunks) {
-                    v[i] = i8_get16<T>(xr, c * 64 + g * 16, a.cin);
+#pragma unroll
+                    for (int j = 0; j < NI; j++) v[i][j] = i8_piece<T>(xr, c * 64 + g * 16 + j * N, a.cin);
                     w[i][0] = wf[(int64_t)c * 256];
                     w[i][1] = wf[(int64_t)c * 256 + 64];
                 }
             }
             i8_level lev(0);
             bool far = false;
-            if constexpr (sizeof(T) != 1) {
+            if constexpr (NI != 1) {
                 i8_max<T> most;
 #pragma unroll
                 for (int i = 0; i < KEEP; i++)
-                    if (i * 8 + wave < chunks) most.add(v[i]);
+                    if (i * 8 + wave < chunks)
+#pragma unroll
+                        for (int j = 0; j < NI; j++) most.add(v[i][j]);
                 uint32_t top = most.bits();
                 top = max(top, (uint32_t)__shfl_xor((int)top, 16));
                 top = max(top, (uint32_t)__shfl_xor((int)top, 32));
@@ -625,16 +707,17 @@ __global__ __launch_bounds__(512, 2) void k_i8_few(i8_args a, const T *__restric
 #pragma unroll
             for (int i = 0; i < KEEP; i++)
                 if (c0 + i * 8 + wave < chunks) {
-                    i32x4 q;
-                    if constexpr (sizeof(T) == 1) q = __builtin_bit_cast(i32x4, v[i].w[0]);
-                    else q = i8_levels16<T>(lev, far, v[i]);
-                    acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i][0], q, acc[0], 0, 0, 0);
-                    acc[1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i][1], q, acc[1], 0, 0, 0);
+                    struct { i8_lev<T> p[NI]; } q;
+#pragma unroll
+                    for (int j = 0; j < NI; j++) q.p[j] = i8_levels<T>(lev, far, v[i][j]);
+                    acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, q), w[i][0], acc[0], 0, 0, 0);
+                    acc[1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, q), w[i][1], acc[1], 0, 0, 0);
                 }
         }
     }
     part[wave][0][lane] = acc[0];
     part[wave][1][lane] = acc[1];
+    if (wave == 0 && g == 0) scales[m] = sx;
     __syncthreads();
     if (wave != 0) return;
 #pragma unroll
@@ -642,7 +725,15 @@ __global__ __launch_bounds__(512, 2) void k_i8_few(i8_args a, const T *__restric
         acc[0] += part[i][0][lane];
         acc[1] += part[i][1][lane];
     }
-    if (m < rows) i8_store8(a, e, panel * 64 + half * 32 + g * 8, row0 + m, sx, live, acc[0], acc[1]);
+    const int c0 = panel * 64 + m * 4 + pair * 2, n = a.cout - c0;
+    if (n <= 0) return;
+    const i8_chan<2> ch(a, live ? e : 0, c0);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (g * 4 + i < rows) {
+            const int sum[2] = {acc[0][i], acc[1][i]};
+            i8_store<2>(a, (row0 + i) * a.cout, (uint32_t)(g * 4) * (uint32_t)a.cout + c0, n, scales[g * 4 + i], live, ch, sum);
+        }
 }
 
 // Many rows and a long contraction, rows in 8 bits (pitch and address multiples of 16): tiles of WR * RG * 16 rows x WC * 64 channels
@@ -706,7 +797,7 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void k_i8_tile(i8_args a, const in
             for (int i = 0; i < NL; i++)
                 i8_dma(of_a ? src[i] + (int64_t)c * 4096 : src[i] + min((c_lo + c) * 64 + piece * 16, last), to + i * 1024);
         };
-        const uint8_t *const la = i8_sm + wc * 4096 + lane * 16, *const lb = i8_sm + NA * 1024 + wr * RG * 1024 + m * 64 + ((g ^ (m >> 2)) << 4);
+        const uint8_t *const la = i8_sm + wc * 4096 + lane * 16, *const lb = i8_sm + NA * 1024 + wr * RG * 1024 + i8_place(m, g);
         i32x4 fa[2][4], fb[2][RG];
         auto fetch = [&](int k, i32x4 (&A)[4], i32x4 (&B)[RG]) {
             const int at = (k % NBUF) * STAGE;
@@ -719,7 +810,7 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void k_i8_tile(i8_args a, const in
 #pragma unroll
             for (int h = 0; h < RG; h++)
 #pragma unroll
-                for (int nb = 0; nb < 4; nb++) acc[h][nb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[nb], B[h], acc[h][nb], 0, 0, 0);
+                for (int nb = 0; nb < 4; nb++) acc[h][nb] = __builtin_amdgcn_mfma_i32_16x16x64_i8(B[h], A[nb], acc[h][nb], 0, 0, 0);
         };
         auto step = [&](int k, i32x4 (&A)[4], i32x4 (&B)[RG], i32x4 (&nA)[4], i32x4 (&nB)[RG]) {
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(NL) : "memory");      // chunk k + 1 is in LDS, for every wave
@@ -750,8 +841,11 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void k_i8_tile(i8_args a, const in
     if (panel >= panels) return;
 #pragma unroll
     for (int h = 0; h < RG; h++) {
-        const int r = (wr * RG + h) * 16 + m;
-        if (r < rows) i8_store(a, e, panel, row0 + r, live ? a.sx[i8_source(a, row0 + r)] : 0.f, live, acc[h]);
+        const int r = (wr * RG + h) * 16;
+        if (r >= rows) break;
+        float sx[4];
+        i8_scales(a, row0 + r, rows - r, live, sx);
+        i8_store_panel(a, e, panel, row0 + r, rows - r, sx, live, acc[h]);
     }
 }
 // The sums of a tile's ranges of chunks: a workgroup owns 16 rows x 64 channels, its 8 waves share the ranges (one wave for all of
@@ -760,14 +854,14 @@ template <int RG, int WR, int WC>
 __global__ __launch_bounds__(512) void k_i8_join(i8_args a, int32_t ny, int32_t total, int32_t splits, const i32x4 *__restrict__ part) {
     constexpr int NW = WR * WC, BM = WR * RG * 16;
     __shared__ i32x4 sum[8][4][64];
-    const int lane = threadIdx.x & 63, m = lane & 15, me = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, me = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.x % RG, wave = blockIdx.x / RG % NW, id = blockIdx.x / (RG * NW);
     int e, rows;
     int64_t row0;
     if (!i8_tile<BM>(a, id / ny, e, row0, rows)) return;             // (the whole workgroup)
     const bool live = e < a.n_experts;
-    const int wr = wave % WR, wc = wave / WR, panel = id % ny * WC + wc, r = (wr * RG + h) * 16 + m;
-    if (panel >= (a.cout + 63) >> 6 || (wr * RG + h) * 16 >= rows) return;
+    const int wr = wave % WR, wc = wave / WR, panel = id % ny * WC + wc, r = (wr * RG + h) * 16;
+    if (panel >= (a.cout + 63) >> 6 || r >= rows) return;
     i32x4 acc[4];
 #pragma unroll
     for (int nb = 0; nb < 4; nb++) acc[nb] = i32x4{0, 0, 0, 0};
@@ -785,7 +879,9 @@ __global__ __launch_bounds__(512) void k_i8_join(i8_args a, int32_t ny, int32_t 
     for (int w = 1; w < 8; w++)
 #pragma unroll
         for (int nb = 0; nb < 4; nb++) acc[nb] += sum[w][nb][lane];
-    if (r < rows) i8_store(a, e, panel, row0 + r, live ? a.sx[i8_source(a, row0 + r)] : 0.f, live, acc);
+    float sx[4];
+    i8_scales(a, row0 + r, rows - r, live, sx);
+    i8_store_panel(a, e, panel, row0 + r, rows - r, sx, live, acc);
 }
 
 // rows of 8 bits whose pitch or address 16 does not divide: a copy with pitch i8_pitch
@@ -794,7 +890,7 @@ __global__ __launch_bounds__(256) void k_i8_pad(const int8_t *__restrict__ x, in
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n * nv; i += gridDim.x * 256ll) {
         const int64_t r = i / nv;
         const int k0 = (int)(i - r * nv) * 16;
-        *reinterpret_cast<u32x4 *>(out + r * pitch + k0) = i8_get16<int8_t>(x + r * cin, k0, cin).w[0];
+        *reinterpret_cast<u32x4 *>(out + r * pitch + k0) = i8_piece<int8_t>(x + r * cin, k0, cin);
     }
 }
 
@@ -811,8 +907,10 @@ static i8_plan i8_choose(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows
     i8_plan p = {};
     const int64_t chunks = i8_chunks(cin), panels = i8_panels(cout);
     auto tiles = [&](int bm) { return grouped ? n_rows / bm + n_experts + 1 : cg3d_divup(n_rows, bm); };
-    const int64_t each = grouped ? n_rows / n_experts : n_rows;      // rows of a matrix, about
-    if (each <= 32) {
+    // workgroups of the kernel for few rows (empty experts' leave at once): up to two for a CU it is the fastest, one where rows are short;
+    // of long rows each of them would read too much by itself
+    const int64_t few = (n_rows / 16 + (grouped ? (n_experts < n_rows ? n_experts : n_rows) : 1)) * panels * 2;
+    if (few <= (chunks <= 2 ? 256 : 512) && chunks <= 128) {
         p.kind = i8_plan::FEW;
         p.tiles = tiles(16);
         p.rows8 = dtype != CG3D_DT_I8 && chunks > 8 * (dtype == CG3D_DT_F32 ? i8_few<float>::CHUNKS : i8_few<i8_bf16>::CHUNKS);
@@ -899,7 +997,7 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
     }
     if (p.kind == i8_plan::FUSED) {
         // enough workgroups for the chip: the panels of a row tile are shared out where there are fewer than 1024 tiles
-        const int32_t parts = (int32_t)(cg3d_divup(1024, p.tiles) < panels ? cg3d_divup(1024, p.tiles) : panels);
+        const int32_t parts = (int32_t)(cg3d_divup(I8_WANT, p.tiles) < panels ? cg3d_divup(I8_WANT, p.tiles) : panels);
         const int32_t each = (int32_t)cg3d_divup(panels, parts);
         const int lds = (int)i8_chunks(cin) * 4096 + 256;           // (at most 32.25 KB)
 #define I8_F(T, RG, KEEP) hipLaunchKernelGGL((k_i8_fused<T, RG, KEEP>), dim3((unsigned)p.tiles, (unsigned)parts), dim3(256), lds, s, a, reinterpret_cast<const T *>(x))

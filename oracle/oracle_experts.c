@@ -149,13 +149,10 @@ static int bad_shape(int32_t e, int32_t cin, int32_t cout) {
     return e < 1 || e > 1024 || cin < 1 || cin > 131071 || cout < 1 || cout > (1 << 20);
 }
 static int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
-static int channel(int nb, int m) { return (nb >> 1) * 32 + (m >> 2) * 8 + (nb & 1) * 4 + (m & 3); }
 /* where weight (e, k, n) lies in the packed form */
 static int64_t place(int32_t e, int32_t k, int32_t n, int32_t cin, int32_t cout) {
     const int64_t panels = up(cout, 64), chunks = up(cin, 64);
-    int nb = 0, m = 0;
-    for (int i = 0; i < 64; i++)
-        if (channel(i >> 4, i & 15) == n % 64) { nb = i >> 4; m = i & 15; }
+    const int nb = n % 4, m = n % 64 / 4;
     const int lane = (k % 64) / 16 * 16 + m;
     return ((((int64_t)e * panels + n / 64) * chunks + k / 64) * 4 + nb) * 1024 + lane * 16 + k % 16;
 }
@@ -191,7 +188,7 @@ int cg3d_int8_weight(const void *w, int32_t dtype, int32_t E, int32_t cin, int32
 int cg3d_int8_quantize_rows(const void *x, int32_t dtype, int64_t n, int32_t cin, int64_t pitch, int8_t *q, float *scale,
                             cg3d_stream_t stream) {
     (void)stream;
-    if (!fl(dtype) || n < 0 || cin < 1 || cin > 131071 || pitch < cin) return CG3D_ERR_ARG;
+    if (!fl(dtype) || n < 0 || cin < 1 || cin > 131071 || pitch < cin || pitch > (1 << 30)) return CG3D_ERR_ARG;
     if (n == 0) return CG3D_OK;
     if (!x || !q || !scale || odd(x, dtype) || odd(scale, 0)) return CG3D_ERR_ARG;
     for (int64_t r = 0; r < n; r++) {
