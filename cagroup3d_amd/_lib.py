@@ -101,7 +101,7 @@ _SIGNATURES = {
     "cg3d_expert_plan_ws_bytes": (c_int64, [c_int64, c_int32, c_int32]),
     "cg3d_expert_plan": (c_int32, [P, c_int32, c_int64, c_int32, c_int32, P, P, P, P, P, P]),
     "cg3d_expert_gather": (c_int32, [P, c_int32, P, c_int64, c_int32, c_int32, P, P]),
-    "cg3d_expert_combine": (c_int32, [P, c_int32, P, P, c_int32, c_int64, c_int32, c_int32, P, P]),
+    "cg3d_expert_combine": (c_int32, [P, c_int32, P, P, c_int32, c_int64, c_int32, c_int32, P, c_int32, P]),
     "cg3d_expert_combine_bwd": (c_int32, [P, P, c_int32, P, P, c_int32, c_int64, c_int32, c_int32, P, P, P]),
     "cg3d_int8_weight_bytes": (c_int64, [c_int32, c_int32, c_int32]),
     "cg3d_int8_weight": (c_int32, [P, c_int32, c_int32, c_int32, c_int32, P, P, P, P]),

@@ -39,10 +39,12 @@ struct ex_f32 {
 // instructions on gfx950)
 template <typename T, int V> struct __attribute__((packed, aligned(2))) ex_vec { T e[V]; };
 typedef uint32_t ex_u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t ex_u32x2 __attribute__((ext_vector_type(2), aligned(2)));
 // results are streamed past the caches (non-temporal): they are larger than a die's 4 MB of L2 where it matters (combination of
 // 155 773 x 2 rows of 256 bytes 27.2 -> 24.5 us, of 20 011 x 8 rows of 502 bytes 28.1 -> 22.4 us; nothing at 2.5 MB)
 template <typename vec> static __device__ __forceinline__ void ex_put(vec *p, const vec &v) {
     if constexpr (sizeof(vec) == 16) { __builtin_nontemporal_store(__builtin_bit_cast(ex_u32x4, v), reinterpret_cast<ex_u32x4 *>(p)); return; }
+    if constexpr (sizeof(vec) == 8) { __builtin_nontemporal_store(__builtin_bit_cast(ex_u32x2, v), reinterpret_cast<ex_u32x2 *>(p)); return; }
     *p = v;
 }
 
@@ -291,10 +293,10 @@ __global__ __launch_bounds__(256) void k_expert_gather(const T *__restrict__ x, 
     }
 }
 
-template <typename T, int V>
+template <typename T, int V, typename O>
 __global__ __launch_bounds__(256) void k_expert_combine(const T *__restrict__ y, const int32_t *__restrict__ pos, const void *__restrict__ w,
                                                         int32_t wtype, int64_t n_tokens, int32_t k, int32_t c, int32_t nv, uint64_t magic,
-                                                        T *__restrict__ out) {
+                                                        O *__restrict__ out) {
     typedef ex_vec<T, V> vec;
     const int64_t P = n_tokens * k;
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n_tokens * nv; i += gridDim.x * 256ll) {
@@ -323,10 +325,10 @@ __global__ __launch_bounds__(256) void k_expert_combine(const T *__restrict__ y,
                     for (int j = 0; j < V; j++) acc[j] += ws[s] * T::to(v[s].e[j]);
                 }
         }
-        vec o;
+        ex_vec<O, V> o;
 #pragma unroll
-        for (int j = 0; j < V; j++) o.e[j] = T::from(acc[j]);
-        ex_put(reinterpret_cast<vec *>(out + t * c + a), o);
+        for (int j = 0; j < V; j++) o.e[j] = O::from(acc[j]);
+        ex_put(reinterpret_cast<ex_vec<O, V> *>(out + t * c + a), o);
     }
 }
 
@@ -407,20 +409,25 @@ extern "C" int cg3d_expert_gather(const void *x, int32_t dtype, const int32_t *r
 }
 
 extern "C" int cg3d_expert_combine(const void *y, int32_t dtype, const int32_t *pos, const void *w, int32_t wtype, int64_t n_tokens,
-                                   int32_t k, int32_t c, void *out, cg3d_stream_t stream) {
-    if (ex_bad(dtype, wtype, n_tokens, k, c)) return CG3D_ERR_ARG;
+                                   int32_t k, int32_t c, void *out, int32_t out_dtype, cg3d_stream_t stream) {
+    if (ex_bad(dtype, wtype, n_tokens, k, c) || out_dtype < CG3D_DT_F32 || out_dtype > CG3D_DT_F16 || (dtype != CG3D_DT_F32 && out_dtype != dtype))
+        return CG3D_ERR_ARG;
     if (n_tokens == 0) return CG3D_OK;
-    if (!y || !pos || !out || ex_odd(y, dtype) || ex_odd(out, dtype) || ex_odd(w, wtype)) return CG3D_ERR_ARG;
+    if (!y || !pos || !out || ex_odd(y, dtype) || ex_odd(out, out_dtype) || ex_odd(w, wtype)) return CG3D_ERR_ARG;
     hipStream_t s = cg3d_hs(stream);
-#define EX_LAUNCH(T, V)                                                                                            \
+#define EX_LAUNCH_O(T, V, O)                                                                                       \
     do {                                                                                                           \
         const int32_t nv = (int32_t)cg3d_divup(c, V);                                                              \
         const int64_t nb = ex_grid(cg3d_divup(n_tokens * nv, 256));                                                \
-        hipLaunchKernelGGL((k_expert_combine<T, V>), dim3((unsigned)nb), dim3(256), 0, s, reinterpret_cast<const T *>(y), pos, w, wtype, \
-                           n_tokens, k, c, nv, ex_magic(nv), reinterpret_cast<T *>(out));                                        \
+        hipLaunchKernelGGL((k_expert_combine<T, V, O>), dim3((unsigned)nb), dim3(256), 0, s, reinterpret_cast<const T *>(y), pos, w, \
+                           wtype, n_tokens, k, c, nv, ex_magic(nv), reinterpret_cast<O *>(out));                   \
     } while (0)
-    EX_DISPATCH(EX_LAUNCH);
+#define EX_LAUNCH(T, V) EX_LAUNCH_O(T, V, T)
+    if (out_dtype == dtype) EX_DISPATCH(EX_LAUNCH);
+    else if (out_dtype == CG3D_DT_BF16) { if (c >= 4) EX_LAUNCH_O(ex_f32, 4, ex_bf16); else EX_LAUNCH_O(ex_f32, 1, ex_bf16); }
+    else { if (c >= 4) EX_LAUNCH_O(ex_f32, 4, ex_f16); else EX_LAUNCH_O(ex_f32, 1, ex_f16); }
 #undef EX_LAUNCH
+#undef EX_LAUNCH_O
     CG3D_CHECK_LAUNCH();
     return CG3D_OK;
 }

@@ -113,13 +113,13 @@ def _gather(x, plan):
     return out
 
 
-def _combine(y, plan, w):
+def _combine(y, plan, w, out_dtype):
     lib = _lib.get()
     lib.check(y, w)
     with on_device(y):
-        out = torch.empty((plan.n_tokens, y.shape[1]), dtype=y.dtype, device=y.device)
+        out = torch.empty((plan.n_tokens, y.shape[1]), dtype=out_dtype, device=y.device)
         lib.call("cg3d_expert_combine", y.data_ptr(), DTYPES[y.dtype], plan.address(POS), ptr(w), 0 if w is None else DTYPES[w.dtype],
-                 plan.n_tokens, plan.k, y.shape[1], out.data_ptr(), lib.stream())
+                 plan.n_tokens, plan.k, y.shape[1], out.data_ptr(), DTYPES[out_dtype], lib.stream())
     return out
 
 
@@ -133,33 +133,33 @@ class _Gather(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        return None if dout is None else _combine(dout.contiguous(), ctx.plan, None), None
+        return None if dout is None else _combine(dout.contiguous(), ctx.plan, None, dout.dtype), None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, plan, w):
+    def forward(ctx, y, plan, w, out_dtype):
         y, w = y.contiguous(), None if w is None else w.contiguous()
-        ctx.plan = plan
+        ctx.plan, ctx.dtype = plan, y.dtype
         ctx.save_for_backward(y if ctx.needs_input_grad[2] else None, w)
         ctx.set_materialize_grads(False)
-        return _combine(y, plan, w)
+        return _combine(y, plan, w, out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         if dout is None:
-            return None, None, None
+            return None, None, None, None
         y, w = ctx.saved_tensors
         plan, c = ctx.plan, dout.shape[1]
         lib = _lib.get()
-        dout = dout.contiguous()
+        dout = dout.to(ctx.dtype).contiguous()                  # (wider than the output where the rows are)
         with on_device(dout):
             dy = torch.empty((plan.n_rows, c), dtype=dout.dtype, device=dout.device) if ctx.needs_input_grad[0] else None
             dw = torch.empty_like(w) if ctx.needs_input_grad[2] else None
             lib.call("cg3d_expert_combine_bwd", dout.data_ptr(), ptr(y), DTYPES[dout.dtype], plan.address(PAIRS), ptr(w),
                      0 if w is None else DTYPES[w.dtype], plan.n_tokens, plan.k, c, ptr(dy), ptr(dw), lib.stream())
-        return dy, None, dw
+        return dy, None, dw, None
 
 
 def expert_gather(x, plan):
@@ -170,11 +170,14 @@ def expert_gather(x, plan):
     return _Gather.apply(x, plan)
 
 
-def expert_combine(rows, plan, weights=None):
+def expert_combine(rows, plan, weights=None, out_dtype=None):
     """rows [T * k, C] in the plan's order -> [T, C]: out[t] = sum_s weights[t, s] * rows[pos[t, s]] over the slots that have a
-    row, summed in float32 in slot order (differentiable in rows and weights).  weights [T, k] float32 / bfloat16 / float16;
-    None: all ones."""
+    row, summed in float32 in slot order and rounded once, to out_dtype (default: the rows' own; float32 rows: any of the three)
+    -- differentiable in rows and weights.  weights [T, k] float32 / bfloat16 / float16; None: all ones."""
     _check_rows("expert_combine", rows, getattr(plan, "n_rows", 0), plan, "rows")
+    out_dtype = out_dtype or rows.dtype
+    need(out_dtype == rows.dtype or (rows.dtype == torch.float32 and out_dtype in FLOATS), "expert_combine: out_dtype must be the rows' own, "
+         "or float32, bfloat16 or float16 for float32 rows")
     if weights is not None:
         need(isinstance(weights, torch.Tensor) and weights.dtype in FLOATS, "expert_combine: weights must be float32, bfloat16 or float16")
         if weights.dim() == 1 and plan.k == 1:
@@ -183,5 +186,5 @@ def expert_combine(rows, plan, weights=None):
             raise CG3DError("expert_combine: weights must be [%d, %d] on %s, got %s on %s" % (plan.n_tokens, plan.k, rows.device,
                                                                                               tuple(weights.shape), weights.device))
     if not (torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))):
-        return _combine(rows.contiguous(), plan, None if weights is None else weights.contiguous())
-    return _Combine.apply(rows, plan, weights)
+        return _combine(rows.contiguous(), plan, None if weights is None else weights.contiguous(), out_dtype)
+    return _Combine.apply(rows, plan, weights, out_dtype)

@@ -592,7 +592,8 @@ int cg3d_adamw_step(const int64_t *table, const int32_t *pid, int64_t nrows, con
  * Element types `dtype` of rows, `wtype` of weights: CG3D_DT_F32 / _BF16 / _F16.  Rows are contiguous [*, c] of any width.
  *   gather:       out[j] = x[rows[j]]           (out [P, c]; rows without a pair are zeros)
  *   combine:      out[t] = sum_s w[t, s] * y[pos[t, s]]   (w NULL: all ones -- also the gather's gradient); fp32 sums in slot
- *                 order, rounded once; a token without rows gives zeros
+ *                 order, rounded once, to out_dtype (dtype, or any of the three from fp32 rows); a token without rows gives
+ *                 zeros
  *   combine_bwd:  for row j of pair (t, s): dy[j] = w[t, s] * dout[t] (rows without a pair: zeros), dw[t, s] = <dout[t], y[j]>
  *                 (0 without a row);
  *                 dy or dw may be NULL (not both); y may be NULL without dw */
@@ -606,7 +607,7 @@ int cg3d_expert_plan(const void *experts, int32_t wide, int64_t n_tokens, int32_
 int cg3d_expert_gather(const void *x, int32_t dtype, const int32_t *rows, int64_t n_tokens, int32_t k, int32_t c, void *out,
                        cg3d_stream_t stream);
 int cg3d_expert_combine(const void *y, int32_t dtype, const int32_t *pos, const void *w, int32_t wtype, int64_t n_tokens, int32_t k,
-                        int32_t c, void *out, cg3d_stream_t stream);
+                        int32_t c, void *out, int32_t out_dtype, cg3d_stream_t stream);
 int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, const int32_t *pairs, const void *w, int32_t wtype,
                             int64_t n_tokens, int32_t k, int32_t c, void *dy, void *dw, cg3d_stream_t stream);
 

@@ -99,11 +99,11 @@ int cg3d_expert_gather(const void *x, int32_t dtype, const int32_t *rows, int64_
     return CG3D_OK;
 }
 int cg3d_expert_combine(const void *y, int32_t dtype, const int32_t *pos, const void *w, int32_t wtype, int64_t n_tokens, int32_t k,
-                        int32_t c, void *out, cg3d_stream_t stream) {
+                        int32_t c, void *out, int32_t out_dtype, cg3d_stream_t stream) {
     (void)stream;
-    if (bad(dtype, wtype, n_tokens, k, c)) return CG3D_ERR_ARG;
+    if (bad(dtype, wtype, n_tokens, k, c) || !fl(out_dtype) || (dtype != CG3D_DT_F32 && out_dtype != dtype)) return CG3D_ERR_ARG;
     if (n_tokens == 0) return CG3D_OK;
-    if (!y || !pos || !out || odd(y, dtype) || odd(out, dtype) || odd(w, wtype)) return CG3D_ERR_ARG;
+    if (!y || !pos || !out || odd(y, dtype) || odd(out, out_dtype) || odd(w, wtype)) return CG3D_ERR_ARG;
     for (int64_t t = 0; t < n_tokens; t++)
         for (int32_t a = 0; a < c; a++) {
             double acc = 0;
@@ -111,7 +111,7 @@ int cg3d_expert_combine(const void *y, int32_t dtype, const int32_t *pos, const 
                 const int32_t r = pos[t * k + s];
                 if (r >= 0 && r < n_tokens * k) acc += (w ? (double)ld(w, wtype, t * k + s) : 1.0) * ld(y, dtype, (int64_t)r * c + a);
             }
-            st(out, dtype, t * c + a, acc);
+            st(out, out_dtype, t * c + a, acc);
         }
     return CG3D_OK;
 }

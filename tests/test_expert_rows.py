@@ -150,7 +150,9 @@ def refusals(dev):
                 lambda: expert_gather(x, ids), lambda: expert_gather(x[:3], plan), lambda: expert_gather(x[:, :0], plan),
                 lambda: expert_gather(x.double(), plan), lambda: expert_gather(x[0], plan), lambda: expert_gather(None, plan),
                 lambda: expert_combine(x, plan), lambda: expert_combine(y.long(), plan), lambda: expert_combine(y, plan, w[:3]),
-                lambda: expert_combine(y, plan, w.t()), lambda: expert_combine(y, plan, w.double()), lambda: expert_combine(y, None, w)):
+                lambda: expert_combine(y, plan, w.t()), lambda: expert_combine(y, plan, w.double()), lambda: expert_combine(y, None, w),
+                lambda: expert_combine(y, plan, w, torch.float64), lambda: expert_combine(y.half(), plan, w, torch.float32),
+                lambda: expert_combine(y.half(), plan, w, torch.bfloat16)):
         with pytest.raises(_lib.CG3DError):
             bad()
 
@@ -173,10 +175,12 @@ def test_entry_points_refuse(oracle):
         assert lib.raw("cg3d_expert_plan_ws_bytes")(2 ** 31, 1, 3) == -1
         for dt, t, k, c in ((3, 4, 2, 8), (-1, 4, 2, 8), (0, -1, 2, 8), (0, 4, 0, 8), (0, 4, 2, 0), (0, 2 ** 31, 1, 8)):
             assert lib.raw("cg3d_expert_gather")(ok["x"], dt, ok["p"], t, k, c, ok["x"], None) == -1
-            assert lib.raw("cg3d_expert_combine")(ok["x"], dt, ok["p"], None, 0, t, k, c, ok["x"], None) == -1
+            assert lib.raw("cg3d_expert_combine")(ok["x"], dt, ok["p"], None, 0, t, k, c, ok["x"], max(dt, 0), None) == -1
             assert lib.raw("cg3d_expert_combine_bwd")(ok["x"], None, dt, ok["p"], None, 0, t, k, c, ok["x"], None, None) == -1
         assert lib.raw("cg3d_expert_gather")(ok["x"] + 2, 0, ok["p"], 4, 2, 8, ok["x"], None) == -1
-        assert lib.raw("cg3d_expert_combine")(ok["x"], 0, ok["p"], ok["x"], 3, 4, 2, 8, ok["x"], None) == -1
+        assert lib.raw("cg3d_expert_combine")(ok["x"], 0, ok["p"], ok["x"], 3, 4, 2, 8, ok["x"], 0, None) == -1
+        for dt, out in ((0, 3), (0, -1), (1, 0), (1, 2), (2, 0)):
+            assert lib.raw("cg3d_expert_combine")(ok["x"], dt, ok["p"], None, 0, 4, 2, 8, ok["x"], out, None) == -1
         assert lib.raw("cg3d_expert_combine_bwd")(ok["x"], ok["x"], 0, ok["p"], ok["x"], 0, 4, 2, 8, None, None, None) == -1
         assert lib.raw("cg3d_expert_combine_bwd")(ok["x"], None, 0, ok["p"], ok["x"], 0, 4, 2, 8, ok["x"], ok["x"], None) == -1
         assert lib.raw("cg3d_expert_gather")(None, 0, ok["p"], 4, 2, 8, ok["x"], None) == -1
@@ -247,6 +251,23 @@ def test_hip_shared_and_broadcast_inputs(hip):
     assert torch.equal(base.grad.double(), want)              # multiples of 0.75: exact
     ref = (2 * base.detach().double() * n).sum()
     assert abs(float(gate.grad) - float(ref)) < 1e-4 * float((2 * base.detach().double().abs() * n).sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("c", [3, 64, 129])
+def test_hip_fp32_rows_to_a_narrower_output(hip, out, c):
+    """One rounding only: fp32 rows, a 16-bit output, and its gradients, which are formed in fp32."""
+    ids = routing(300, 3, 7, "dropped", 50).cuda()
+    plan = expert_plan(ids, 7)
+    g = torch.Generator().manual_seed(51)
+    y, w = torch.randn(900, c, generator=g).cuda().requires_grad_(), torch.rand(300, 3, generator=g).cuda().requires_grad_()
+    do = torch.randn(300, c, generator=g).to(out).cuda()
+    got = expert_combine(y, plan, w, out)
+    wide = expert_combine(y, plan, w)
+    assert got.dtype == out and torch.equal(got, wide.to(out))
+    for a, b in zip(torch.autograd.grad(got, [y, w], do), torch.autograd.grad(wide, [y, w], do.float())):
+        assert a.dtype == torch.float32 and torch.equal(a, b)
 
 
 @pytest.mark.gpu

@@ -290,6 +290,15 @@ def test_hip_quantize_rows(hip, n, cin, dtype):
     check_levels(x, *quantize_rows(x))
 
 
+@pytest.mark.gpu
+def test_hip_large_tiles_are_reached(hip):
+    """Sizes whose products go to the largest tiles, dense and grouped, with a ragged last tile each way."""
+    dense(6500, 530, 1900, BF16, F32, True, 40, "cuda")
+    dense(6401, 576, 2052, I8, BF16, False, 41, "cuda")
+    grouped(ids_of(9000, 2, 4, "dropped", 42), 4, 600, 700, F32, F32, 2, True, 43, "cuda")
+    grouped(ids_of(20000, 1, 3, "uniform", 44), 3, 528, 640, I8, F16, 1, False, 45, "cuda")
+
+
 WIDE = [(1, 64, 64), (1, 4096, 256), (5, 512, 320), (16, 1000, 72), (31, 2048, 100), (64, 512, 512), (65, 576, 64), (127, 64, 128), (128, 128, 64),
         (300, 512, 192), (1003, 200, 77), (513, 1024, 300), (2050, 384, 136), (4099, 64, 64), (700, 1100, 520), (40, 43904, 128), (300, 9000, 64),
         (3, MAX_CIN, 5), (5000, 130, 40), (256, 2048, 512), (1000, 640, 640)]
