@@ -963,7 +963,7 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
     const bool padded = (cin & 15) || ((uintptr_t)x & 15);
     const i8_plan p = i8_choose(dtype, n_x, cin, n_rows, cout, n_experts, offsets != nullptr, padded);
     const int64_t panels = i8_panels(cout);
-    if (p.tiles > (1ll << 23) || (p.kind == i8_plan::TILE && p.tiles * p.ny > (1ll << 22))) return CG3D_ERR_ARG;      // (2^32 threads of a launch)
+    if (p.tiles >= (1ll << 24) || (p.kind == i8_plan::TILE && p.tiles * p.ny >= (p.big ? 1ll << 23 : 1ll << 24))) return CG3D_ERR_ARG;      // (2^32 threads of a launch)
     i8_args a = {sx, w, sw, bias, offsets, rows, y, n_rows, n_x, cin, cout, n_experts, out_dtype, bias_per_expert ? cout : 0};
     const int8_t *q = reinterpret_cast<const int8_t *>(x);
     int64_t pitch = cin;

@@ -623,7 +623,7 @@ int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, cons
  *     cg3d_int8_linear_ws_bytes bytes, 16-byte aligned, may be NULL where that is 0 (grouped = 1 for a call with offsets).  bias: NULL, [cout], or [n_experts][cout] (bias_per_expert = 1).
  *     Dense: offsets = rows = NULL, n_experts = 1, n_x = n_rows.  Grouped: offsets [n_experts + 1] of cg3d_expert_plan; row r of y
  *     is the product of row rows[r] of x (rows NULL: row r, n_x = n_rows) with its expert's matrix; rows at and behind
- *     offsets[n_experts] are zeros.  y [n_rows][cout] of out_dtype. */
+ *     offsets[n_experts] are zeros.  y [n_rows][cout] of out_dtype.  n_rows < 2^30, fewer than 2^36 results. */
 int64_t cg3d_int8_weight_bytes(int32_t n_experts, int32_t cin, int32_t cout);
 int cg3d_int8_weight(const void *w, int32_t dtype, int32_t n_experts, int32_t cin, int32_t cout, int8_t *packed, float *scale, void *ws,
                      cg3d_stream_t stream);

@@ -323,6 +323,37 @@ def test_hip_graph_replays_with_new_inputs(hip):
 
 
 @pytest.mark.gpu
+def test_hip_offsets_past_32_bits(hip):
+    """More than 2^31 elements of rows: gather, combination and gradient at the far end."""
+    t, k, e, c = 1100000, 2, 5, 1024
+    ids = routing(t, k, e, "uniform", 60).cuda()
+    plan = expert_plan(ids, e)
+    x = torch.randn(t, 8, device="cuda").to(torch.bfloat16).repeat(1, c // 8)
+    rows = expert_gather(x, plan)
+    tail = slice(t * k - 50, t * k)
+    assert torch.equal(rows[tail], x[plan.rows[tail].long()]) and torch.equal(rows[:50], x[plan.rows[:50].long()])
+    rows.requires_grad_()
+    w = torch.ones(t, k, device="cuda", requires_grad=True)
+    out = expert_combine(rows, plan, w)
+    assert torch.equal(out[-50:], (2 * x[-50:].float()).to(torch.bfloat16))
+    dy, dw = torch.autograd.grad(out, [rows, w], x)
+    assert torch.equal(dy[tail], x[plan.rows[tail].long()])
+    want = x[-50:].double().square().sum(1, keepdim=True).expand(50, k)
+    assert bool(((dw[-50:].double() - want).abs() <= (c + 1) * 2.0 ** -24 * want).all())
+
+
+@pytest.mark.gpu
+def test_hip_second_gradients_are_refused(hip):
+    ids = routing(20, 2, 3, "uniform", 61).cuda()
+    plan = expert_plan(ids, 3)
+    x, w = torch.randn(20, 8, device="cuda", requires_grad=True), torch.rand(20, 2, device="cuda", requires_grad=True)
+    out = expert_combine(expert_gather(x, plan), plan, w)
+    (g,) = torch.autograd.grad(out.square().sum(), [w], create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+@pytest.mark.gpu
 def test_hip_on_another_stream(hip):
     ids, x = routing(30000, 2, 18, "uniform", 30).cuda(), torch.randn(30000, 64, device="cuda")
     want = expert_gather(x, expert_plan(ids, 18))

@@ -301,7 +301,7 @@ def test_hip_large_tiles_are_reached(hip):
 
 WIDE = [(1, 64, 64), (1, 4096, 256), (5, 512, 320), (16, 1000, 72), (31, 2048, 100), (64, 512, 512), (65, 576, 64), (127, 64, 128), (128, 128, 64),
         (300, 512, 192), (1003, 200, 77), (513, 1024, 300), (2050, 384, 136), (4099, 64, 64), (700, 1100, 520), (40, 43904, 128), (300, 9000, 64),
-        (3, MAX_CIN, 5), (5000, 130, 40), (256, 2048, 512), (1000, 640, 640)]
+        (3, MAX_CIN, 5), (5000, 130, 40), (256, 2048, 512), (1000, 640, 640), (25001, 70, 260), (25000, 200, 130), (13000, 500, 264), (26000, 33, 64)]
 
 
 @pytest.mark.gpu
@@ -312,7 +312,8 @@ def test_hip_dense(hip, n, cin, cout, dtype, out, bias):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,cin,cout", [(70, 200, 77), (130, 64, 64), (5, 512, 64), (260, 1024, 128)])
+@pytest.mark.parametrize("n,cin,cout", [(70, 200, 77), (130, 64, 64), (5, 512, 64), (260, 1024, 128), (3000, 1024, 192),
+                                        (2000, 320, 320)])
 def test_hip_dense_at_odd_addresses(hip, n, cin, cout):
     for dtype, out in ((F32, F32), (BF16, BF16), (F16, F16), (I8, F32)):
         dense(n, cin, cout, dtype, out, True, 13, "cuda", offset=1)
@@ -323,7 +324,7 @@ def test_hip_dense_at_odd_addresses(hip, n, cin, cout):
     (1, 1, 1, 64, 64, "uniform"), (1, 2, 18, 128, 64, "uniform"), (4, 2, 64, 512, 512, "uniform"), (20, 2, 5, 33, 18, "dropped"),
     (300, 2, 18, 128, 64, "dropped"), (300, 2, 18, 128, 64, "one"), (50, 2, 7, 70, 90, "none"), (900, 4, 61, 96, 200, "uniform"),
     (64, 1, 200, 100, 70, "uniform"), (1500, 2, 3, 640, 256, "dropped"), (700, 2, 4, 1024, 130, "uniform"), (3000, 2, 10, 64, 64, "uniform"),
-    (16, 4, 1024, 64, 32, "uniform")])
+    (16, 4, 1024, 64, 32, "uniform"), (13000, 2, 5, 130, 300, "dropped"), (9000, 3, 7, 500, 130, "uniform")])
 @pytest.mark.parametrize("dtype,out,bias,gather", [(F32, F32, 2, True), (BF16, BF16, 0, True), (F16, F16, 1, False), (I8, F32, 2, True), (I8, BF16, 2, False)])
 def test_hip_grouped(hip, t, k, experts, cin, cout, kind, dtype, out, bias, gather):
     grouped(ids_of(t, k, experts, kind, 14), experts, cin, cout, dtype, out, bias, gather, 15, "cuda")
@@ -409,6 +410,40 @@ def test_hip_graph_replays_with_new_inputs(hip):
             g.replay()
         for j in range(2):
             assert torch.equal(outs[j], step(ids[(turn + j) % 3], xs[(turn + j) % 3]))
+
+
+@pytest.mark.gpu
+def test_hip_large_tiles_in_a_graph(hip):
+    x, _, w, b = make(6500, 600, 1900, BF16, 46)
+    x, weight, b = x.cuda(), int8_weight(w.cuda()), b.cuda()
+    other = make(6500, 600, 1, BF16, 47)[0].cuda()
+    static = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    int8_linear(static, weight, b)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = int8_linear(static, weight, b)
+    for v in (x, other, x):
+        static.copy_(v)
+        graph.replay()
+        assert torch.equal(out, int8_linear(v, weight, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,cin,cout", [(2200000, 64, 1024), (600000, 4096, 64), (36, 512, 1 << 20)])
+def test_hip_offsets_past_32_bits(hip, n, cin, cout):
+    """Results (or rows, or a matrix) of more than 2^31 bytes: the last rows and channels are those of a small call."""
+    g = torch.Generator(device="cuda").manual_seed(48)
+    x = torch.randint(-128, 128, (n, cin), generator=g, device="cuda", dtype=torch.int32).to(I8) if n * cin < 2 ** 28 else \
+        torch.randint(-128, 128, (n // 8, cin), generator=g, device="cuda", dtype=torch.int32).to(I8).repeat(8, 1)
+    sx = torch.rand(n, generator=g, device="cuda") + 0.1
+    wq = torch.randint(-128, 128, (cin, cout), generator=g, device="cuda", dtype=torch.int32).to(I8)
+    sw = torch.rand(cout, generator=g, device="cuda") + 0.1
+    y = int8_linear(x, int8_weight(wq, sw), scale=sx, out_dtype=BF16)
+    for rows in (slice(0, 20), slice(n - 20, n)):
+        for cols in (slice(0, 70), slice(max(0, cout - 70), cout)):
+            want = int8_linear(x[rows], int8_weight(wq[:, cols].contiguous(), sw[cols].contiguous()), scale=sx[rows], out_dtype=BF16)
+            assert torch.equal(y[rows, cols], want)
 
 
 @pytest.mark.gpu
