@@ -73,13 +73,15 @@ def _plan_ws_words(lib, t, k, n_experts):
 def expert_plan(experts, n_experts):
     """experts int32 / int64 [T, k] (or [T]): the experts of each token; an id outside [0, n_experts) has no row.  A token may
     name an expert twice: it then has two rows.  Rows are in expert order, pairs of one expert in the order of (token, slot)."""
-    need(isinstance(experts, torch.Tensor) and experts.dtype in (torch.int32, torch.int64) and experts.dim() in (1, 2),
-         "expert_plan: experts must be an int32 or int64 tensor [T, k] or [T]")
+    if not (isinstance(experts, torch.Tensor) and experts.dtype in (torch.int32, torch.int64) and experts.dim() in (1, 2)):
+        raise CG3DError("expert_plan: experts must be an int32 or int64 tensor [T, k] or [T]")
     n_experts = int(n_experts)
-    need(1 <= n_experts <= MAX_EXPERTS, "expert_plan: n_experts = %d is not in 1 .. %d", n_experts, MAX_EXPERTS)
+    if not 1 <= n_experts <= MAX_EXPERTS:
+        raise CG3DError("expert_plan: n_experts = %d is not in 1 .. %d" % (n_experts, MAX_EXPERTS))
     ids = (experts if experts.dim() == 2 else experts.unsqueeze(1)).contiguous()
     t, k = ids.shape
-    need(k >= 1 and t * k < 2 ** 31, "expert_plan: %d x %d pairs (k >= 1, fewer than 2^31 pairs)", t, k)
+    if k < 1 or t * k >= 2 ** 31:
+        raise CG3DError("expert_plan: %d x %d pairs (k >= 1, fewer than 2^31 pairs)" % (t, k))
     lib = _lib.get()
     lib.check(ids)
     with on_device(ids):

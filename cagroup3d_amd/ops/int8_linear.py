@@ -22,21 +22,19 @@ MAX_CIN = 131071                  # the int32 sum of so many products of 8-bit v
 
 
 def _no_grad_for(who, *tensors):
-    need(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)),
-         "%s has no gradient: call it under torch.no_grad() or on detached tensors", who)
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise CG3DError("%s has no gradient: call it under torch.no_grad() or on detached tensors" % who)
 
 
 class Int8Weight:
     """Weights in the product kernels' order.  packed int8 (cg3d_int8_weight_bytes), scale float32 [E, cout]."""
 
-    __slots__ = ("packed", "scale", "n_experts", "cin", "cout", "grouped")
+    __slots__ = ("packed", "scale", "n_experts", "cin", "cout", "grouped", "device", "packed_ptr", "scale_ptr")
 
     def __init__(self, packed, scale, n_experts, cin, cout, grouped):
         self.packed, self.scale, self.n_experts, self.cin, self.cout, self.grouped = packed, scale, n_experts, cin, cout, grouped
-
-    @property
-    def device(self):
-        return self.packed.device
+        self.device, self.packed_ptr, self.scale_ptr = packed.device, packed.data_ptr(), scale.data_ptr()
 
 
 def int8_weight(w, scale=None):
@@ -102,49 +100,54 @@ def int8_linear(x, weight, bias=None, scale=None, out_dtype=None, plan=None, gat
 
     plan (ops/expert_rows.expert_plan): weight holds plan.n_experts matrices and each row is multiplied by its expert's; x has the
     plan's rows ([T * k, cin], what expert_gather gives), or with gather=True the tokens ([T, cin]), whose rows are picked in the
-    product -- quantised once for a token, not once for a row.  Rows behind the last are zeros."""
-    need(isinstance(weight, Int8Weight), "int8_linear: weight must come from int8_weight")
+    product.  Rows behind the last are zeros."""
+    # (plain comparisons before any message is made: the call's host time is that of a small product)
+    if not isinstance(weight, Int8Weight):
+        raise CG3DError("int8_linear: weight must come from int8_weight")
     _rows_in("int8_linear", x, ROWS_IN)
-    need(x.shape[1] == weight.cin, "int8_linear: x has %d columns, weight %d rows", x.shape[1], weight.cin)
-    in8 = x.dtype == torch.int8
-    out_dtype = out_dtype or (torch.float32 if in8 else x.dtype)
-    need(out_dtype in FLOATS, "int8_linear: out_dtype must be float32, bfloat16 or float16")
-    n_x = n_rows = x.shape[0]
-    if in8:
-        need(isinstance(scale, torch.Tensor) and scale.dtype == torch.float32 and scale.shape == (n_x,),
-             "int8_linear: rows in 8 bits need their scale, float32 [%d]", n_x)
+    n_x, cin = x.shape
+    dtype, dev, cout, n_experts = x.dtype, x.device, weight.cout, weight.n_experts
+    if cin != weight.cin:
+        raise CG3DError("int8_linear: x has %d columns, weight %d rows" % (cin, weight.cin))
+    if weight.device != dev:
+        raise CG3DError("int8_linear: x is on %s, weight on %s" % (dev, weight.device))
+    if dtype is torch.int8:
+        need(isinstance(scale, torch.Tensor) and scale.dtype == torch.float32 and scale.shape == (n_x,) and scale.device == dev,
+             "int8_linear: rows in 8 bits need their scale beside them, float32 [%d]", n_x)
+        out_dtype = out_dtype or torch.float32
+        scale = scale.contiguous()
     else:
         need(scale is None, "int8_linear: the scale of rows in floats is computed here")
+        out_dtype = out_dtype or dtype
+    if out_dtype not in FLOATS:
+        raise CG3DError("int8_linear: out_dtype must be float32, bfloat16 or float16")
     if plan is None:
-        need(weight.n_experts == 1 and not gather, "int8_linear: %d matrices (or gather) need a plan", weight.n_experts)
+        if n_experts != 1 or gather:
+            raise CG3DError("int8_linear: %d matrices (or gather) need a plan" % n_experts)
+        n_rows, offsets, rows = n_x, None, None
     else:
-        need(isinstance(plan, ExpertPlan), "int8_linear: plan must come from expert_plan")
-        need(weight.n_experts == plan.n_experts, "int8_linear: %d matrices for a plan of %d experts", weight.n_experts, plan.n_experts)
+        need(isinstance(plan, ExpertPlan) and plan.device == dev, "int8_linear: plan must come from expert_plan, on %s", dev)
+        need(n_experts == plan.n_experts, "int8_linear: %d matrices for a plan of %d experts", n_experts, plan.n_experts)
         n_rows = plan.n_rows
         need(n_x == (plan.n_tokens if gather else n_rows), "int8_linear: x has %d rows, the plan %d tokens and %d rows", n_x, plan.n_tokens, n_rows)
+        offsets, rows = plan.address(OFFSETS), plan.address(ROWS) if gather else None
     per_expert = 0
     if bias is not None:
+        need(isinstance(bias, torch.Tensor) and bias.dtype in FLOATS and bias.device == dev and (
+            bias.shape == (cout,) or (weight.grouped and bias.shape == (n_experts, cout))),
+            "int8_linear: bias must be floats [%d] (or [%d, %d] with a matrix for each expert) on %s", cout, n_experts, cout, dev)
         per_expert = int(bias.dim() == 2)
-        if bias.dtype not in FLOATS or not (bias.shape == (weight.cout,) or (weight.grouped and bias.shape == (weight.n_experts, weight.cout))):
-            raise CG3DError("int8_linear: bias must be floats [%d]%s, got %s" % (
-                weight.cout, " or [%d, %d]" % (weight.n_experts, weight.cout) if weight.grouped else "", tuple(bias.shape)))
     _no_grad_for("int8_linear", x, bias, scale)
-    for t in (weight, bias, scale, plan):
-        if t is not None and t.device != x.device:
-            raise CG3DError("int8_linear: x is on %s, another argument on %s" % (x.device, t.device))
-    lib = _lib.get()
-    x = x.contiguous()
     if bias is not None:
         bias = bias.detach().to(torch.float32).contiguous()
-    if scale is not None:
-        scale = scale.contiguous()
-    lib.check(x, bias, scale)
-    code = DTYPES[x.dtype]
+    lib = _lib.get()
+    x = x.contiguous()
+    lib.check(x)
+    code = DTYPES[dtype]
     with on_device(x):
-        ws_bytes = _ws_bytes(lib, code, n_x, weight.cin, n_rows, weight.cout, weight.n_experts, int(plan is not None))
-        y = torch.empty((n_rows, weight.cout), dtype=out_dtype, device=x.device)
-        ws = torch.empty(ws_bytes, dtype=torch.int8, device=x.device) if ws_bytes > 0 else None
-        lib.call("cg3d_int8_linear", x.data_ptr(), code, ptr(scale), n_x, weight.cin, weight.packed.data_ptr(), weight.scale.data_ptr(), ptr(bias),
-                 per_expert, None if plan is None else plan.address(OFFSETS), plan.address(ROWS) if gather else None, y.data_ptr(),
-                 DTYPES[out_dtype], n_rows, weight.cout, weight.n_experts, ptr(ws), lib.stream())
+        ws_bytes = _ws_bytes(lib, code, n_x, cin, n_rows, cout, n_experts, int(plan is not None))
+        y = torch.empty((n_rows, cout), dtype=out_dtype, device=dev)
+        ws = torch.empty(ws_bytes, dtype=torch.int8, device=dev) if ws_bytes > 0 else None
+        lib.call("cg3d_int8_linear", x.data_ptr(), code, ptr(scale), n_x, cin, weight.packed_ptr, weight.scale_ptr, ptr(bias), per_expert,
+                 offsets, rows, y.data_ptr(), DTYPES[out_dtype], n_rows, cout, n_experts, ptr(ws), lib.stream())
     return y
