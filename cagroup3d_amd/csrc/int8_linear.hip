@@ -31,8 +31,6 @@ typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 #define I8_MAX_CIN 131071            // 2^14 * 131071 < 2^31: -128 * -128 included
 #define I8_MAX_EXPERTS 1024
 #define I8_FUSED_CIN 512
-#define I8_SPLIT 256
-#define I8_WANT 384
 
 template <typename T, int V> struct __attribute__((packed, aligned(1))) i8_vec { T e[V]; };
 
@@ -906,11 +904,18 @@ static int64_t i8_pitch(int32_t cin) { return i8_chunks(cin) * 64; }
 static i8_plan i8_choose(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts, bool grouped, bool padded) {
     i8_plan p = {};
     const int64_t chunks = i8_chunks(cin), panels = i8_panels(cout);
-    auto tiles = [&](int bm) { return grouped ? n_rows / bm + n_experts + 1 : cg3d_divup(n_rows, bm); };
-    // workgroups of the kernel for few rows (empty experts' leave at once): up to two for a CU it is the fastest, one where rows are short;
-    // of long rows each of them would read too much by itself
-    const int64_t few = (n_rows / 16 + (grouped ? (n_experts < n_rows ? n_experts : n_rows) : 1)) * panels * 2;
-    if (few <= (chunks <= 2 ? 256 : 512) && chunks <= 128) {
+    // (a list of rows has at most one tile that is not full, and only lists with rows have tiles: at most so many, and those of the rows
+    // behind the last)
+    const int64_t lists = n_experts < n_rows ? n_experts : n_rows;
+    auto tiles = [&](int bm) { return grouped ? n_rows / bm + lists + 1 : cg3d_divup(n_rows, bm); };
+    // The kernel for few rows, by its workgroups (about 2.5 us for each 256 of them, more where rows are long) against what the others
+    // take for any number of rows.  512 -> 512 bf16: 128 rows 4.6 against 7.7 us, 512 rows (528) 7.5 / 7.8, 1024 rows 12.9 / 8.0; 8 experts
+    // of it, 64 / 256 rows 6.0 / 8.8 and (384) 9.4 / 9.1.  Where the others quantise first: 1024 -> 1024, 128 rows 5.5 / 12.9, 512 rows
+    // (1056) 16.3 / 15.4; 768 -> 768, 512 rows (792) 11.5 / 14.5, 1024 rows (1560) 21 / 14.6; 18 experts of 1024 -> 1024, 256 rows (1088)
+    // 19 / 33; 4096 -> 4096, 32 rows (384) 12.8 / 17.9, 64 rows (640) 19.6 / 20.4.  Of very long rows each would read too much by itself
+    // (512 x 43 904 -> 128: 38 us against 18).
+    const int64_t few = (n_rows / 16 + (grouped ? lists : 1)) * panels * 2;
+    if (cin <= I8_FUSED_CIN ? few <= 320 : chunks <= 128 && (few <= 384 || few * chunks <= 18000)) {
         p.kind = i8_plan::FEW;
         p.tiles = tiles(16);
         p.rows8 = dtype != CG3D_DT_I8 && chunks > 8 * (dtype == CG3D_DT_F32 ? i8_few<float>::CHUNKS : i8_few<i8_bf16>::CHUNKS);
@@ -920,13 +925,13 @@ static i8_plan i8_choose(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows
     } else {
         p.kind = i8_plan::TILE;
         p.rows8 = dtype != CG3D_DT_I8 || padded;
-        p.big = tiles(256) * cg3d_divup(panels, 4) >= 200;
+        p.big = tiles(256) * cg3d_divup(panels, 4) >= 200;           // (a round of 256 x 256 tiles nearly full)
         p.ny = (int32_t)cg3d_divup(panels, p.big ? 4 : 2);
         p.tiles = tiles(p.big ? 256 : 128);
         const int64_t total = p.tiles * p.ny;
         p.splits = 1;
-        if (!p.big && total < 256) {                                 // half the chip's places empty: the contraction is shared out
-            const int64_t want = cg3d_divup(I8_SPLIT, total), most = chunks / 8;
+        if (!p.big && total < 256) {                                 // fewer tiles than CUs: the contraction is shared out, 8 chunks or more
+            const int64_t want = cg3d_divup(256, total), most = chunks / 8;        // (512 x 43 904 -> 128, tile + join: 14.3 + 5.5 / 11.7 + 6.8 / 15.8 + 7.8 us for 128 / 256 / 512)
             p.splits = (int32_t)(want < most ? want : most > 1 ? most : 1);
         }
     }
@@ -996,8 +1001,11 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
         return CG3D_OK;
     }
     if (p.kind == i8_plan::FUSED) {
-        // enough workgroups for the chip: the panels of a row tile are shared out where there are fewer than 1024 tiles
-        const int32_t parts = (int32_t)(cg3d_divup(I8_WANT, p.tiles) < panels ? cg3d_divup(I8_WANT, p.tiles) : panels);
+        // enough workgroups for the chip: the panels of a row tile are shared out where there are fewer than 384 tiles, though each part
+        // quantises the rows for itself (512 -> 512, 10 000 rows: 20.6 / 16.4 / 18.3 / 16.9 / 25.4 us at 128 / 256 / 384 / 512 / 1024
+        // wanted, 20 000 rows 24.7 / 24.5 / 22.0 / 21.9 / 27.9; 512 -> 2048, 5000 rows 33.4 / 22.7 / 23.9 / 26.8 / 26.0)
+        const int64_t want = cg3d_divup(384, p.tiles);
+        const int32_t parts = (int32_t)(want < panels ? want : panels);
         const int32_t each = (int32_t)cg3d_divup(panels, parts);
         const int lds = (int)i8_chunks(cin) * 4096 + 256;           // (at most 32.25 KB)
 #define I8_F(T, RG, KEEP) hipLaunchKernelGGL((k_i8_fused<T, RG, KEEP>), dim3((unsigned)p.tiles, (unsigned)parts), dim3(256), lds, s, a, reinterpret_cast<const T *>(x))
