@@ -650,12 +650,12 @@ __global__ __launch_bounds__(256, RG == 4 || KEEP * sizeof(T) > 8 ? 4 : RG == 2 
 // floats that fit (CHUNKS chunks of a wave) are quantised here, in the operand's own layout -- each workgroup finds the rows' maxima for
 // itself, through LDS; the waves' sums are joined there too.  grid: (16-row tiles, pairs of tiles).
 template <typename T> struct i8_few { static constexpr int CHUNKS = sizeof(T) == 4 ? 4 : 8; };
-template <typename T>
-__global__ __launch_bounds__(512, 2) void k_i8_few(i8_args a, const T *__restrict__ x, int64_t pitch) {
+template <typename T, int KEEP>
+__global__ __launch_bounds__(512, KEEP == 1 || (KEEP == 2 && !__is_same(T, float) && !__is_same(T, i8_f16)) ? 6 : KEEP * sizeof(T) <= 8 ? 4 : 2) void k_i8_few(i8_args a, const T *__restrict__ x, int64_t pitch) {
     __shared__ i32x4 part[8][2][64];
     __shared__ uint32_t tops[8][16];
     __shared__ float scales[16];
-    constexpr int KEEP = i8_few<T>::CHUNKS, NI = sizeof(T), N = i8_els<T>;
+    constexpr int NI = sizeof(T), N = i8_els<T>;
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int panels = (a.cout + 63) >> 6, chunks = (a.cin + 63) >> 6, panel = blockIdx.y >> 1, pair = blockIdx.y & 1;
     int e, rows;
@@ -831,8 +831,9 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void k_i8_tile(i8_args a, const in
         i32x4 *to = part + ((((int64_t)blockIdx.z * total + id) * NW + wave) * (RG * 4)) * 64 + lane;
 #pragma unroll
         for (int h = 0; h < RG; h++)
+            if ((wr * RG + h) * 16 < rows)                          // (a group without rows is not joined either)
 #pragma unroll
-            for (int nb = 0; nb < 4; nb++) to[(h * 4 + nb) * 64] = acc[h][nb];
+                for (int nb = 0; nb < 4; nb++) to[(h * 4 + nb) * 64] = acc[h][nb];
         return;
     }
     const int panel = by * WC + wc;
@@ -908,14 +909,17 @@ static i8_plan i8_choose(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows
     // behind the last)
     const int64_t lists = n_experts < n_rows ? n_experts : n_rows;
     auto tiles = [&](int bm) { return grouped ? n_rows / bm + lists + 1 : cg3d_divup(n_rows, bm); };
-    // The kernel for few rows, by its workgroups (about 2.5 us for each 256 of them, more where rows are long) against what the others
-    // take for any number of rows.  512 -> 512 bf16: 128 rows 4.6 against 7.7 us, 512 rows (528) 7.5 / 7.8, 1024 rows 12.9 / 8.0; 8 experts
-    // of it, 64 / 256 rows 6.0 / 8.8 and (384) 9.4 / 9.1.  Where the others quantise first: 1024 -> 1024, 128 rows 5.5 / 12.9, 512 rows
-    // (1056) 16.3 / 15.4; 768 -> 768, 512 rows (792) 11.5 / 14.5, 1024 rows (1560) 21 / 14.6; 18 experts of 1024 -> 1024, 256 rows (1088)
-    // 19 / 33; 4096 -> 4096, 32 rows (384) 12.8 / 17.9, 64 rows (640) 19.6 / 20.4.  Of very long rows each would read too much by itself
-    // (512 x 43 904 -> 128: 38 us against 18).
-    const int64_t few = (n_rows / 16 + (grouped ? lists : 1)) * panels * 2;
-    if (cin <= I8_FUSED_CIN ? few <= 320 : chunks <= 128 && (few <= 384 || few * chunks <= 18000)) {
+    // The kernel for few rows: at most three workgroups a CU where the rows are short, else by its weights' fragments (half as many for
+    // rows of fp32, which take it twice as long) against the rounds of 128 x 128 tiles, one to a CU, that the others would need.  Its
+    // time against theirs, bf16: 512 -> 512, 500 rows (512 workgroups) 6.2 / 8.7 us, 1000 rows (1008) 8.5 / 8.9, 2000 rows 12.6 / 9.3;
+    // 128 -> 128, 2000 rows (504) 5.4 / 6.0, 4000 rows (1004) 6.8 / 6.1; 18 experts of it, 2000 rows (572) 6.5 / 6.8.  1024 -> 1024, 500
+    // rows 10.8 / 16.7, 1000 rows (32 256 fragments) 17.5 / 16.8 (fp32, 500 rows 15.8 / 16.8); 2048 -> 2048, 250 rows (32 768) 17.1 / 21.2 (fp32,
+    // 128 rows 17.6 / 21.1); 18 experts of 1024 -> 1024, 512 rows (25 600) 16.1 / 17.2, 1200 rows (47 616) 27.9 / 20.8; 64 experts of it, 64
+    // rows (35 328, 2 rounds) 16.4 / 38.6, 1000 rows (64 512) 31.6 / 40.8, 2000 rows (96 768) 49.4 / 45.8.  Of very long rows each would read
+    // too much by itself (512 x 43 904 -> 128: 38 us against 18).
+    const int64_t few = (n_rows / 16 + (grouped ? lists : 1)) * panels * 2, rounds256 = tiles(128) * cg3d_divup(panels, 2);
+    const int64_t most_few = (dtype == CG3D_DT_F32 ? 16500 : 33000) * (rounds256 > 256 ? rounds256 : 256) / 256;
+    if (cin <= I8_FUSED_CIN ? few <= 768 : chunks <= 128 && (few <= 384 || few * chunks <= most_few)) {
         p.kind = i8_plan::FEW;
         p.tiles = tiles(16);
         p.rows8 = dtype != CG3D_DT_I8 && chunks > 8 * (dtype == CG3D_DT_F32 ? i8_few<float>::CHUNKS : i8_few<i8_bf16>::CHUNKS);
@@ -930,9 +934,13 @@ static i8_plan i8_choose(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows
         p.tiles = tiles(p.big ? 256 : 128);
         const int64_t total = p.tiles * p.ny;
         p.splits = 1;
-        if (!p.big && total < 256) {                                 // fewer tiles than CUs: the contraction is shared out, 8 chunks or more
-            const int64_t want = cg3d_divup(256, total), most = chunks / 8;        // (512 x 43 904 -> 128, tile + join: 14.3 + 5.5 / 11.7 + 6.8 / 15.8 + 7.8 us for 128 / 256 / 512)
-            p.splits = (int32_t)(want < most ? want : most > 1 ? most : 1);
+        if (!p.big && chunks > 32) {
+            // The contraction is shared out while that fills CUs that have no tile, at 16 chunks or more.  Tile + join, rows in 8 bits: 4096 ->
+            // 4096, 100 rows (32 tiles) 16.9 us in 4 parts, 19.0 in 2; 43 904 -> 128, 512 rows 18.0 us in 64, 19.5 in 21.  With 32 chunks or
+            // fewer the join takes what the parts save: 2048 -> 2048, 1000 rows (128 tiles) 22.1 us in 2 parts, 18.4 in one; 1024 -> 1024, 2000
+            // rows 23.0 and 13.0.
+            const int64_t want = 256 / total, most = chunks / 16;
+            p.splits = (int32_t)(want < 1 ? 1 : want < most ? want : most);
         }
     }
     int64_t at = 0;
@@ -993,10 +1001,15 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
         const dim3 grid((unsigned)p.tiles, (unsigned)(panels * 2));
         if (panels * 2 > 65535) return CG3D_ERR_ARG;
         if (p.rows8) a.cin = (int32_t)pitch;                         // (zeros behind the row: whole pieces)
-        if (dtype == CG3D_DT_F32) hipLaunchKernelGGL((k_i8_few<float>), grid, dim3(512), 0, s, a, reinterpret_cast<const float *>(x), pitch);
-        else if (dtype == CG3D_DT_BF16) hipLaunchKernelGGL((k_i8_few<i8_bf16>), grid, dim3(512), 0, s, a, reinterpret_cast<const i8_bf16 *>(x), pitch);
-        else if (dtype == CG3D_DT_F16) hipLaunchKernelGGL((k_i8_few<i8_f16>), grid, dim3(512), 0, s, a, reinterpret_cast<const i8_f16 *>(x), pitch);
-        else hipLaunchKernelGGL((k_i8_few<int8_t>), grid, dim3(512), 0, s, a, q, pitch);
+        const int64_t each = cg3d_divup(i8_chunks(a.cin), 8);        // chunks of a wave
+#define I8_FEW(T, KEEP) hipLaunchKernelGGL((k_i8_few<T, KEEP>), grid, dim3(512), 0, s, a, reinterpret_cast<const T *>(x), pitch)
+#define I8_FEW_K(T) do { if (each <= 1) I8_FEW(T, 1); else if (each <= 2) I8_FEW(T, 2); else if (each <= 4) I8_FEW(T, 4); else I8_FEW(T, 8); } while (0)
+        if (dtype == CG3D_DT_F32) { if (each <= 1) I8_FEW(float, 1); else if (each <= 2) I8_FEW(float, 2); else I8_FEW(float, 4); }
+        else if (dtype == CG3D_DT_BF16) I8_FEW_K(i8_bf16);
+        else if (dtype == CG3D_DT_F16) I8_FEW_K(i8_f16);
+        else I8_FEW_K(int8_t);
+#undef I8_FEW_K
+#undef I8_FEW
         CG3D_CHECK_LAUNCH();
         return CG3D_OK;
     }
