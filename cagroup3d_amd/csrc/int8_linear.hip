@@ -998,8 +998,7 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
         x = lev;
     }
     if (p.kind == i8_plan::FEW) {
-        const dim3 grid((unsigned)p.tiles, (unsigned)(panels * 2));
-        if (panels * 2 > 65535) return CG3D_ERR_ARG;
+        const dim3 grid((unsigned)p.tiles, (unsigned)(panels * 2));      // (at most 2^15)
         if (p.rows8) a.cin = (int32_t)pitch;                         // (zeros behind the row: whole pieces)
         const int64_t each = cg3d_divup(i8_chunks(a.cin), 8);        // chunks of a wave
 #define I8_FEW(T, KEEP) hipLaunchKernelGGL((k_i8_few<T, KEEP>), grid, dim3(512), 0, s, a, reinterpret_cast<const T *>(x), pitch)

@@ -30,11 +30,11 @@ def _no_grad_for(who, *tensors):
 class Int8Weight:
     """Weights in the product kernels' order.  packed int8 (cg3d_int8_weight_bytes), scale float32 [E, cout]."""
 
-    __slots__ = ("packed", "scale", "n_experts", "cin", "cout", "grouped", "device", "packed_ptr", "scale_ptr")
+    __slots__ = ("packed", "scale", "n_experts", "cin", "cout", "grouped", "device")
 
     def __init__(self, packed, scale, n_experts, cin, cout, grouped):
         self.packed, self.scale, self.n_experts, self.cin, self.cout, self.grouped = packed, scale, n_experts, cin, cout, grouped
-        self.device, self.packed_ptr, self.scale_ptr = packed.device, packed.data_ptr(), scale.data_ptr()
+        self.device = packed.device
 
 
 def int8_weight(w, scale=None):
@@ -60,7 +60,7 @@ def int8_weight(w, scale=None):
         if scale is None:
             out, ws = torch.empty((2, e, cout), dtype=torch.float32, device=w.device)
         else:
-            out, ws = scale.detach().clone().view(e, cout), None          # (the handle's own: the caller may reuse the memory)
+            out, ws = scale.detach().clone(memory_format=torch.contiguous_format).view(e, cout), None      # (the handle's own: the caller may reuse the memory)
         lib.call("cg3d_int8_weight", ptr(w), DTYPES[w.dtype], e, cin, cout, ptr(packed),
                  ptr(out) if ws is not None else None, ptr(ws), lib.stream())
     return Int8Weight(packed, out, e, cin, cout, grouped)
@@ -148,6 +148,6 @@ def int8_linear(x, weight, bias=None, scale=None, out_dtype=None, plan=None, gat
         ws_bytes = _ws_bytes(lib, code, n_x, cin, n_rows, cout, n_experts, int(plan is not None))
         y = torch.empty((n_rows, cout), dtype=out_dtype, device=dev)
         ws = torch.empty(ws_bytes, dtype=torch.int8, device=dev) if ws_bytes > 0 else None
-        lib.call("cg3d_int8_linear", x.data_ptr(), code, ptr(scale), n_x, cin, weight.packed_ptr, weight.scale_ptr, ptr(bias), per_expert,
+        lib.call("cg3d_int8_linear", x.data_ptr(), code, ptr(scale), n_x, cin, weight.packed.data_ptr(), weight.scale.data_ptr(), ptr(bias), per_expert,
                  offsets, rows, y.data_ptr(), DTYPES[out_dtype], n_rows, cout, n_experts, ptr(ws), lib.stream())
     return y

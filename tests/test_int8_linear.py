@@ -4,6 +4,9 @@ CPU (-m "not gpu"): the oracle's restatement against a plain implementation in 6
 against the same -- every type in and out, sizes around the tiles, long contractions, single rows, experts without rows, dropped
 pairs, gathered rows -- the levels at exact ties and at the ends of the types' ranges, a captured graph, another stream, a layer of
 experts as it is served."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -274,6 +277,24 @@ def test_no_cpu_fallback():
 
 
 # ------------------------------------------------------------------------------------------------------------------- GPU
+def weights_that_are_views_or_copies(dev):
+    g = torch.Generator().manual_seed(60)
+    w, scale = torch.randint(-127, 128, (3, 40, 20), generator=g).to(I8).to(dev), (torch.rand(20, 3, generator=g) + 0.1).to(dev)
+    x, plan = torch.randn(12, 40, generator=g).to(dev), expert_plan(torch.arange(12).remainder(3).to(dev), 3)
+    weight = int8_weight(w, scale.t())                            # (its columns are the neighbours in memory)
+    y = int8_linear(x, weight, plan=plan, gather=True)
+    assert torch.equal(y, int8_linear(x, int8_weight(w, scale.t().contiguous()), plan=plan, gather=True))
+    for other in (copy.deepcopy(weight), pickle.loads(pickle.dumps(weight))):      # own memory, also when the first is gone
+        weight.packed.zero_()
+        assert torch.equal(int8_linear(x, other, plan=plan, gather=True), y)
+        weight.packed.copy_(other.packed)
+
+
+def test_weights_that_are_views_or_copies(oracle):
+    with _lib.use_library(oracle):
+        weights_that_are_views_or_copies("cpu")
+
+
 @pytest.mark.gpu
 def test_hip_levels_and_nonfinite(hip):
     levels("cuda")
@@ -288,6 +309,29 @@ def test_hip_levels_and_nonfinite(hip):
 def test_hip_quantize_rows(hip, n, cin, dtype):
     x = make(n, cin, 1, dtype, 11)[0].cuda()
     check_levels(x, *quantize_rows(x))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,cin,cout", [
+    (20, 500, 70), (50, 1000, 70), (50, 1900, 40), (20, 4000, 70), (20, 6000, 70),                          # few rows, by the chunks a wave holds
+    (25000, 60, 60), (25000, 60, 130), (25000, 120, 130), (25000, 120, 250), (25000, 300, 250), (25000, 300, 60), (25000, 300, 130),
+    (1700, 300, 250),                                                                                       # one pass: panels of a wave, chunks held
+    (3000, 4100, 130), (3000, 700, 700)])                                                                   # tiles, in parts and whole
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (F16, F16), (I8, F32)])
+def test_hip_each_kernel_of_the_choice(hip, n, cin, cout, dtype, out):
+    dense(n, cin, cout, dtype, out, True, 50, "cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,k,experts,cin,cout", [(1500, 2, 5, 4200, 130), (300, 2, 18, 1000, 200), (60, 2, 64, 1000, 520)])
+@pytest.mark.parametrize("dtype,out,gather", [(F32, F32, True), (BF16, BF16, True), (I8, F32, False)])
+def test_hip_grouped_long_rows(hip, t, k, experts, cin, cout, dtype, out, gather):
+    grouped(ids_of(t, k, experts, "dropped", 51), experts, cin, cout, dtype, out, 2, gather, 52, "cuda")
+
+
+@pytest.mark.gpu
+def test_hip_weights_that_are_views_or_copies(hip):
+    weights_that_are_views_or_copies("cuda")
 
 
 @pytest.mark.gpu
