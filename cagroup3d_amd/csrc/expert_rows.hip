@@ -374,12 +374,12 @@ __global__ __launch_bounds__(256) void k_expert_combine_bwd(const T *__restrict_
 }
 
 static bool ex_bad(int32_t dtype, int32_t wtype, int64_t n_tokens, int32_t k, int32_t c) {
-    return dtype < CG3D_DT_F32 || dtype > CG3D_DT_F16 || wtype < CG3D_DT_F32 || wtype > CG3D_DT_F16 || n_tokens < 0 || k < 1 || c < 1 ||
+    return dtype < CG3D_DT_F32 || dtype > CG3D_DT_F16 || wtype < CG3D_DT_F32 || wtype > CG3D_DT_F16 || n_tokens < 0 || k < 1 || c < 1 || c > (1 << 30) ||
            n_tokens > 0x7fffffffll / k;
 }
 static bool ex_odd(const void *p, int32_t dtype) { return ((uintptr_t)p & (dtype == CG3D_DT_F32 ? 3 : 1)) != 0; }
 
-static uint64_t ex_magic(int32_t nv) { return nv > 1 ? ~0ull / (uint64_t)nv + 1 : 0; }      // (nv > 1 does not divide 2^64 - 1 + 1 evenly unless a power of two: then exact too)
+static uint64_t ex_magic(int32_t nv) { return nv > 1 ? ~0ull / (uint64_t)nv + 1 : 0; }      // ceil(2^64 / nv)
 static int64_t ex_grid(int64_t nb) { return nb < (1 << 22) ? nb : (1 << 22); }      // (fewer than 2^32 threads; the kernels loop)
 
 #define EX_DISPATCH(LAUNCH)                                                                                        \

@@ -19,6 +19,7 @@ from .._lib import CG3DError, ptr
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.int8: 3}       # CG3D_DT_*
 FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 MAX_EXPERTS = 1024
+MAX_COLUMNS = 1 << 30
 
 
 def on_device(t):
@@ -97,8 +98,8 @@ def expert_plan(experts, n_experts):
 def _check_rows(who, x, n, plan, what):
     if not isinstance(plan, ExpertPlan):
         raise CG3DError("%s: plan must come from expert_plan" % who)
-    if not (isinstance(x, torch.Tensor) and x.dtype in FLOATS and x.dim() == 2 and x.shape[0] == n and x.shape[1] >= 1):
-        raise CG3DError("%s: %s must be [%d, C] float32, bfloat16 or float16, got %s" % (
+    if not (isinstance(x, torch.Tensor) and x.dtype in FLOATS and x.dim() == 2 and x.shape[0] == n and 1 <= x.shape[1] <= MAX_COLUMNS):
+        raise CG3DError("%s: %s must be [%d, C] float32, bfloat16 or float16 with C in 1 .. 2^30, got %s" % (
             who, what, n, (x.dtype, tuple(x.shape)) if isinstance(x, torch.Tensor) else type(x)))
     if x.device != plan.device:
         raise CG3DError("%s: %s is on %s, the plan on %s" % (who, what, x.device, plan.device))

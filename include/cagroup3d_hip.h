@@ -587,7 +587,7 @@ int cg3d_adamw_step(const int64_t *table, const int32_t *pid, int64_t nrows, con
  *     pairs   int32 [P]              the pair of each row; behind offsets[n_experts] ~p of a pair p without a row, each once
  *     pos     int32 [P]              the row of each pair; negative: none (~pos is one of the rows behind the last, which the
  *                                    passes that write rows clear)
- *   1 <= n_experts <= 1024, k >= 1, P < 2^31; ws: cg3d_expert_plan_ws_bytes bytes, 16-byte aligned (may be NULL where
+ *   1 <= n_experts <= 1024, k >= 1, P < 2^31, 1 <= c <= 2^30; ws: cg3d_expert_plan_ws_bytes bytes, 16-byte aligned (may be NULL where
  *   that is 0).
  * Element types `dtype` of rows, `wtype` of weights: CG3D_DT_F32 / _BF16 / _F16.  Rows are contiguous [*, c] of any width.
  *   gather:       out[j] = x[rows[j]]           (out [P, c]; rows without a pair are zeros)

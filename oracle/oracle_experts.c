@@ -83,7 +83,7 @@ int cg3d_expert_plan(const void *experts, int32_t wide, int64_t n_tokens, int32_
     return CG3D_OK;
 }
 static int bad(int32_t dt, int32_t wt, int64_t n, int32_t k, int32_t c) {
-    return !fl(dt) || !fl(wt) || n < 0 || k < 1 || c < 1 || n > 0x7fffffffll / k;
+    return !fl(dt) || !fl(wt) || n < 0 || k < 1 || c < 1 || c > (1 << 30) || n > 0x7fffffffll / k;
 }
 int cg3d_expert_gather(const void *x, int32_t dtype, const int32_t *rows, int64_t n_tokens, int32_t k, int32_t c, void *out,
                        cg3d_stream_t stream) {

@@ -188,6 +188,23 @@ def test_entry_points_refuse(oracle):
         assert h.raw("cg3d_expert_plan")(i.data_ptr(), 0, 100000, 2, 18, i.data_ptr(), i.data_ptr(), i.data_ptr(), i.data_ptr(), None, None) == -1
 
 
+def test_too_many_columns_are_refused(oracle):
+    """A number of columns that the C-ABI's 32 bits do not hold (no memory behind the tensors' one element)."""
+    p = torch.zeros(64).data_ptr()
+    for lib in (oracle, _lib.bind(_lib.HIP_LIB_PATH)):
+        assert lib.raw("cg3d_expert_gather")(p, 0, p, 4, 2, (1 << 30) + 1, p, None) == -1
+        assert lib.raw("cg3d_expert_combine")(p, 0, p, None, 0, 4, 2, (1 << 30) + 1, p, 0, None) == -1
+        assert lib.raw("cg3d_expert_combine_bwd")(p, None, 0, p, None, 0, 4, 2, (1 << 30) + 1, p, None, None) == -1
+    with _lib.use_library(oracle):
+        plan = expert_plan(torch.zeros(2, 1, dtype=torch.int32), 1)
+        for wide in ((1 << 30) + 1, (1 << 32) + 8):
+            x = torch.zeros(1).expand(2, wide)
+            with pytest.raises(_lib.CG3DError):
+                expert_gather(x, plan)
+            with pytest.raises(_lib.CG3DError):
+                expert_combine(x, plan)
+
+
 def test_no_cpu_fallback():
     with _lib.use_library(_lib.bind(_lib.HIP_LIB_PATH)):
         with pytest.raises(_lib.CG3DError):
