@@ -14,10 +14,7 @@
 #include "cg3d_common.h"
 
 #define EX_MAX_EXPERTS 1024
-#define EX_THREADS 512               // of the plan's workgroups
-#define EX_STEPS 4                   // ids of a lane in flight
-#define EX_CHUNK (EX_THREADS * EX_STEPS)
-#define EX_BLOCKS 256
+#define EX_STEPS 2                   // ids of a lane in flight
 
 // ---------------------------------------------------------------- element types
 struct ex_bf16 {
@@ -98,7 +95,7 @@ static __device__ __forceinline__ void ex_block_scan(int32_t *tot, int n, int32_
 }
 
 // A chunk of blockDim * EX_STEPS pairs belongs to a workgroup: wave w takes the EX_STEPS * 64 pairs behind w of those, all its ids in
-// flight at once.  Chunks of one workgroup follow each other, so that any number of pairs needs at most EX_BLOCKS workgroups.
+// flight at once.  Chunks of one workgroup follow each other, so that any number of pairs needs at most ex_shape's workgroups.
 // ex_chunk_ranks: counts of the keys in the wave's row h[0 .. E] of LDS and each pair's rank in the wave.
 static __device__ __forceinline__ void ex_chunk_keys(const void *ids, int32_t wide, int64_t p, int64_t n, int E, int (&key)[EX_STEPS]) {
 #pragma unroll
@@ -131,26 +128,26 @@ static __device__ __forceinline__ void ex_chunk_count(const int (&key)[EX_STEPS]
 }
 
 // more than one workgroup: counts [nblk][W4] of the workgroups' pairs go through memory (W4: E + 1 up to a multiple of 4)
-__global__ __launch_bounds__(EX_THREADS) void k_expert_plan_count(const void *__restrict__ ids, int32_t wide, int64_t n, int32_t E,
+__global__ __launch_bounds__(1024) void k_expert_plan_count(const void *__restrict__ ids, int32_t wide, int64_t n, int32_t E,
                                                                   int32_t bits, int32_t chunks, int32_t *__restrict__ counts) {
     extern __shared__ int32_t ex_sm[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, W4 = (E + 4) & ~3;
-    const int64_t p = (int64_t)blockIdx.x * chunks * EX_CHUNK + wave * (EX_STEPS * 64) + lane;
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, wave = tid >> 6, W4 = (E + 4) & ~3;
+    const int64_t chunk = (int64_t)nt * EX_STEPS, p = blockIdx.x * chunks * chunk + wave * (EX_STEPS * 64) + lane;
     int key[EX_STEPS];
     ex_chunk_keys(ids, wide, p, n, E, key);
-    for (int i = tid; i < W4; i += EX_THREADS) ex_sm[i] = 0;
+    for (int i = tid; i < W4; i += nt) ex_sm[i] = 0;
     __syncthreads();
     ex_chunk_count(key, p, n, bits, lane, ex_sm);
     for (int c = 1; c < chunks; c++) {
-        ex_chunk_keys(ids, wide, p + (int64_t)c * EX_CHUNK, n, E, key);
-        ex_chunk_count(key, p + (int64_t)c * EX_CHUNK, n, bits, lane, ex_sm);
+        ex_chunk_keys(ids, wide, p + c * chunk, n, E, key);
+        ex_chunk_count(key, p + c * chunk, n, bits, lane, ex_sm);
     }
     __syncthreads();
-    for (int i = tid; i < W4; i += EX_THREADS) counts[(int64_t)blockIdx.x * W4 + i] = ex_sm[i];
+    for (int i = tid; i < W4; i += nt) counts[(int64_t)blockIdx.x * W4 + i] = ex_sm[i];
 }
-// The first row of each key for this workgroup, from the counts of all of them (the workgroup adds the at most EX_BLOCKS rows up
+// The first row of each key for this workgroup, from the counts of all of them (the workgroup adds their rows up
 // itself, four columns of a thread at a time), or from its own pairs when it is the only one; then chunk by chunk the rows of the pairs.
-__global__ __launch_bounds__(EX_THREADS) void k_expert_plan_place(const void *__restrict__ ids, int32_t wide, int64_t n, int32_t k,
+__global__ __launch_bounds__(1024) void k_expert_plan_place(const void *__restrict__ ids, int32_t wide, int64_t n, int32_t k,
                                                                   int32_t E, int32_t bits, int32_t chunks, const int32_t *__restrict__ counts,
                                                                   int32_t *__restrict__ offsets, int32_t *__restrict__ rows,
                                                                   int32_t *__restrict__ pairs, int32_t *__restrict__ pos) {
@@ -230,13 +227,29 @@ __global__ __launch_bounds__(EX_THREADS) void k_expert_plan_place(const void *__
     }
 }
 
-// chunks of a workgroup and workgroups for n pairs
-static int32_t ex_chunks(int64_t n) { return n <= 2 * EX_CHUNK ? (n <= EX_CHUNK ? 1 : 2) : (int32_t)cg3d_divup(cg3d_divup(n, EX_CHUNK), EX_BLOCKS); }
-static int64_t ex_blocks(int64_t n) { const int64_t b = cg3d_divup(n, (int64_t)ex_chunks(n) * EX_CHUNK); return b > 1 ? b : 1; }
+// Threads, chunks of a workgroup and workgroups for n pairs.  Up to 4096 pairs one workgroup of up to 1024 threads does it, in one
+// launch (1200 / 2000 pairs of 18 experts: 7.2 / 7.8 us, with two workgroups of 512 8.9 / 9.5).  Above, 512 threads and at most 512
+// workgroups (164 214 pairs of 18 experts, both kernels: 10.6 us; 12.0 with 1024 and at most 256, 12.3 with twice the ids of a lane), but
+// every workgroup adds up the counts of all of them, so that many experts in many workgroups want fewer and larger ones (311 546 pairs
+// of 128 experts 16.5 against 21.8 us, of 1024 experts 30 / 72; about the same where workgroups x experts = 20 000).
+struct ex_shape {
+    int32_t threads, chunks;
+    int64_t blocks;
+    ex_shape(int64_t n, int32_t n_experts) {
+        const int64_t small = cg3d_divup(n, 512 * EX_STEPS) < 512 ? cg3d_divup(n, 512 * EX_STEPS) : 512;
+        const bool one = n <= 2 * 1024 * EX_STEPS, wide = one || (n_experts > 64 && small * n_experts > 20480);
+        threads = wide ? 1024 : 512;
+        const int64_t least = n > n_experts / 4 ? n : n_experts / 4;              // (2 pairs of 1024 experts: 15.6 us with 64 threads, 9.6 with 256)
+        if (least < threads) threads = least <= 64 ? 64 : (int32_t)((least + 63) & ~63ll);
+        const int64_t all = cg3d_divup(n, threads * EX_STEPS);
+        chunks = one ? (all > 1 ? 2 : 1) : (int32_t)cg3d_divup(all, wide ? 256 : 512);
+        blocks = one ? 1 : cg3d_divup(all, chunks);
+    }
+};
 
 extern "C" int64_t cg3d_expert_plan_ws_bytes(int64_t n_tokens, int32_t k, int32_t n_experts) {
     if (n_tokens < 0 || k < 1 || n_experts < 1 || n_experts > EX_MAX_EXPERTS || n_tokens > 0x7fffffffll / k) return CG3D_ERR_ARG;
-    const int64_t nblk = ex_blocks(n_tokens * k);
+    const int64_t nblk = ex_shape(n_tokens * k, n_experts).blocks;
     return nblk == 1 ? 0 : nblk * ((n_experts + 4) & ~3) * (int64_t)sizeof(int32_t);
 }
 extern "C" int cg3d_expert_plan(const void *experts, int32_t wide, int64_t n_tokens, int32_t k, int32_t n_experts, int32_t *offsets,
@@ -246,17 +259,19 @@ extern "C" int cg3d_expert_plan(const void *experts, int32_t wide, int64_t n_tok
     const int64_t n = n_tokens * k;
     if (n > 0 && (!experts || !rows || !pairs || !pos || ((uintptr_t)experts & (wide ? 7 : 3)))) return CG3D_ERR_ARG;
     if (need > 0 && (!ws || ((uintptr_t)ws & 15))) return CG3D_ERR_ARG;
-    const int64_t nblk = ex_blocks(n);
-    const int32_t chunks = ex_chunks(n);
+    const ex_shape shape(n, n_experts);
+    const int64_t nblk = shape.blocks;
+    const int32_t chunks = shape.chunks, nt = shape.threads;
     int bits = 1;
     while ((n_experts >> bits) != 0) bits++;
     hipStream_t s = cg3d_hs(stream);
     const int W4 = (n_experts + 4) & ~3;
-    const int nt = n >= EX_THREADS ? EX_THREADS : n <= 64 ? 64 : (int)((n + 63) & ~63ll);
-    const int lds = ((nt / 64 + 2) * W4 + nt / 64) * (int)sizeof(int32_t);          // (at most 41 KB)
+    const int lds = ((nt / 64 + 2) * W4 + nt / 64) * (int)sizeof(int32_t);          // (at most 72.4 KB)
+    if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(&k_expert_plan_place), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+        return CG3D_ERR_LAUNCH;
     int32_t *counts = need > 0 ? reinterpret_cast<int32_t *>(ws) : nullptr;
     if (counts) {
-        hipLaunchKernelGGL(k_expert_plan_count, dim3((unsigned)nblk), dim3(EX_THREADS), W4 * sizeof(int32_t), s, experts, wide, n,
+        hipLaunchKernelGGL(k_expert_plan_count, dim3((unsigned)nblk), dim3(nt), W4 * sizeof(int32_t), s, experts, wide, n,
                            n_experts, bits, chunks, counts);
         CG3D_CHECK_LAUNCH();
     }

@@ -223,6 +223,13 @@ def test_hip_plan(hip, t, k, n_experts, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n_experts", [1, 64, 65, 300, 1024])
+@pytest.mark.parametrize("t", [2, 63, 64, 65, 257, 1023, 1025, 2048, 2049, 4095, 4096, 4097, 21505, 600001])
+def test_hip_plan_at_the_borders_of_its_launches(hip, t, n_experts):
+    check_plan(routing(t, 1, n_experts, "dropped", 8, torch.int32).cuda(), n_experts)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("t,k,n_experts,c,kind", SMALL + [(5000, 2, 18, 64, "uniform"), (3001, 8, 61, 251, "dropped"), (900, 3, 4, 1030, "dropped"),
                                                           (20011, 2, 18, 128, "uniform")])
 @pytest.mark.parametrize("dtype,wdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.float16),
