@@ -282,7 +282,7 @@ template <typename T> static __device__ __forceinline__ void i8_put_levels(int8_
     }
 }
 // L lanes (a power of two, at most a wave) own one row of at most L * KEEP pieces and hold it in registers: as few lanes as KEEP
-// pieces of each allow (with 64 lanes and one piece 100 000 x 512 bf16 took 39.5 us, with 16 and four 28)
+// pieces of each allow (with 64 lanes and one piece 100 000 x 512 bf16 took 39.5 us, with 16 and four 26.7: 5.8 TB/s, the memory's)
 template <typename T>
 __global__ __launch_bounds__(256) void k_i8_rows(const T *__restrict__ x, int64_t n, int32_t cin, int64_t pitch, int32_t lshift,
                                                  int8_t *__restrict__ q, float *__restrict__ scale) {
@@ -309,7 +309,10 @@ __global__ __launch_bounds__(256) void k_i8_rows(const T *__restrict__ x, int64_
         for (int64_t a = (int64_t)KEEP * L * N + lane; a < pitch; a += L) dst[a] = 0;
     }
 }
-// longer rows, one to a workgroup of B threads; rows of more than B * KEEP pieces are read again for their levels
+// Longer rows, one to a workgroup of B threads; rows of more than B * KEEP pieces are read again for their levels.  Bound by memory
+// and, with a barrier between a row's reads and its writes, by the rows that a CU has under way: B and KEEP by the row's length, and for
+// 16-bit rows by how many there are (4000 rows of 10 976 fp32 49.9 us with 1024 threads of 4 pieces, 37.9 with 512 of 8 = 5.8 TB/s; 512 rows
+// of 43 904: fp32 26.1 us with 1024 threads = 4.3 TB/s, 30.6 with 512, bf16 17.4 and 15.8; 100 rows 6.9 and 7.9).
 template <typename T, int B, int KEEP>
 __global__ __launch_bounds__(B) void k_i8_long_rows(const T *__restrict__ x, int64_t n, int32_t cin, int64_t pitch, int8_t *__restrict__ q,
                                                     float *__restrict__ scale) {
@@ -360,8 +363,15 @@ static void i8_launch_rows(const T *x, int64_t n, int32_t cin, int64_t pitch, in
     else if (cin <= 2048) hipLaunchKernelGGL((k_i8_long_rows<T, 128, 2 * F>), gb, dim3(128), 0, s, x, n, cin, pitch, q, scale);
     else if (cin <= 4096) hipLaunchKernelGGL((k_i8_long_rows<T, 256, 2 * F>), gb, dim3(256), 0, s, x, n, cin, pitch, q, scale);
     else if (cin <= 8192) hipLaunchKernelGGL((k_i8_long_rows<T, 512, 2 * F>), gb, dim3(512), 0, s, x, n, cin, pitch, q, scale);
-    else if (cin <= 16384) hipLaunchKernelGGL((k_i8_long_rows<T, 1024, 2 * F>), gb, dim3(1024), 0, s, x, n, cin, pitch, q, scale);
-    else hipLaunchKernelGGL((k_i8_long_rows<T, 1024, 6 * F>), gb, dim3(1024), 0, s, x, n, cin, pitch, q, scale);
+    else if (cin <= 16384) hipLaunchKernelGGL((k_i8_long_rows<T, 512, 4 * F>), gb, dim3(512), 0, s, x, n, cin, pitch, q, scale);
+    else {
+        if constexpr (F == 1)
+            if (n >= 512 && cin <= 512 * 12 * N) {
+                hipLaunchKernelGGL((k_i8_long_rows<T, 512, 12>), gb, dim3(512), 0, s, x, n, cin, pitch, q, scale);
+                return;
+            }
+        hipLaunchKernelGGL((k_i8_long_rows<T, 1024, 6 * F>), gb, dim3(1024), 0, s, x, n, cin, pitch, q, scale);
+    }
 }
 extern "C" int cg3d_int8_quantize_rows(const void *x, int32_t dtype, int64_t n, int32_t cin, int64_t pitch, int8_t *q, float *scale,
                                        cg3d_stream_t stream) {
