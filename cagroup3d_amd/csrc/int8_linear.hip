@@ -530,19 +530,24 @@ static __device__ __forceinline__ int i8_place(int r, int p) { return r * 64 + (
 // neighbouring lanes neighbouring pieces (a chunk of a row is 4, 8 or 16 lanes, so a load of the wave is whole lines), finds their
 // maxima over those lanes, and leaves their levels in LDS in the order of the MFMA's operand.  A level's divisions are done once for a
 // row: of the NI rows that a lane has pieces of, lane l sees to row l % NI and its neighbours get the factor from it.  Then wave
-// (wm, wn) multiplies RG of the 4 row groups by panels wn, wn + RG, ... of the part blockIdx.y of the channels, the weights streaming
-// past from the caches, every fragment used RG times.  RG = 4 / 2 / 1 for at least 4 / 2 / 1 panels a part.
+// (wm, wn) multiplies RG of the 4 row groups by panels wn, wn + RG, ... of its part of the channels, the weights streaming past from the
+// caches, every fragment used RG times.  RG = 4 / 2 / 1 for at least 4 / 2 / 1 panels a part.  The first `whole` tiles are one workgroup
+// each, the panels of every other are shared out to `parts`.
+// Bound by memory where panels are few (155 773 x 64 fp32 -> 64: 14.7 us = 5.4 TB/s, a copy's rate); with many, by what a workgroup does one
+// after the other -- rows in, products, results out -- which the three others of its CU overlap only in part: 82 107 x 512 bf16 -> 512
+// 48 us = 3.5 TB/s and 0.9 POP/s (31 us to read and write, 18 us to multiply), 131 072 rows 3.9 TB/s.
 template <typename T, int RG, int KEEP>                  // KEEP: chunks of a row held in registers; longer rows are read again, from the caches
-__global__ __launch_bounds__(256, RG == 4 || KEEP * sizeof(T) > 8 ? 4 : RG == 2 ? 5 : 6) void k_i8_fused(i8_args a, const T *__restrict__ x) {
+__global__ __launch_bounds__(256, RG == 4 || KEEP * sizeof(T) > 8 ? 4 : RG == 2 ? 5 : 6) void k_i8_fused(i8_args a, const T *__restrict__ x, int32_t whole, int32_t parts) {
     extern __shared__ __attribute__((aligned(16))) uint8_t i8_sm[];
     constexpr int NI = sizeof(T), LPR = 4 * NI, RPI = 64 / LPR, N = i8_els<T>;     // lanes of a row's chunk, rows of a load, elements of a piece
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int panels = (a.cout + 63) >> 6, chunks = (a.cin + 63) >> 6;
-    const int p_lo = (int)((int64_t)panels * blockIdx.y / gridDim.y), p_hi = (int)((int64_t)panels * (blockIdx.y + 1) / gridDim.y);
+    const int late = (int)blockIdx.x - whole, tile = late < 0 ? blockIdx.x : whole + late / parts, part = late < 0 ? 0 : late % parts;
+    const int of = late < 0 ? 1 : parts, p_lo = panels * part / of, p_hi = panels * (part + 1) / of;
     float *const scales = reinterpret_cast<float *>(i8_sm + chunks * 4096);        // [64], behind [4 groups][chunks][1 KB]
     int e, rows;
     int64_t row0;
-    if (!i8_tile<64>(a, blockIdx.x, e, row0, rows)) return;                        // (the whole workgroup)
+    if (!i8_tile<64>(a, tile, e, row0, rows)) return;                              // (the whole workgroup)
     const bool live = e < a.n_experts;
     if (live && wave * 16 < rows) {
         const int rl = lane / LPR, k0 = (lane % LPR) * N;
@@ -1026,11 +1031,21 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
         // enough workgroups for the chip: the panels of a row tile are shared out where there are fewer than 384 tiles, though each part
         // quantises the rows for itself (512 -> 512, 10 000 rows: 20.6 / 16.4 / 18.3 / 16.9 / 25.4 us at 128 / 256 / 384 / 512 / 1024
         // wanted, 20 000 rows 24.7 / 24.5 / 22.0 / 21.9 / 27.9; 512 -> 2048, 5000 rows 33.4 / 22.7 / 23.9 / 26.8 / 26.0)
-        const int64_t want = cg3d_divup(384, p.tiles);
-        const int32_t parts = (int32_t)(want < panels ? want : panels);
+        int64_t whole = 0, parts = cg3d_divup(384, p.tiles);
+        parts = parts < panels ? parts : panels;
         const int32_t each = (int32_t)cg3d_divup(panels, parts);
+        // and those of the last few tiles behind whole rounds of the chip (four workgroups a CU), four panels or more to a part: 512 -> 512,
+        // 73 728 rows (128 tiles of 1152) 49.0 -> 44.9 us, 82 107 rows (259 of 1283) 52.3 -> 50.9; 256 -> 2048, 82 107 rows 118.9 -> 105.4; with
+        // 512 tiles left it loses (98 304 rows 55.4 -> 58.3)
+        const int64_t late = p.tiles % 1024;
+        if (p.tiles > 1024 && late > 0 && late <= 384 && panels >= 8) {
+            whole = p.tiles - late;
+            parts = cg3d_divup(768, late);
+            parts = parts < panels / 4 ? parts : panels / 4;
+        }
+        const int64_t blocks = whole + (p.tiles - whole) * parts;
         const int lds = (int)i8_chunks(cin) * 4096 + 256;           // (at most 32.25 KB)
-#define I8_F(T, RG, KEEP) hipLaunchKernelGGL((k_i8_fused<T, RG, KEEP>), dim3((unsigned)p.tiles, (unsigned)parts), dim3(256), lds, s, a, reinterpret_cast<const T *>(x))
+#define I8_F(T, RG, KEEP) hipLaunchKernelGGL((k_i8_fused<T, RG, KEEP>), dim3((unsigned)blocks), dim3(256), lds, s, a, reinterpret_cast<const T *>(x), (int32_t)whole, (int32_t)parts)
 #define I8_FK(T, RG) do { if (chunks <= 1) I8_F(T, RG, 1); else if (chunks <= 2) I8_F(T, RG, 2); else I8_F(T, RG, (sizeof(T) == 4 ? 4 : 8)); } while (0)
 #define I8_FC(T) do { if (each >= 4) I8_FK(T, 4); else if (each >= 2) I8_FK(T, 2); else I8_FK(T, 1); } while (0)
         const int64_t chunks = i8_chunks(cin);

@@ -315,7 +315,7 @@ def test_hip_quantize_rows(hip, n, cin, dtype):
 @pytest.mark.parametrize("n,cin,cout", [
     (20, 500, 70), (50, 1000, 70), (50, 1900, 40), (20, 4000, 70), (20, 6000, 70),                          # few rows, by the chunks a wave holds
     (25000, 60, 60), (25000, 60, 130), (25000, 120, 130), (25000, 120, 250), (25000, 300, 250), (25000, 300, 60), (25000, 300, 130),
-    (1700, 300, 250),                                                                                       # one pass: panels of a wave, chunks held
+    (1700, 300, 250), (70000, 40, 520), (66500, 130, 1100),                                                                                       # one pass: panels of a wave, chunks held
     (3000, 4100, 130), (3000, 700, 700)])                                                                   # tiles, in parts and whole
 @pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (F16, F16), (I8, F32)])
 def test_hip_each_kernel_of_the_choice(hip, n, cin, cout, dtype, out):
