@@ -55,6 +55,8 @@ static __device__ __forceinline__ float ex_weight(const void *w, int32_t wtype, 
 // ---------------------------------------------------------------- plan
 // A wave takes 64 consecutive pairs at a time.  Lanes with equal keys find each other by one ballot per bit of the key; a lane's
 // rank among them is the number of earlier lanes, the wave's running count of the key is kept in LDS (only this wave touches it).
+// Bound by the chain ids - counts - offsets - rows, each a trip to memory, not by its 20 bytes a pair: 82 107 x 2 ids of 18 experts count
+// 3.3 + place 6.7 us, 155 773 x 2 4.6 + 8.5 us; one token 3 us, a launch.
 static __device__ __forceinline__ int ex_key(const void *ids, int32_t wide, int64_t p, int E) {
     if (wide) {
         const int64_t v = reinterpret_cast<const int64_t *>(ids)[p];
@@ -285,6 +287,8 @@ extern "C" int cg3d_expert_plan(const void *experts, int32_t wide, int64_t n_tok
 // A thread owns V elements (16 bytes) of one token's row; the last vector of a row whose width V does not divide is moved back to
 // end with the row (its first elements are then computed twice, with the same result).  Rows shorter than a vector: V = 1.  The
 // combination takes a token's slots EX_SLOTS at a time: their rows are looked up, and then read, together.
+// Bound by memory: 155 773 x 2 rows of 256 bytes gather 28 us (120 MB, 4.3 TB/s), combine 24.6 us (4.9 TB/s), its gradient 43.5 us (201 MB, 4.6
+// TB/s); 20 011 x 8 rows of 502 bytes 24.8, 22.4 and 41.3 us (90, 90 and 171 MB).  A copy of 512 MB reaches 5.4 TB/s.
 #define EX_SLOTS 4
 // i / nv by a multiplication: magic = ceil(2^64 / nv), exact while i * nv < 2^64 (i counts 16-byte pieces of memory)
 static __device__ __forceinline__ int64_t ex_div(int64_t i, int32_t nv, uint64_t magic) {

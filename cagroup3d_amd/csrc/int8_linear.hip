@@ -184,7 +184,8 @@ static __device__ __forceinline__ i8_lev<T> i8_levels(const i8_level &lev, bool 
 }
 
 // ---------------------------------------------------------------- weights (once per model)
-// w [E][cin][cout]: a thread of 16 to a channel, reads along the contraction are rows of the matrix
+// w [E][cin][cout]: a thread of 16 to a channel, reads along the contraction are rows of the matrix (18 x 1024 x 1024 fp32: 13 us,
+// 5.7 TB/s; the packing 27 us)
 template <typename T>
 __global__ __launch_bounds__(1024) void k_i8_weight_scale(const T *__restrict__ w, int32_t cin, int32_t cout, float *__restrict__ scale,
                                                           uint32_t *__restrict__ top) {
@@ -663,7 +664,10 @@ __global__ __launch_bounds__(256, RG == 4 || KEEP * sizeof(T) > 8 ? 4 : RG == 2 
 // Few rows: a workgroup of 8 waves owns 16 rows x 32 channels (tiles nb of a pair) and its waves share the contraction (chunk c belongs
 // to wave c % 8), so that every weight is read once, by loads that are all under way before the rows are even looked at.  Rows in
 // floats that fit (CHUNKS chunks of a wave) are quantised here, in the operand's own layout -- each workgroup finds the rows' maxima for
-// itself, through LDS; the waves' sums are joined there too.  grid: (16-row tiles, pairs of tiles).
+// itself, through LDS; the waves' sums are joined there too.  grid: (16-row tiles, pairs of tiles).  KEEP: chunks of a wave held at once;
+// registers for no more than there are let up to three workgroups onto a CU (8 experts of 640 -> 256, 1000 rows: 24.4 us with 8, 10.9 with 2).
+// Bound by the weights' way from memory, and for small ones by a launch and two trips to memory: 1 x 4096 bf16 -> 4096 8.5 us = 2.0 TB/s
+// of weights, 1003 x 200 fp16 -> 77 5.3 us, 8 rows of 64 experts 512 -> 512 4.8 us.
 template <typename T> struct i8_few { static constexpr int CHUNKS = sizeof(T) == 4 ? 4 : 8; };
 template <typename T, int KEEP>
 __global__ __launch_bounds__(512, KEEP == 1 || (KEEP == 2 && !__is_same(T, float) && !__is_same(T, i8_f16)) ? 6 : KEEP * sizeof(T) <= 8 ? 4 : 2) void k_i8_few(i8_args a, const T *__restrict__ x, int64_t pitch) {
@@ -757,6 +761,9 @@ __global__ __launch_bounds__(512, KEEP == 1 || (KEEP == 2 && !__is_same(T, float
 // `part` (one i32x4 of a lane after the other, as the tile holds them) and k_i8_join adds them up.
 // The direct loads and their waits are written out, since the compiler waits for ALL of them before any read of LDS: a wave has
 // issued the NL loads of each chunk in order, so vmcnt(NL) leaves only the newest chunk's in flight.
+// Bound by the matrix unit: 4096 x 4096 x 4096 in 64 us with the rows' quantisation left out = 2.1 POP/s, as the library's product of
+// these sizes (68 us, 2.0 POP/s).  256 x 256 with 8 waves and 128 x 64 of it a wave reads LDS least for what registers hold; 128 x 128 a
+// wave with 4 waves does not fit them (354 us).
 // 16 bytes of each lane to lds + 16 lane.  (M0 holds the address; the compiler uses it for nothing in a kernel without other such loads.)
 static __device__ __forceinline__ void i8_dma(const void *src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"((uint64_t)(uintptr_t)src), "s"(lds) : "memory");
@@ -863,7 +870,7 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void k_i8_tile(i8_args a, const in
     }
 }
 // The sums of a tile's ranges of chunks: a workgroup owns 16 rows x 64 channels, its 8 waves share the ranges (one wave for all of
-// them: 64 waves on the whole chip for 512 x 128 results, 18.7 us at 85 ranges).
+// them: 64 waves on the whole chip for 512 x 128 results, 18.7 us at 85 ranges; now 5.2 us at 64 = 3.3 TB/s of sums).
 template <int RG, int WR, int WC>
 __global__ __launch_bounds__(512) void k_i8_join(i8_args a, int32_t ny, int32_t total, int32_t splits, const i32x4 *__restrict__ part) {
     constexpr int NW = WR * WC, BM = WR * RG * 16;
