@@ -371,6 +371,10 @@ static void i8_launch_rows(const T *x, int64_t n, int32_t cin, int64_t pitch, in
                 hipLaunchKernelGGL((k_i8_long_rows<T, 512, 12>), gb, dim3(512), 0, s, x, n, cin, pitch, q, scale);
                 return;
             }
+        if (cin <= 32768) {                                          // (two workgroups fit a CU: 3000 x 20 000 fp32 71.9 -> 67.5 us)
+            hipLaunchKernelGGL((k_i8_long_rows<T, 1024, 4 * F>), gb, dim3(1024), 0, s, x, n, cin, pitch, q, scale);
+            return;
+        }
         hipLaunchKernelGGL((k_i8_long_rows<T, 1024, 6 * F>), gb, dim3(1024), 0, s, x, n, cin, pitch, q, scale);
     }
 }

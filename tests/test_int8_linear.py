@@ -330,7 +330,7 @@ def test_hip_grouped_long_rows(hip, t, k, experts, cin, cout, dtype, out, gather
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,cin", [(70, 257), (70, 1000), (30, 2047), (30, 4095), (20, 8193), (20, 16384), (20, 16385), (600, 17001), (600, 49152), (520, 49153)])
+@pytest.mark.parametrize("n,cin", [(70, 257), (70, 1000), (30, 2047), (30, 4095), (20, 8193), (20, 16384), (20, 16385), (600, 17001), (20, 32768), (20, 32769), (600, 49152), (520, 49153)])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_hip_quantize_long_rows(hip, n, cin, dtype):
     x = make(n, cin, 1, dtype, 14)[0].cuda()
