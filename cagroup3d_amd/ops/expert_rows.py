@@ -25,7 +25,7 @@ MAX_COLUMNS = 1 << 30
 def on_device(t):
     """The context a call on `t` is made in: the launches go to the current stream of t's device, also where another device is
     the current one."""
-    if t.is_cuda and t.device.index != torch.cuda.current_device():
+    if t.is_cuda and t.device.index != _lib._GET_DEVICE():
         return torch.cuda.device(t.device)
     return _HERE
 
@@ -126,6 +126,17 @@ def _combine(y, plan, w, out_dtype):
     return out
 
 
+def _once(backward):
+    """once_differentiable, whose bookkeeping (4 us a call) is for a backward pass that is itself recorded."""
+    recorded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
@@ -134,7 +145,7 @@ class _Gather(torch.autograd.Function):
         return _gather(x, plan)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         return None if dout is None else _combine(dout.contiguous(), ctx.plan, None, dout.dtype), None
 
@@ -149,7 +160,7 @@ class _Combine(torch.autograd.Function):
         return _combine(y, plan, w, out_dtype)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         if dout is None:
             return None, None, None, None
