@@ -930,6 +930,7 @@ struct i8_plan {
 static int64_t i8_pitch(int32_t cin) { return i8_chunks(cin) * 64; }
 static i8_plan i8_choose(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts, bool grouped, bool padded) {
     i8_plan p = {};
+    if (n_rows == 0) return p;                                       // (nothing is launched)
     const int64_t chunks = i8_chunks(cin), panels = i8_panels(cout);
     // (a list of rows has at most one tile that is not full, and only lists with rows have tiles: at most so many, and those of the rows
     // behind the last)

@@ -268,6 +268,15 @@ def test_entry_points_refuse(oracle):
             assert lib.raw("cg3d_int8_linear")(*{**good, **change}.values(), None) == -1, change
 
 
+@pytest.mark.parametrize("cin,cout", [(1, 1), (512, 512), (4096, 4096), (4096, 16384), (131071, 1 << 20)])
+@pytest.mark.parametrize("grouped_call", [0, 1])
+def test_no_rows_need_no_workspace(oracle, cin, cout, grouped_call):
+    """Any weights, no rows: nothing is launched, and the choice of a kernel has no sizes to divide by."""
+    for lib in (oracle, _lib.bind(_lib.HIP_LIB_PATH)):
+        for dtype in range(4):
+            assert lib.raw("cg3d_int8_linear_ws_bytes")(dtype, 0, cin, 0, cout, 3 if grouped_call else 1, grouped_call) == 0
+
+
 def test_no_cpu_fallback():
     with _lib.use_library(_lib.bind(_lib.HIP_LIB_PATH)):
         with pytest.raises(_lib.CG3DError):
