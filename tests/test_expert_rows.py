@@ -378,6 +378,26 @@ def test_hip_second_gradients_are_refused(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t,n_experts", [(3, 1024), (2000, 1024), (30000, 1024), (30000, 18)])
+def test_hip_plans_in_a_graph(hip, t, n_experts):
+    """Every shape of the plan's launches captured once and replayed with other ids, eager plans in between."""
+    fixed = routing(t, 2, n_experts, "uniform", 62, torch.int32).cuda()
+    expert_plan(fixed, n_experts)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = expert_plan(fixed, n_experts)
+    for seed in range(3):
+        ids = routing(t, 2, n_experts, "dropped", 63 + seed, torch.int32).cuda()
+        fixed.copy_(ids)
+        graph.replay()
+        want = expert_plan(ids, n_experts)
+        torch.cuda.synchronize()
+        for a, b in ((held.offsets, want.offsets), (held.rows, want.rows), (held.pairs, want.pairs), (held.pos, want.pos)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_hip_on_another_stream(hip):
     ids, x = routing(30000, 2, 18, "uniform", 30).cuda(), torch.randn(30000, 64, device="cuda")
     want = expert_gather(x, expert_plan(ids, 18))
