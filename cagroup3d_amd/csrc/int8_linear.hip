@@ -31,6 +31,7 @@ typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 #define I8_MAX_CIN 131071            // 2^14 * 131071 < 2^31: -128 * -128 included
 #define I8_MAX_EXPERTS 1024
 #define I8_FUSED_CIN 512
+#define I8_FUSED_LONG 832            // for many rows of 16 bits
 
 template <typename T, int V> struct __attribute__((packed, aligned(1))) i8_vec { T e[V]; };
 
@@ -531,7 +532,7 @@ static __device__ __forceinline__ void i8_scales(const i8_args &a, int64_t row0,
 // one piece of every row touch every bank once
 static __device__ __forceinline__ int i8_place(int r, int p) { return r * 64 + ((p ^ (r >> 2)) << 4); }
 
-// Rows of at most I8_FUSED_CIN columns: one pass over them.  A workgroup of 4 waves owns 64 rows; each wave brings 16 of them in,
+// Rows of at most I8_FUSED_CIN columns (many: I8_FUSED_LONG): one pass over them.  A workgroup of 4 waves owns 64 rows; each wave brings 16 of them in,
 // neighbouring lanes neighbouring pieces (a chunk of a row is 4, 8 or 16 lanes, so a load of the wave is whole lines), finds their
 // maxima over those lanes, and leaves their levels in LDS in the order of the MFMA's operand.  A level's divisions are done once for a
 // row: of the NI rows that a lane has pieces of, lane l sees to row l % NI and its neighbours get the factor from it.  Then wave
@@ -950,13 +951,17 @@ static i8_plan i8_choose(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows
         p.kind = i8_plan::FEW;
         p.tiles = tiles(16);
         p.rows8 = dtype != CG3D_DT_I8 && chunks > 8 * (dtype == CG3D_DT_F32 ? i8_few<float>::CHUNKS : i8_few<i8_bf16>::CHUNKS);
-    } else if (cin <= I8_FUSED_CIN) {
+    } else if (cin <= I8_FUSED_CIN || (cin <= I8_FUSED_LONG && n_rows >= 20000 && (dtype == CG3D_DT_BF16 || dtype == CG3D_DT_F16))) {
+        // (longer rows lose what quantising them in the product gains, to fewer workgroups on a CU: bf16, 30 000 rows 704 -> 128 20.7 us
+        // against 26.0 in two passes, 704 -> 512 33.4 / 36.6, 832 -> 512 38.1 / 39.9, 960 -> 512 42.0 / 42.9; 82 107 rows 576 -> 64 36.6 / 52.1,
+        // 960 -> 128 68.1 / 65.6; 10 000 rows 704 -> 512 25.3 / 22.3; fp32, 30 000 rows 704 -> 128 34.6 / 31.2)
         p.kind = i8_plan::FUSED;
         p.tiles = tiles(64);
     } else {
         p.kind = i8_plan::TILE;
         p.rows8 = dtype != CG3D_DT_I8 || padded;
-        p.big = tiles(256) * cg3d_divup(panels, 4) >= 200;           // (a round of 256 x 256 tiles nearly full)
+        // a round of 256 x 256 tiles nearly full; with one or two panels half of each is empty (82 107 x 576 -> 64 39.6 us against 22.8)
+        p.big = panels > 2 && tiles(256) * cg3d_divup(panels, 4) >= 200;
         p.ny = (int32_t)cg3d_divup(panels, p.big ? 4 : 2);
         p.tiles = tiles(p.big ? 256 : 128);
         const int64_t total = p.tiles * p.ny;
@@ -1056,7 +1061,7 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
             parts = parts < panels / 4 ? parts : panels / 4;
         }
         const int64_t blocks = whole + (p.tiles - whole) * parts;
-        const int lds = (int)i8_chunks(cin) * 4096 + 256;           // (at most 32.25 KB)
+        const int lds = (int)i8_chunks(cin) * 4096 + 256;           // (at most 52.25 KB)
 #define I8_F(T, RG, KEEP) hipLaunchKernelGGL((k_i8_fused<T, RG, KEEP>), dim3((unsigned)blocks), dim3(256), lds, s, a, reinterpret_cast<const T *>(x), (int32_t)whole, (int32_t)parts)
 #define I8_FK(T, RG) do { if (chunks <= 1) I8_F(T, RG, 1); else if (chunks <= 2) I8_F(T, RG, 2); else I8_F(T, RG, (sizeof(T) == 4 ? 4 : 8)); } while (0)
 #define I8_FC(T) do { if (each >= 4) I8_FK(T, 4); else if (each >= 2) I8_FK(T, 2); else I8_FK(T, 1); } while (0)

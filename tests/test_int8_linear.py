@@ -324,15 +324,15 @@ def test_hip_quantize_rows(hip, n, cin, dtype):
 @pytest.mark.parametrize("n,cin,cout", [
     (20, 500, 70), (50, 1000, 70), (50, 1900, 40), (20, 4000, 70), (20, 6000, 70),                          # few rows, by the chunks a wave holds
     (25000, 60, 60), (25000, 60, 130), (25000, 120, 130), (25000, 120, 250), (25000, 300, 250), (25000, 300, 60), (25000, 300, 130),
-    (1700, 300, 250), (70000, 40, 520), (66500, 130, 1100),                                                                                       # one pass: panels of a wave, chunks held
-    (3000, 4100, 130), (3000, 700, 700)])                                                                   # tiles, in parts and whole
+    (1700, 300, 250), (70000, 40, 520), (66500, 130, 1100), (21000, 700, 130), (20001, 832, 300),   # one pass: panels of a wave, chunks held
+    (3000, 4100, 130), (3000, 700, 700), (53000, 600, 70)])                                                                   # tiles, in parts and whole
 @pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (F16, F16), (I8, F32)])
 def test_hip_each_kernel_of_the_choice(hip, n, cin, cout, dtype, out):
     dense(n, cin, cout, dtype, out, True, 50, "cuda")
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("t,k,experts,cin,cout", [(1500, 2, 5, 4200, 130), (300, 2, 18, 1000, 200), (60, 2, 64, 1000, 520)])
+@pytest.mark.parametrize("t,k,experts,cin,cout", [(1500, 2, 5, 4200, 130), (300, 2, 18, 1000, 200), (60, 2, 64, 1000, 520), (12000, 2, 7, 600, 100)])
 @pytest.mark.parametrize("dtype,out,gather", [(F32, F32, True), (BF16, BF16, True), (I8, F32, False)])
 def test_hip_grouped_long_rows(hip, t, k, experts, cin, cout, dtype, out, gather):
     grouped(ids_of(t, k, experts, "dropped", 51), experts, cin, cout, dtype, out, 2, gather, 52, "cuda")
