@@ -138,7 +138,7 @@ def int8_linear(x, weight, bias=None, scale=None, out_dtype=None, plan=None, gat
             "int8_linear: bias must be floats [%d] (or [%d, %d] with a matrix for each expert) on %s", cout, n_experts, cout, dev)
         per_expert = int(bias.dim() == 2)
     _no_grad_for("int8_linear", x, bias, scale)
-    if bias is not None:
+    if bias is not None and not (bias.dtype is torch.float32 and bias.is_contiguous()):
         bias = bias.detach().to(torch.float32).contiguous()
     lib = _lib.get()
     x = x.contiguous()
