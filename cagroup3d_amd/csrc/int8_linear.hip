@@ -766,9 +766,10 @@ __global__ __launch_bounds__(512, KEEP == 1 || (KEEP == 2 && !__is_same(T, float
 // `part` (one i32x4 of a lane after the other, as the tile holds them) and k_i8_join adds them up.
 // The direct loads and their waits are written out, since the compiler waits for ALL of them before any read of LDS: a wave has
 // issued the NL loads of each chunk in order, so vmcnt(NL) leaves only the newest chunk's in flight.
-// Bound by the matrix unit: 4096 x 4096 x 4096 in 64 us with the rows' quantisation left out = 2.1 POP/s, as the library's product of
-// these sizes (68 us, 2.0 POP/s).  256 x 256 with 8 waves and 128 x 64 of it a wave reads LDS least for what registers hold; 128 x 128 a
-// wave with 4 waves does not fit them (354 us).
+// 4096 x 4096 x 4096, rows in 8 bits: 64 us = 2.1 POP/s, as the library's product of these sizes (68 us, 2.0 POP/s); the matrix unit is busy
+// 47 % of the cycles.  A chunk is 1024 cycles of matrix instructions on each SIMD, 96 KB of fragments from LDS and 32 KB into it, and what
+// raises the traffic costs time: 256 x 128 tiles with three buffers, two workgroups on a CU, 80 against 71 us in one run.  128 x 128 a wave
+// with 4 waves would read a third less but does not fit the registers (354 us).  Rows whose chunks lie together in memory: no difference.
 // 16 bytes of each lane to lds + 16 lane.  (M0 holds the address; the compiler uses it for nothing in a kernel without other such loads.)
 static __device__ __forceinline__ void i8_dma(const void *src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"((uint64_t)(uintptr_t)src), "s"(lds) : "memory");
