@@ -250,8 +250,8 @@ def run(state):
         return int8_linear(state["x"], state["handle"], state["bias"], scale=state.get("sx"), out_dtype=DTYPES[case["out"]])
     if case["kind"] == "experts":
         plan = expert_plan(state["ids"], case["experts"])
-        y = int8_linear(state["x"], state["handle"], state["bias"], plan=plan, gather=True, out_dtype=torch.float32)
-        return expert_combine(y, plan, state["gate"], out_dtype=state["x"].dtype)  # rounded once, as in the plain form
+        y = int8_linear(state["x"], state["handle"], state["bias"], plan=plan, gather=True)
+        return expert_combine(y, plan, state["gate"])
     plan = expert_plan(state["ids"], case["experts"])
     gathered = expert_gather(state["x"], plan)
     combined = expert_combine(state["y"], plan, state["w"])
