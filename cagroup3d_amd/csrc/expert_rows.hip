@@ -453,9 +453,9 @@ extern "C" int cg3d_expert_combine(const void *y, int32_t dtype, const int32_t *
 
 extern "C" int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, const int32_t *pairs, const void *w, int32_t wtype,
                                        int64_t n_tokens, int32_t k, int32_t c, void *dy, void *dw, cg3d_stream_t stream) {
-    if (ex_bad(dtype, wtype, n_tokens, k, c) || (!dy && !dw)) return CG3D_ERR_ARG;
-    if (n_tokens == 0) return CG3D_OK;
-    if (!dout || !pairs || (dw && (!y || !w)) || ex_odd(dout, dtype) || ex_odd(y, dtype) || ex_odd(dy, dtype) || ex_odd(w, wtype) || ex_odd(dw, wtype))
+    if (ex_bad(dtype, wtype, n_tokens, k, c)) return CG3D_ERR_ARG;
+    if (n_tokens == 0) return CG3D_OK;                               // (empty tensors have no address)
+    if ((!dy && !dw) || !dout || !pairs || (dw && (!y || !w)) || ex_odd(dout, dtype) || ex_odd(y, dtype) || ex_odd(dy, dtype) || ex_odd(w, wtype) || ex_odd(dw, wtype))
         return CG3D_ERR_ARG;
     hipStream_t s = cg3d_hs(stream);
 #define EX_LAUNCH(T, V)                                                                                            \

@@ -596,7 +596,8 @@ int cg3d_adamw_step(const int64_t *table, const int32_t *pid, int64_t nrows, con
  *                 zeros
  *   combine_bwd:  for row j of pair (t, s): dy[j] = w[t, s] * dout[t] (rows without a pair: zeros), dw[t, s] = <dout[t], y[j]>
  *                 (0 without a row);
- *                 dy or dw may be NULL (not both); y may be NULL without dw */
+ *                 dy or dw may be NULL (not both); y may be NULL without dw
+ *   n_tokens = 0: nothing is read or written, and no address is needed */
 #define CG3D_DT_F32 0
 #define CG3D_DT_BF16 1
 #define CG3D_DT_F16 2

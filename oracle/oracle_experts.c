@@ -118,9 +118,9 @@ int cg3d_expert_combine(const void *y, int32_t dtype, const int32_t *pos, const 
 int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, const int32_t *pairs, const void *w, int32_t wtype,
                             int64_t n_tokens, int32_t k, int32_t c, void *dy, void *dw, cg3d_stream_t stream) {
     (void)stream;
-    if (bad(dtype, wtype, n_tokens, k, c) || (!dy && !dw)) return CG3D_ERR_ARG;
+    if (bad(dtype, wtype, n_tokens, k, c)) return CG3D_ERR_ARG;
     if (n_tokens == 0) return CG3D_OK;
-    if (!dout || !pairs || (dw && (!y || !w)) || odd(dout, dtype) || odd(y, dtype) || odd(dy, dtype) || odd(w, wtype) || odd(dw, wtype))
+    if ((!dy && !dw) || !dout || !pairs || (dw && (!y || !w)) || odd(dout, dtype) || odd(y, dtype) || odd(dy, dtype) || odd(w, wtype) || odd(dw, wtype))
         return CG3D_ERR_ARG;
     const int64_t P = n_tokens * k;
     for (int64_t j = 0; j < P; j++) {

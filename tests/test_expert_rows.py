@@ -451,3 +451,33 @@ def test_hip_refusals(hip):
     for bad in (lambda: expert_gather(torch.zeros(4, 8), plan), lambda: expert_combine(torch.zeros(8, 8, device="cuda"), plan, torch.zeros(4, 2))):
         with pytest.raises(_lib.CG3DError):
             bad()
+
+
+def empty_batch(dev):
+    """No tokens: every gradient exists and is empty, whichever inputs ask for one, with and without weights."""
+    for k in (1, 3):
+        plan = expert_plan(torch.zeros(0, k, dtype=torch.int64, device=dev), 3)
+        for dtype, out in ((torch.float32, None), (torch.bfloat16, None), (torch.float32, torch.float16)):
+            for need_y, need_w in ((True, True), (True, False), (False, True)):
+                x = torch.zeros(0, 4, dtype=dtype, device=dev, requires_grad=True)
+                y = torch.zeros(0, 4, dtype=dtype, device=dev, requires_grad=need_y)
+                w = torch.zeros(0, k, device=dev, requires_grad=need_w)
+                (expert_gather(x, plan).sum() + expert_combine(y, plan, w, out).sum()).backward()
+                assert x.grad.shape == (0, 4) and (y.grad is not None) == need_y and (w.grad is not None) == need_w
+                assert not need_y or y.grad.shape == (0, 4) and y.grad.dtype == dtype
+                assert not need_w or w.grad.shape == (0, k)
+            y = torch.zeros(0, 4, dtype=dtype, device=dev, requires_grad=True)
+            expert_combine(y, plan, None, out).sum().backward()
+            assert y.grad.shape == (0, 4)
+
+
+def test_empty_batch_has_gradients(oracle):
+    with _lib.use_library(oracle):
+        empty_batch("cpu")
+    for lib in (oracle, _lib.bind(_lib.HIP_LIB_PATH)):           # no addresses behind empty tensors: nothing is launched
+        assert lib.raw("cg3d_expert_combine_bwd")(None, None, 0, None, None, 0, 0, 2, 8, None, None, None) == 0
+
+
+@pytest.mark.gpu
+def test_hip_empty_batch_has_gradients(hip):
+    empty_batch("cuda")
