@@ -6,11 +6,13 @@ matrices of their own -- what the class-aware head does with its voxels (ops/hea
     ...                                            # the experts' layers (me.grouped_conv, int8_linear(plan=plan), ...)
     out = expert_combine(rows, plan, weights)      # [T, C] = sum over the k slots of weights * rows
 
-Nothing is read back to the host: the calls can be captured into a graph.  No sum uses an atomic: results and gradients are the
+Nothing is read back to the host: the calls can be captured into a graph.  torch.jit.trace records gather and combination (the plan
+is made outside of it); there is no forward-mode derivative and no second one.  No sum uses an atomic: results and gradients are the
 same from run to run.  Rows behind the last (as many as there are dropped pairs) are zeros in every output of that shape."""
 import contextlib
 import functools
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -36,6 +38,21 @@ _HERE = contextlib.nullcontext()
 def need(ok, message, *args):
     if not ok:
         raise CG3DError(message % args)
+
+
+_TRACING = getattr(torch._C, "_is_tracing", None) or torch.jit.is_tracing
+_MODES = getattr(torch._C, "_len_torch_dispatch_stack", None) or (lambda: 0)
+
+
+def recorded():
+    """Whether torch has to see the call also without gradients: torch.jit.trace records it, forward-mode differentiation has its
+    tangents refused -- both where it goes through an autograd.Function.  (The kernels take addresses: of a call that goes to them
+    directly a trace holds nothing but an uninitialised output.)  A graph of torch's own operators cannot hold it at all."""
+    if _MODES():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        if get_proxy_mode() is not None:
+            raise CG3DError("the operators take the addresses of their inputs: a graph of torch's own operators (make_fx) cannot hold them")
+    return forward_ad._current_level >= 0 or _TRACING()
 
 
 class ExpertPlan:
@@ -74,6 +91,8 @@ def _plan_ws_words(lib, t, k, n_experts):
 def expert_plan(experts, n_experts):
     """experts int32 / int64 [T, k] (or [T]): the experts of each token; an id outside [0, n_experts) has no row.  A token may
     name an expert twice: it then has two rows.  Rows are in expert order, pairs of one expert in the order of (token, slot)."""
+    if recorded() and _TRACING():
+        raise CG3DError("expert_plan: a trace would keep the plan of the ids it was made with; make the plan outside the trace")
     if not (isinstance(experts, torch.Tensor) and experts.dtype in (torch.int32, torch.int64) and experts.dim() in (1, 2)):
         raise CG3DError("expert_plan: experts must be an int32 or int64 tensor [T, k] or [T]")
     n_experts = int(n_experts)
@@ -106,23 +125,43 @@ def _check_rows(who, x, n, plan, what):
 
 
 def _gather(x, plan):
+    _check_rows("expert_gather", x, getattr(plan, "n_tokens", 0), plan, "x")
     lib = _lib.get()
     x = x.contiguous()
     lib.check(x)
     with on_device(x):
-        out = torch.empty((plan.n_rows, x.shape[1]), dtype=x.dtype, device=x.device)
-        lib.call("cg3d_expert_gather", x.data_ptr(), DTYPES[x.dtype], plan.address(ROWS), plan.n_tokens, plan.k, x.shape[1], out.data_ptr(),
+        c = int(x.shape[1])                                     # (in a trace sizes are tensors)
+        out = torch.empty((plan.n_rows, c), dtype=x.dtype, device=x.device)
+        lib.call("cg3d_expert_gather", x.data_ptr(), DTYPES[x.dtype], plan.address(ROWS), plan.n_tokens, plan.k, c, out.data_ptr(),
                  lib.stream())
     return out
+
+
+def _combine_inputs(rows, plan, weights, out_dtype):
+    """-> rows and weights [T, k] as the kernels take them, the output's type."""
+    _check_rows("expert_combine", rows, getattr(plan, "n_rows", 0), plan, "rows")
+    out_dtype = out_dtype or rows.dtype
+    need(out_dtype == rows.dtype or (rows.dtype == torch.float32 and out_dtype in FLOATS), "expert_combine: out_dtype must be the rows' own, "
+         "or float32, bfloat16 or float16 for float32 rows")
+    if weights is not None:
+        need(isinstance(weights, torch.Tensor) and weights.dtype in FLOATS, "expert_combine: weights must be float32, bfloat16 or float16")
+        if weights.dim() == 1 and plan.k == 1:
+            weights = weights.unsqueeze(1)
+        if weights.shape != (plan.n_tokens, plan.k) or weights.device != rows.device:
+            raise CG3DError("expert_combine: weights must be [%d, %d] on %s, got %s on %s" % (plan.n_tokens, plan.k, rows.device,
+                                                                                              tuple(weights.shape), weights.device))
+        weights = weights.contiguous()
+    return rows.contiguous(), weights, out_dtype
 
 
 def _combine(y, plan, w, out_dtype):
     lib = _lib.get()
     lib.check(y, w)
     with on_device(y):
-        out = torch.empty((plan.n_tokens, y.shape[1]), dtype=out_dtype, device=y.device)
+        c = int(y.shape[1])
+        out = torch.empty((plan.n_tokens, c), dtype=out_dtype, device=y.device)
         lib.call("cg3d_expert_combine", y.data_ptr(), DTYPES[y.dtype], plan.address(POS), ptr(w), 0 if w is None else DTYPES[w.dtype],
-                 plan.n_tokens, plan.k, y.shape[1], out.data_ptr(), DTYPES[out_dtype], lib.stream())
+                 plan.n_tokens, plan.k, c, out.data_ptr(), DTYPES[out_dtype], lib.stream())
     return out
 
 
@@ -152,9 +191,9 @@ class _Gather(torch.autograd.Function):
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, plan, w, out_dtype):
-        y, w = y.contiguous(), None if w is None else w.contiguous()
-        ctx.plan, ctx.dtype = plan, y.dtype
+    def forward(ctx, rows, plan, weights, out_dtype):
+        y, w, out_dtype = _combine_inputs(rows, plan, weights, out_dtype)
+        ctx.plan, ctx.dtype, ctx.w_shape = plan, y.dtype, None if w is None else weights.shape
         ctx.save_for_backward(y if ctx.needs_input_grad[2] else None, w)
         ctx.set_materialize_grads(False)
         return _combine(y, plan, w, out_dtype)
@@ -173,32 +212,21 @@ class _Combine(torch.autograd.Function):
             dw = torch.empty_like(w) if ctx.needs_input_grad[2] else None
             lib.call("cg3d_expert_combine_bwd", dout.data_ptr(), ptr(y), DTYPES[dout.dtype], plan.address(PAIRS), ptr(w),
                      0 if w is None else DTYPES[w.dtype], plan.n_tokens, plan.k, c, ptr(dy), ptr(dw), lib.stream())
-        return dy, None, dw, None
+        return dy, None, None if dw is None else dw.view(ctx.w_shape), None
 
 
 def expert_gather(x, plan):
     """x [T, C] float32 / bfloat16 / float16 -> [T * k, C], the tokens' rows in the plan's order (differentiable in x)."""
-    _check_rows("expert_gather", x, getattr(plan, "n_tokens", 0), plan, "x")
-    if not (x.requires_grad and torch.is_grad_enabled()):
-        return _gather(x, plan)
-    return _Gather.apply(x, plan)
+    if recorded() or (torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad):
+        return _Gather.apply(x, plan)
+    return _gather(x, plan)
 
 
 def expert_combine(rows, plan, weights=None, out_dtype=None):
     """rows [T * k, C] in the plan's order -> [T, C]: out[t] = sum_s weights[t, s] * rows[pos[t, s]] over the slots that have a
     row, summed in float32 in slot order and rounded once, to out_dtype (default: the rows' own; float32 rows: any of the three)
     -- differentiable in rows and weights.  weights [T, k] float32 / bfloat16 / float16; None: all ones."""
-    _check_rows("expert_combine", rows, getattr(plan, "n_rows", 0), plan, "rows")
-    out_dtype = out_dtype or rows.dtype
-    need(out_dtype == rows.dtype or (rows.dtype == torch.float32 and out_dtype in FLOATS), "expert_combine: out_dtype must be the rows' own, "
-         "or float32, bfloat16 or float16 for float32 rows")
-    if weights is not None:
-        need(isinstance(weights, torch.Tensor) and weights.dtype in FLOATS, "expert_combine: weights must be float32, bfloat16 or float16")
-        if weights.dim() == 1 and plan.k == 1:
-            weights = weights.unsqueeze(1)
-        if weights.shape != (plan.n_tokens, plan.k) or weights.device != rows.device:
-            raise CG3DError("expert_combine: weights must be [%d, %d] on %s, got %s on %s" % (plan.n_tokens, plan.k, rows.device,
-                                                                                              tuple(weights.shape), weights.device))
-    if not (torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))):
-        return _combine(rows.contiguous(), plan, None if weights is None else weights.contiguous(), out_dtype)
-    return _Combine.apply(rows, plan, weights, out_dtype)
+    if recorded() or (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (rows, weights))):
+        return _Combine.apply(rows, plan, weights, out_dtype)
+    rows, weights, out_dtype = _combine_inputs(rows, plan, weights, out_dtype)
+    return _combine(rows, plan, weights, out_dtype)

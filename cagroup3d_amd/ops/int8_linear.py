@@ -8,23 +8,45 @@ its own for each expert's rows: the served form of the kernel-size-1 convolution
     y = int8_linear(x, weight, plan=plan, gather=True)      # each expert's tokens with its matrix (ops/expert_rows.expert_plan)
 
 The integer sums are exact, so results do not depend on how the work is split.  There is no gradient: a call on inputs that require
-one, with gradients enabled, is refused."""
+one, with gradients enabled, or that carry a tangent is refused.  torch.jit.trace records the calls; weights are laid out and plans
+made outside of it."""
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .._lib import CG3DError, ptr
-from .expert_rows import DTYPES, FLOATS, OFFSETS, ROWS, ExpertPlan, need, on_device
+from .expert_rows import DTYPES, FLOATS, OFFSETS, ROWS, ExpertPlan, need, on_device, recorded
 
 ROWS_IN = tuple(DTYPES)
 MAX_CIN = 131071                  # the int32 sum of so many products of 8-bit values cannot overflow
 
 
+def _no_tangent_for(who, *tensors):
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+                raise CG3DError("%s has no forward-mode derivative" % who)
+
+
 def _no_grad_for(who, *tensors):
     for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
+        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
             raise CG3DError("%s has no gradient: call it under torch.no_grad() or on detached tensors" % who)
+    _no_tangent_for(who, *tensors)
+
+
+class _Recorded(torch.autograd.Function):
+    """A call that torch.jit.trace has to see: f(*args), which has no gradient."""
+
+    @staticmethod
+    def forward(ctx, f, *args):
+        return f(*args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise CG3DError("products in 8 bits have no gradient")
 
 
 class Int8Weight:
@@ -40,6 +62,9 @@ class Int8Weight:
 def int8_weight(w, scale=None):
     """w [cin, cout] or [E, cin, cout] (the layout of the framework's kernels).  Floats: every output channel is quantised to
     scale * (-127 .. 127), scale = max |w| / 127.  int8: `scale` float32 [cout] ([E, cout]) must be given and w is taken as it is."""
+    if recorded():
+        need(not torch.jit.is_tracing(), "int8_weight: a trace would keep the weights it was made with; lay them out outside the trace")
+        _no_tangent_for("int8_weight", w, scale)
     need(isinstance(w, torch.Tensor) and w.dtype in DTYPES and w.dim() in (2, 3),
          "int8_weight: w must be float32, bfloat16, float16 or int8, [cin, cout] or [experts, cin, cout]")
     grouped = w.dim() == 3
@@ -80,12 +105,16 @@ def _ws_bytes(lib, *sizes):
 def quantize_rows(x):
     """x [rows, cin] float32 / bfloat16 / float16 -> (q int8 [rows, cin], scale float32 [rows]): scale = max |x| / 127 of each row,
     q = the nearest level, ties to the even one.  A row of zeros has the scale 0, one with an infinity or a NaN the scale NaN."""
-    _rows_in("quantize_rows", x, FLOATS)
     _no_grad_for("quantize_rows", x)
+    return _Recorded.apply(_quantize, x) if recorded() else _quantize(x)
+
+
+def _quantize(x):
+    _rows_in("quantize_rows", x, FLOATS)
     lib = _lib.get()
     x = x.detach().contiguous()
     lib.check(x)
-    n, cin = x.shape
+    n, cin = (int(i) for i in x.shape)                            # (in a trace sizes are tensors)
     with on_device(x):
         q = torch.empty((n, cin), dtype=torch.int8, device=x.device)
         scale = torch.empty(n, dtype=torch.float32, device=x.device)
@@ -101,11 +130,18 @@ def int8_linear(x, weight, bias=None, scale=None, out_dtype=None, plan=None, gat
     plan (ops/expert_rows.expert_plan): weight holds plan.n_experts matrices and each row is multiplied by its expert's; x has the
     plan's rows ([T * k, cin], what expert_gather gives), or with gather=True the tokens ([T, cin]), whose rows are picked in the
     product.  Rows behind the last are zeros."""
+    _no_grad_for("int8_linear", x, bias, scale)
+    args = x, weight, bias, scale, out_dtype, plan, gather
+    return _Recorded.apply(_linear, *args) if recorded() else _linear(*args)
+
+
+def _linear(x, weight, bias, scale, out_dtype, plan, gather):
     # (plain comparisons before any message is made: the call's host time is that of a small product)
     if not isinstance(weight, Int8Weight):
         raise CG3DError("int8_linear: weight must come from int8_weight")
     _rows_in("int8_linear", x, ROWS_IN)
     n_x, cin = x.shape
+    n_x, cin = int(n_x), int(cin)                                 # (in a trace sizes are tensors)
     dtype, dev, cout, n_experts = x.dtype, x.device, weight.cout, weight.n_experts
     if cin != weight.cin:
         raise CG3DError("int8_linear: x has %d columns, weight %d rows" % (cin, weight.cin))
@@ -137,7 +173,6 @@ def int8_linear(x, weight, bias=None, scale=None, out_dtype=None, plan=None, gat
             bias.shape == (cout,) or (weight.grouped and bias.shape == (n_experts, cout))),
             "int8_linear: bias must be floats [%d] (or [%d, %d] with a matrix for each expert) on %s", cout, n_experts, cout, dev)
         per_expert = int(bias.dim() == 2)
-    _no_grad_for("int8_linear", x, bias, scale)
     if bias is not None and not (bias.dtype is torch.float32 and bias.is_contiguous()):
         bias = bias.detach().to(torch.float32).contiguous()
     lib = _lib.get()

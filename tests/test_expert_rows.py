@@ -6,6 +6,8 @@ one workgroup sorts -- the gradients against the formulas and against difference
 with the grouped product of the framework."""
 import pytest
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from cagroup3d_amd import _lib, me
 from cagroup3d_amd.ops.expert_rows import MAX_EXPERTS, expert_combine, expert_gather, expert_plan
@@ -481,3 +483,43 @@ def test_empty_batch_has_gradients(oracle):
 @pytest.mark.gpu
 def test_hip_empty_batch_has_gradients(hip):
     empty_batch("cuda")
+
+
+def traced_and_dual(dev):
+    """What torch has to see of a call -- a trace, forward-mode differentiation -- is seen by it without gradients too: a trace
+    computes, and has its checks, on new inputs; a tangent is refused and not dropped; a plan, which is no tensor, is not made in a
+    trace."""
+    ids = routing(9, 2, 3, "dropped", 70).to(dev)
+    plan = expert_plan(ids, 3)
+    g = torch.Generator().manual_seed(71)
+    x, y, w = torch.randn(9, 8, generator=g).to(dev), torch.randn(18, 8, generator=g).to(dev), torch.rand(9, 2, generator=g).to(dev)
+    calls = ((lambda a: expert_gather(a, plan), x), (lambda a: expert_combine(a, plan, w), y), (lambda a: expert_combine(a, plan), y),
+             (lambda a: expert_combine(y, plan, a, torch.bfloat16), w))
+    for f, a in calls:
+        for grad in (False, True):
+            traced = torch.jit.trace(f, (a.clone().requires_grad_(grad),))
+            junk = [torch.full_like(f(a), 7.0) for _ in range(4)]            # (memory that an output without a kernel would show)
+            del junk
+            assert torch.equal(traced(3 * a), f(3 * a))
+            with pytest.raises(RuntimeError, match="must be"):               # (TorchScript's own error around the refusal)
+                traced(a[:-1].contiguous())
+        with forward_ad.dual_level():
+            assert torch.equal(f(a), f(a))                                   # (no tangent)
+            with pytest.raises(NotImplementedError):
+                f(forward_ad.make_dual(a, torch.ones_like(a)))
+        with pytest.raises(_lib.CG3DError):
+            make_fx(f)(a)
+    with pytest.raises(_lib.CG3DError):
+        torch.jit.trace(lambda i: expert_plan(i, 3).rows, (ids,))
+    with pytest.raises(_lib.CG3DError):
+        make_fx(lambda i: expert_plan(i, 3).rows)(ids)
+
+
+def test_traces_and_tangents(oracle):
+    with _lib.use_library(oracle):
+        traced_and_dual("cpu")
+
+
+@pytest.mark.gpu
+def test_hip_traces_and_tangents(hip):
+    traced_and_dual("cuda")

@@ -9,6 +9,8 @@ import pickle
 
 import pytest
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from cagroup3d_amd import _lib
 from cagroup3d_amd.ops.expert_rows import expert_combine, expert_gather, expert_plan
@@ -555,3 +557,48 @@ def test_hip_refusals(hip):
         with pytest.raises(_lib.CG3DError):
             bad()
     assert int8_linear(torch.zeros(0, 8, device="cuda"), w).shape == (0, 6)
+
+
+def traced_and_dual(dev):
+    """torch.jit.trace records the calls (and their checks run on new inputs); a tangent, a graph of torch's own operators and weights
+    laid out inside a trace are refused."""
+    x, _, w, b = make(12, 40, 20, F32, 70, 3)
+    x, w, b = x.to(dev), w.to(dev), b.to(dev)
+    weight, one, plan = int8_weight(w), int8_weight(w[0]), expert_plan(torch.arange(12).remainder(3).to(dev), 3)
+    q, s = quantize_rows(x)
+    calls = ((lambda a: int8_linear(a, one, b[0]), x), (lambda a: int8_linear(a, weight, b, plan=plan, gather=True, out_dtype=BF16), x),
+             (lambda a: int8_linear(a, weight, plan=plan), x.to(BF16)), (lambda a: int8_linear(q, one, scale=a), s), (lambda a: int8_linear(x, one, a), b[0]),
+             (lambda a: quantize_rows(a)[0], x), (lambda a: quantize_rows(a)[1], x))
+    for f, a in calls:
+        traced = torch.jit.trace(f, (a,))
+        junk = [torch.full_like(f(a), 7.0) for _ in range(4)]
+        del junk
+        other = (a.flip(0) * 3).contiguous()
+        assert torch.equal(traced(other), f(other))
+        with torch.no_grad():
+            traced = torch.jit.trace(f, (a.clone().requires_grad_(),))
+        assert torch.equal(traced(other), f(other))
+        with forward_ad.dual_level():
+            assert torch.equal(f(a), f(a))
+            with pytest.raises(_lib.CG3DError):
+                f(forward_ad.make_dual(a, torch.ones_like(a)))
+        with pytest.raises(_lib.CG3DError):
+            make_fx(f)(a)
+        with pytest.raises(_lib.CG3DError):
+            torch.jit.trace(f, (a.clone().requires_grad_(),))
+    with pytest.raises(RuntimeError, match="columns"):
+        torch.jit.trace(calls[0][0], (x,))(x[:, 1:].contiguous())
+    with pytest.raises(_lib.CG3DError):
+        torch.jit.trace(lambda a: int8_linear(x, int8_weight(a)), (w[0],))
+    with forward_ad.dual_level(), pytest.raises(_lib.CG3DError):
+        int8_weight(forward_ad.make_dual(w, torch.ones_like(w)))
+
+
+def test_traces_and_tangents(oracle):
+    with _lib.use_library(oracle):
+        traced_and_dual("cpu")
+
+
+@pytest.mark.gpu
+def test_hip_traces_and_tangents(hip):
+    traced_and_dual("cuda")
