@@ -75,9 +75,14 @@ class ExpertPlan:
     pos = property(lambda self: self._slice(2, self.n_rows).view(self.n_tokens, self.k))
     offsets = property(lambda self: self._slice(3, self.n_experts + 1))
 
-    def address(self, i):
-        """Of table i: rows, pairs, pos, offsets."""
-        return self._tables.data_ptr() + 4 * (self._at + i * self.n_rows)
+    def address(self, i, tables=None):
+        """Of table i: rows, pairs, pos, offsets -- in `tables`, a saved form of them."""
+        return (self._tables if tables is None else tables).data_ptr() + 4 * (self._at + i * self.n_rows)
+
+    def to_save(self):
+        """The tables as a saved tensor of a pass, so that one that is written before its backward pass is noticed (None for a plan made
+        in inference mode, whose tensors autograd neither saves nor watches)."""
+        return None if self._tables.is_inference() else self._tables
 
 
 ROWS, PAIRS, POS, OFFSETS = range(4)
@@ -154,13 +159,13 @@ def _combine_inputs(rows, plan, weights, out_dtype):
     return rows.contiguous(), weights, out_dtype
 
 
-def _combine(y, plan, w, out_dtype):
+def _combine(y, plan, w, out_dtype, tables=None):
     lib = _lib.get()
     lib.check(y, w)
     with on_device(y):
         c = int(y.shape[1])
         out = torch.empty((plan.n_tokens, c), dtype=out_dtype, device=y.device)
-        lib.call("cg3d_expert_combine", y.data_ptr(), DTYPES[y.dtype], plan.address(POS), ptr(w), 0 if w is None else DTYPES[w.dtype],
+        lib.call("cg3d_expert_combine", y.data_ptr(), DTYPES[y.dtype], plan.address(POS, tables), ptr(w), 0 if w is None else DTYPES[w.dtype],
                  plan.n_tokens, plan.k, c, out.data_ptr(), DTYPES[out_dtype], lib.stream())
     return out
 
@@ -179,14 +184,19 @@ def _once(backward):
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
+        out = _gather(x, plan)
         ctx.plan = plan
+        ctx.save_for_backward(plan.to_save())
         ctx.set_materialize_grads(False)
-        return _gather(x, plan)
+        return out
 
     @staticmethod
     @_once
     def backward(ctx, dout):
-        return None if dout is None else _combine(dout.contiguous(), ctx.plan, None, dout.dtype), None
+        if dout is None:
+            return None, None
+        tables, = ctx.saved_tensors
+        return _combine(dout.contiguous(), ctx.plan, None, dout.dtype, tables), None
 
 
 class _Combine(torch.autograd.Function):
@@ -194,7 +204,7 @@ class _Combine(torch.autograd.Function):
     def forward(ctx, rows, plan, weights, out_dtype):
         y, w, out_dtype = _combine_inputs(rows, plan, weights, out_dtype)
         ctx.plan, ctx.dtype, ctx.w_shape = plan, y.dtype, None if w is None else weights.shape
-        ctx.save_for_backward(y if ctx.needs_input_grad[2] else None, w)
+        ctx.save_for_backward(y if ctx.needs_input_grad[2] else None, w, plan.to_save())
         ctx.set_materialize_grads(False)
         return _combine(y, plan, w, out_dtype)
 
@@ -203,14 +213,14 @@ class _Combine(torch.autograd.Function):
     def backward(ctx, dout):
         if dout is None:
             return None, None, None, None
-        y, w = ctx.saved_tensors
+        y, w, tables = ctx.saved_tensors
         plan, c = ctx.plan, dout.shape[1]
         lib = _lib.get()
         dout = dout.to(ctx.dtype).contiguous()                  # (wider than the output where the rows are)
         with on_device(dout):
             dy = torch.empty((plan.n_rows, c), dtype=dout.dtype, device=dout.device) if ctx.needs_input_grad[0] else None
             dw = torch.empty_like(w) if ctx.needs_input_grad[2] else None
-            lib.call("cg3d_expert_combine_bwd", dout.data_ptr(), ptr(y), DTYPES[dout.dtype], plan.address(PAIRS), ptr(w),
+            lib.call("cg3d_expert_combine_bwd", dout.data_ptr(), ptr(y), DTYPES[dout.dtype], plan.address(PAIRS, tables), ptr(w),
                      0 if w is None else DTYPES[w.dtype], plan.n_tokens, plan.k, c, ptr(dy), ptr(dw), lib.stream())
         return dy, None, None if dw is None else dw.view(ctx.w_shape), None
 

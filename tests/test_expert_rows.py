@@ -523,3 +523,48 @@ def test_traces_and_tangents(oracle):
 @pytest.mark.gpu
 def test_hip_traces_and_tangents(hip):
     traced_and_dual("cuda")
+
+
+def tables_are_saved(dev):
+    """A plan's tables are saved tensors of both passes: one that is written between forward and backward is noticed, hooks of
+    saved tensors see it, and the backward pass reads what they give back."""
+    ids = routing(9, 2, 3, "dropped", 80).to(dev)
+    g = torch.Generator().manual_seed(81)
+    x, y, w = torch.randn(9, 8, generator=g).to(dev), torch.randn(18, 8, generator=g).to(dev), torch.rand(9, 2, generator=g).to(dev)
+
+    def passes(plan):
+        a, b, c = (t.clone().requires_grad_() for t in (x, y, w))
+        return (lambda: (expert_gather(a, plan), (a,)), lambda: (expert_combine(b, plan, c), (b, c)), lambda: (expert_combine(b, plan), (b,)))
+    for i in range(3):
+        plan = expert_plan(ids, 3)
+        want = [t.clone() for o, v in [passes(plan)[i]()] for t in torch.autograd.grad(o.sum(), v)]
+        out, leaves = passes(plan)[i]()
+        plan.pos[0, 0] = 5
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out.sum(), leaves)
+        plan, packed = expert_plan(ids, 3), []
+
+        def pack(t):
+            packed.append(t)
+            return t.clone()
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.clone()):
+            out, leaves = passes(plan)[i]()
+        assert any(t.dtype == torch.int32 for t in packed)
+        with torch.no_grad():
+            for t in (plan.rows, plan.pairs, plan.pos):
+                t.fill_(0)                                                   # (the hooks gave copies)
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(out.sum(), leaves), want))
+        with torch.inference_mode():                                         # a router's plan, made without any bookkeeping
+            plan = expert_plan(ids, 3)
+        out, leaves = passes(plan)[i]()
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(out.sum(), leaves), want))
+
+
+def test_tables_are_saved_tensors(oracle):
+    with _lib.use_library(oracle):
+        tables_are_saved("cpu")
+
+
+@pytest.mark.gpu
+def test_hip_tables_are_saved_tensors(hip):
+    tables_are_saved("cuda")
