@@ -55,6 +55,11 @@ def recorded():
     return forward_ad._current_level >= 0 or _TRACING()
 
 
+def whole(t):
+    """t contiguous, its memory holding its values (that of a lazily negated view holds the opposite ones)."""
+    return (t.resolve_neg() if t.is_neg() else t).contiguous()
+
+
 class ExpertPlan:
     """Where the rows of a routing go.  offsets int32 [n_experts + 1], rows int32 [T * k] (the token of each row, -1 behind the
     last), pairs int32 [T * k] (the pair t * k + s of each row, negative behind the last), pos int32 [T, k] (the row of each pair;
@@ -103,7 +108,7 @@ def expert_plan(experts, n_experts):
     n_experts = int(n_experts)
     if not 1 <= n_experts <= MAX_EXPERTS:
         raise CG3DError("expert_plan: n_experts = %d is not in 1 .. %d" % (n_experts, MAX_EXPERTS))
-    ids = (experts if experts.dim() == 2 else experts.unsqueeze(1)).contiguous()
+    ids = whole(experts if experts.dim() == 2 else experts.unsqueeze(1))
     t, k = ids.shape
     if k < 1 or t * k >= 2 ** 31:
         raise CG3DError("expert_plan: %d x %d pairs (k >= 1, fewer than 2^31 pairs)" % (t, k))
@@ -132,7 +137,7 @@ def _check_rows(who, x, n, plan, what):
 def _gather(x, plan):
     _check_rows("expert_gather", x, getattr(plan, "n_tokens", 0), plan, "x")
     lib = _lib.get()
-    x = x.contiguous()
+    x = whole(x)
     lib.check(x)
     with on_device(x):
         c = int(x.shape[1])                                     # (in a trace sizes are tensors)
@@ -155,8 +160,8 @@ def _combine_inputs(rows, plan, weights, out_dtype):
         if weights.shape != (plan.n_tokens, plan.k) or weights.device != rows.device:
             raise CG3DError("expert_combine: weights must be [%d, %d] on %s, got %s on %s" % (plan.n_tokens, plan.k, rows.device,
                                                                                               tuple(weights.shape), weights.device))
-        weights = weights.contiguous()
-    return rows.contiguous(), weights, out_dtype
+        weights = whole(weights)
+    return whole(rows), weights, out_dtype
 
 
 def _combine(y, plan, w, out_dtype, tables=None):
@@ -196,7 +201,7 @@ class _Gather(torch.autograd.Function):
         if dout is None:
             return None, None
         tables, = ctx.saved_tensors
-        return _combine(dout.contiguous(), ctx.plan, None, dout.dtype, tables), None
+        return _combine(whole(dout), ctx.plan, None, dout.dtype, tables), None
 
 
 class _Combine(torch.autograd.Function):
@@ -216,7 +221,8 @@ class _Combine(torch.autograd.Function):
         y, w, tables = ctx.saved_tensors
         plan, c = ctx.plan, dout.shape[1]
         lib = _lib.get()
-        dout = dout.to(ctx.dtype).contiguous()                  # (wider than the output where the rows are)
+        dout = whole(dout.to(ctx.dtype))                        # (wider than the output where the rows are)
+        lib.check(dout, y, w, tables)                           # (what hooks of saved tensors gave back)
         with on_device(dout):
             dy = torch.empty((plan.n_rows, c), dtype=dout.dtype, device=dout.device) if ctx.needs_input_grad[0] else None
             dw = torch.empty_like(w) if ctx.needs_input_grad[2] else None

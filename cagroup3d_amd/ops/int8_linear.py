@@ -17,7 +17,7 @@ from torch.autograd import forward_ad
 
 from .. import _lib
 from .._lib import CG3DError, ptr
-from .expert_rows import DTYPES, FLOATS, OFFSETS, ROWS, ExpertPlan, need, on_device, recorded
+from .expert_rows import DTYPES, FLOATS, OFFSETS, ROWS, ExpertPlan, need, on_device, recorded, whole
 
 ROWS_IN = tuple(DTYPES)
 MAX_CIN = 131071                  # the int32 sum of so many products of 8-bit values cannot overflow
@@ -78,14 +78,14 @@ def int8_weight(w, scale=None):
     else:
         need(scale is None, "int8_weight: the scale of weights in floats is computed here")
     lib = _lib.get()
-    w = w.detach().contiguous()
+    w = whole(w.detach())
     lib.check(w)
     with on_device(w):
         packed = torch.empty(int(lib.raw("cg3d_int8_weight_bytes")(e, cin, cout)), dtype=torch.int8, device=w.device)
         if scale is None:
             out, ws = torch.empty((2, e, cout), dtype=torch.float32, device=w.device)
         else:
-            out, ws = scale.detach().clone(memory_format=torch.contiguous_format).view(e, cout), None      # (the handle's own: the caller may reuse the memory)
+            out, ws = scale.detach().resolve_neg().clone(memory_format=torch.contiguous_format).view(e, cout), None      # (the handle's own: the caller may reuse the memory)
         lib.call("cg3d_int8_weight", ptr(w), DTYPES[w.dtype], e, cin, cout, ptr(packed),
                  ptr(out) if ws is not None else None, ptr(ws), lib.stream())
     return Int8Weight(packed, out, e, cin, cout, grouped)
@@ -112,7 +112,7 @@ def quantize_rows(x):
 def _quantize(x):
     _rows_in("quantize_rows", x, FLOATS)
     lib = _lib.get()
-    x = x.detach().contiguous()
+    x = whole(x.detach())
     lib.check(x)
     n, cin = (int(i) for i in x.shape)                            # (in a trace sizes are tensors)
     with on_device(x):
@@ -151,7 +151,7 @@ def _linear(x, weight, bias, scale, out_dtype, plan, gather):
         need(isinstance(scale, torch.Tensor) and scale.dtype == torch.float32 and scale.shape == (n_x,) and scale.device == dev,
              "int8_linear: rows in 8 bits need their scale beside them, float32 [%d]", n_x)
         out_dtype = out_dtype or torch.float32
-        scale = scale.contiguous()
+        scale = whole(scale)
     else:
         need(scale is None, "int8_linear: the scale of rows in floats is computed here")
         out_dtype = out_dtype or dtype
@@ -173,10 +173,10 @@ def _linear(x, weight, bias, scale, out_dtype, plan, gather):
             bias.shape == (cout,) or (weight.grouped and bias.shape == (n_experts, cout))),
             "int8_linear: bias must be floats [%d] (or [%d, %d] with a matrix for each expert) on %s", cout, n_experts, cout, dev)
         per_expert = int(bias.dim() == 2)
-    if bias is not None and not (bias.dtype is torch.float32 and bias.is_contiguous()):
-        bias = bias.detach().to(torch.float32).contiguous()
+    if bias is not None and not (bias.dtype is torch.float32 and bias.is_contiguous() and not bias.is_neg()):
+        bias = whole(bias.detach().to(torch.float32))
     lib = _lib.get()
-    x = x.contiguous()
+    x = whole(x)
     lib.check(x)
     code = DTYPES[dtype]
     with on_device(x):

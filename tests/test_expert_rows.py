@@ -568,3 +568,34 @@ def test_tables_are_saved_tensors(oracle):
 @pytest.mark.gpu
 def test_hip_tables_are_saved_tensors(hip):
     tables_are_saved("cuda")
+
+
+def negated_views(dev):
+    """Views whose memory holds the opposite of their values (as torch's conjugates make them) count with their values."""
+    g = torch.Generator().manual_seed(90)
+    ids = routing(9, 2, 3, "dropped", 91).to(dev)
+    x, y, w = torch.randn(9, 8, generator=g).to(dev), torch.randn(18, 8, generator=g).to(dev), torch.rand(9, 2, generator=g).to(dev)
+    plan, neg = expert_plan(ids, 3), torch._neg_view
+    other = expert_plan(neg((-ids).contiguous()), 3)
+    assert torch.equal(other.rows, plan.rows) and torch.equal(other.pos, plan.pos)
+    for grad in (False, True):
+        a, b, c = (t.clone().requires_grad_(grad) for t in (x, y, w))
+        out = expert_gather(neg(a), plan)
+        assert torch.equal(out, expert_gather(-x, plan))
+        both = expert_combine(neg(b), plan, neg(c))
+        assert torch.equal(both, expert_combine(-y, plan, -w)) and torch.equal(expert_combine(neg(b), plan), expert_combine(-y, plan))
+        if grad:
+            got = torch.autograd.grad([out, both], [a, b, c], [neg(y), neg(x)])
+            l, m, n = (t.clone().requires_grad_() for t in (x, y, w))
+            want = torch.autograd.grad([expert_gather(-l, plan), expert_combine(-m, plan, -n)], [l, m, n], [-y, -x])
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_negated_views(oracle):
+    with _lib.use_library(oracle):
+        negated_views("cpu")
+
+
+@pytest.mark.gpu
+def test_hip_negated_views(hip):
+    negated_views("cuda")

@@ -602,3 +602,28 @@ def test_traces_and_tangents(oracle):
 @pytest.mark.gpu
 def test_hip_traces_and_tangents(hip):
     traced_and_dual("cuda")
+
+
+def negated_views(dev):
+    """Views whose memory holds the opposite of their values count with their values."""
+    x, _, w, b = make(12, 40, 20, F32, 80, 3)
+    x, w, b, neg = x.to(dev), w.to(dev), b.to(dev), torch._neg_view
+    weight, one, plan = int8_weight(w), int8_weight(w[0]), expert_plan(torch.arange(12).remainder(3).to(dev), 3)
+    q, s = quantize_rows(x)
+    assert torch.equal(quantize_rows(neg(x))[0], -q) and torch.equal(quantize_rows(neg(x))[1], s)
+    assert torch.equal(int8_linear(neg(x), one, neg(b[0])), int8_linear(-x, one, -b[0]))
+    assert torch.equal(int8_linear(neg(x), weight, neg(b.to(BF16)), plan=plan, gather=True), int8_linear(-x, weight, -b.to(BF16), plan=plan, gather=True))
+    assert torch.equal(int8_linear(neg(q), one, scale=neg(s)), int8_linear(q, one, scale=s))       # (both signs)
+    assert torch.equal(int8_linear(x, int8_weight(neg(w)), plan=plan), int8_linear(x, int8_weight(-w), plan=plan))
+    wq = quantize_rows(w[0].t().contiguous())[0].t()
+    assert torch.equal(int8_linear(x, int8_weight(neg(wq), neg(b[0]))), int8_linear(x, int8_weight(-wq, -b[0])))
+
+
+def test_negated_views(oracle):
+    with _lib.use_library(oracle):
+        negated_views("cpu")
+
+
+@pytest.mark.gpu
+def test_hip_negated_views(hip):
+    negated_views("cuda")
