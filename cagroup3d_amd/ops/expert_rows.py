@@ -60,6 +60,11 @@ def whole(t):
     return (t.resolve_neg() if t.is_neg() else t).contiguous()
 
 
+def held(*things):
+    """What a launch has the addresses of is used once more behind it: torch.compile, which stops at an address and resumes with what
+    the rest of the function uses, would free workspaces and copies of inputs before the launch."""
+
+
 class ExpertPlan:
     """Where the rows of a routing go.  offsets int32 [n_experts + 1], rows int32 [T * k] (the token of each row, -1 behind the
     last), pairs int32 [T * k] (the pair t * k + s of each row, negative behind the last), pos int32 [T, k] (the row of each pair;
@@ -121,6 +126,7 @@ def expert_plan(experts, n_experts):
         rows = plan.address(ROWS)
         lib.call("cg3d_expert_plan", ids.data_ptr(), int(ids.dtype == torch.int64), t, k, n_experts, plan.address(OFFSETS), rows,
                  plan.address(PAIRS), plan.address(POS), rows - 4 * at if at else None, lib.stream())
+    held(ids)
     return plan
 
 
@@ -144,6 +150,7 @@ def _gather(x, plan):
         out = torch.empty((plan.n_rows, c), dtype=x.dtype, device=x.device)
         lib.call("cg3d_expert_gather", x.data_ptr(), DTYPES[x.dtype], plan.address(ROWS), plan.n_tokens, plan.k, c, out.data_ptr(),
                  lib.stream())
+    held(x, plan)
     return out
 
 
@@ -172,6 +179,7 @@ def _combine(y, plan, w, out_dtype, tables=None):
         out = torch.empty((plan.n_tokens, c), dtype=out_dtype, device=y.device)
         lib.call("cg3d_expert_combine", y.data_ptr(), DTYPES[y.dtype], plan.address(POS, tables), ptr(w), 0 if w is None else DTYPES[w.dtype],
                  plan.n_tokens, plan.k, c, out.data_ptr(), DTYPES[out_dtype], lib.stream())
+    held(y, w, plan, tables)
     return out
 
 
@@ -228,6 +236,7 @@ class _Combine(torch.autograd.Function):
             dw = torch.empty_like(w) if ctx.needs_input_grad[2] else None
             lib.call("cg3d_expert_combine_bwd", dout.data_ptr(), ptr(y), DTYPES[dout.dtype], plan.address(PAIRS, tables), ptr(w),
                      0 if w is None else DTYPES[w.dtype], plan.n_tokens, plan.k, c, ptr(dy), ptr(dw), lib.stream())
+        held(dout, y, w, plan, tables)
         return dy, None, None if dw is None else dw.view(ctx.w_shape), None
 
 

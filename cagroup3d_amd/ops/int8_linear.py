@@ -17,7 +17,7 @@ from torch.autograd import forward_ad
 
 from .. import _lib
 from .._lib import CG3DError, ptr
-from .expert_rows import DTYPES, FLOATS, OFFSETS, ROWS, ExpertPlan, need, on_device, recorded, whole
+from .expert_rows import DTYPES, FLOATS, OFFSETS, ROWS, ExpertPlan, held, need, on_device, recorded, whole
 
 ROWS_IN = tuple(DTYPES)
 MAX_CIN = 131071                  # the int32 sum of so many products of 8-bit values cannot overflow
@@ -88,6 +88,7 @@ def int8_weight(w, scale=None):
             out, ws = scale.detach().resolve_neg().clone(memory_format=torch.contiguous_format).view(e, cout), None      # (the handle's own: the caller may reuse the memory)
         lib.call("cg3d_int8_weight", ptr(w), DTYPES[w.dtype], e, cin, cout, ptr(packed),
                  ptr(out) if ws is not None else None, ptr(ws), lib.stream())
+    held(w, ws)
     return Int8Weight(packed, out, e, cin, cout, grouped)
 
 
@@ -120,6 +121,7 @@ def _quantize(x):
         scale = torch.empty(n, dtype=torch.float32, device=x.device)
         lib.call("cg3d_int8_quantize_rows", ptr(x), DTYPES[x.dtype], n, cin, cin, ptr(q), ptr(scale),
                  lib.stream())
+    held(x)
     return q, scale
 
 
@@ -185,4 +187,5 @@ def _linear(x, weight, bias, scale, out_dtype, plan, gather):
         ws = torch.empty(ws_bytes, dtype=torch.int8, device=dev) if ws_bytes > 0 else None
         lib.call("cg3d_int8_linear", x.data_ptr(), code, ptr(scale), n_x, cin, weight.packed.data_ptr(), weight.scale.data_ptr(), ptr(bias), per_expert,
                  offsets, rows, y.data_ptr(), DTYPES[out_dtype], n_rows, cout, n_experts, ptr(ws), lib.stream())
+    held(x, scale, weight, bias, plan, ws)
     return y

@@ -627,3 +627,30 @@ def test_negated_views(oracle):
 @pytest.mark.gpu
 def test_hip_negated_views(hip):
     negated_views("cuda")
+
+
+def compiled(dev):
+    """torch.compile stops at the addresses that a call takes and resumes behind them: workspaces, copies of inputs, weights and plans made
+    for one call are there until it has been made."""
+    x, _, w, b = make(60, 40, 20, F32, 90, 3)
+    x, w, b, gate, ids = x.to(dev), w.to(dev), b.to(dev), torch.rand(60, 2).to(dev), ids_of(60, 2, 3, "dropped", 91).to(dev)
+    weight, plan = int8_weight(w), expert_plan(ids, 3)
+    turned = lambda t: t.t().contiguous().t()                     # (copied by the call)
+    for f in (lambda t: expert_gather(turned(t), expert_plan(turned(ids), 3)), lambda t: expert_combine(turned(expert_gather(t, plan)), plan, turned(gate)),
+              lambda t: quantize_rows(turned(t))[0], lambda t: int8_linear(turned(t), int8_weight(turned(w[0])), b[0].to(BF16)),
+              lambda t: expert_combine(int8_linear(t, weight, b, plan=plan, gather=True), plan, gate),
+              lambda t: torch.autograd.grad(expert_combine(expert_gather(t.requires_grad_(), plan), plan, gate).sum(), [t])[0]):
+        torch._dynamo.reset()
+        g = torch.compile(f, backend="eager")
+        for i in range(20):
+            assert torch.equal(g(x * i), f(x * i))
+
+
+def test_compiled(oracle):
+    with _lib.use_library(oracle):
+        compiled("cpu")
+
+
+@pytest.mark.gpu
+def test_hip_compiled(hip):
+    compiled("cuda")
