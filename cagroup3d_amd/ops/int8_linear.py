@@ -105,7 +105,8 @@ def _ws_bytes(lib, *sizes):
 
 def quantize_rows(x):
     """x [rows, cin] float32 / bfloat16 / float16 -> (q int8 [rows, cin], scale float32 [rows]): scale = max |x| / 127 of each row,
-    q = the nearest level, ties to the even one.  A row of zeros has the scale 0, one with an infinity or a NaN the scale NaN."""
+    q = the nearest level, ties to the even one.  A row of zeros has the scale 0, one with an infinity or a NaN the scale NaN;
+    the scale of a row whose largest magnitude is below 1.5e-36 is subnormal and has fewer bits."""
     _no_grad_for("quantize_rows", x)
     return _Recorded.apply(_quantize, x) if recorded() else _quantize(x)
 

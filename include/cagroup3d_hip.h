@@ -614,9 +614,10 @@ int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, cons
 
 /* ------------------------------------------------------------------------------------------
  * Products in 8-bit integers with a scale for each row and each output channel, dense or grouped by expert (inference).
- *   y[r, n] = (sum_k q[r, k] * w[k, n]) * sx[r] * sw[n] + bias[n]; the sum is exact (int32, cin <= 131071).
+ *   y[r, n] = (sum_k q[r, k] * w[k, n]) * sx[r] * sw[n] + bias[n]; the sum is exact (int32, cin <= 131071), and no step on the way
+ *     leaves fp32's range where the scaled sum does not, for any scales.
  *   quantize_rows: scale[r] = max_k |x[r, k]| / 127, q = 127 x / max rounded to the nearest level, ties to even, decided exactly;
- *     a row with an infinity or NaN: scale NaN, q 0; q [n][pitch], bytes [cin, pitch) zeros.
+ *     a row with an infinity or NaN: scale NaN, q 0; the scale of a row below 1.5e-36 is subnormal and has fewer bits; q [n][pitch], bytes [cin, pitch) zeros.
  *   weight: w [n_experts][cin][cout] -> packed (cg3d_int8_weight_bytes bytes, 16-byte aligned; the kernels' own order).  Floats:
  *     quantised by the same rule for each (expert, channel), scale [n_experts][cout] is written, ws = 4 * n_experts * cout bytes;
  *     CG3D_DT_I8: packed as they are, scale and ws are not used (the caller holds the scales).

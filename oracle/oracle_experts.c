@@ -240,7 +240,9 @@ int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, int64_t n_x,
             if (e < n_experts) {
                 int32_t sum = 0;
                 for (int32_t k = 0; k < cin; k++) sum += (int32_t)q[src * cin + k] * w[place(e, k, n, cin, cout)];
-                v = (float)sum * sx[src] * sw[(int64_t)e * cout + n];
+                const float a = fabsf(sx[src]);               /* (scales at the range's ends: sum * sx is kept inside it) */
+                const float by = a >= 0x1p96f ? 0x1p-64f : a < 0x1p-126f ? 0x1p64f : 1.f;
+                v = (float)sum * (sx[src] * by) * sw[(int64_t)e * cout + n] * (1.f / by);
                 if (bias) v += bias[(bias_per_expert ? (int64_t)e * cout : 0) + n];
             }
             st(y, out_dtype, r * cout + n, v);

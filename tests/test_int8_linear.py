@@ -654,3 +654,48 @@ def test_compiled(oracle):
 @pytest.mark.gpu
 def test_hip_compiled(hip):
     compiled("cuda")
+
+
+def far_scales(dev, sizes):
+    """Row and channel scales at both ends of fp32's range whose product with the sum is back in it: no step on the way leaves the range
+    or its full precision.  In floats (rows of 1e35 against weights of 1e-5 and the like) and in 8 bits, where the scales are given; a
+    result beyond the type is an infinity, one below it rounds once more."""
+    g = torch.Generator().manual_seed(100)
+    for n, cin, cout in sizes:
+        for top, low in ((3e37, 1e-3), (1e35, 1e-5), (3e38, 1e-30), (1e-30, 1e20), (1e-5, 1e35), (1e-30, 3e38)):
+            x = torch.randn(n, cin, generator=g).clamp(-3, 3) * (top / 3.1)
+            w = torch.randn(cin, cout, generator=g).clamp(-3, 3) * (low / 3.1)
+            wq, sw = plain_levels(w.t().contiguous())
+            for dtype in (F32, BF16):
+                v = x.to(dtype)
+                y = int8_linear(v.to(dev), int8_weight(w.to(dev)), out_dtype=F32)
+                want, size = reference(v, None, wq.t().unsqueeze(0), sw.unsqueeze(0), None, torch.zeros(n, dtype=torch.long), torch.arange(n))
+                assert bool((want.abs().amax() < 2.0 ** 127))
+                close(y, want, size, F32)
+        q = torch.randint(-128, 128, (n, cin), generator=g).to(I8)
+        wq = torch.randint(-128, 128, (cin, cout), generator=g).to(I8)
+        for a, b in ((2.0 ** 120, 2.0 ** -149), (2.0 ** 126, 2.0 ** -140), (2.0 ** -149, 2.0 ** 100), (1.5 * 2.0 ** -126, 1.25 * 2.0 ** 127), (2.0 ** -140, 2.0 ** 127),
+                     (1.7 * 2.0 ** -70, 1.3 * 2.0 ** -70), (2.0 ** -100, 1.1), (1.9 * 2.0 ** 64, 1.1 * 2.0 ** -64)):
+            sx = torch.full((n,), a) * (1 + torch.arange(n) % 2)     # (exact: whole and twice as much)
+            sw = torch.full((cout,), b) if b < 2.0 ** -126 else b * (1 + torch.rand(cout, generator=g) / 8)
+            y = int8_linear(q.to(dev), int8_weight(wq.to(dev), sw.to(dev)), scale=sx.to(dev))
+            want, size = reference(q, sx, wq.unsqueeze(0), sw.unsqueeze(0), None, torch.zeros(n, dtype=torch.long), torch.arange(n))
+            assert bool((want.abs().amax() < 2.0 ** 127))
+            close(y, want, size, F32)                             # (2^-126 covers what is below the normal range)
+        zero = torch.zeros(1, cin, dtype=I8)
+        big = int8_weight(wq.to(dev), torch.full((cout,), 3e38, device=dev))
+        assert bool((int8_linear(zero.to(dev), big, scale=torch.full((1,), 3e38, device=dev)) == 0).all())
+        ones = int8_weight(torch.ones(cin, cout, dtype=I8, device=dev), torch.full((cout,), 3e38, device=dev))
+        for sign in (1, -1):
+            y = int8_linear(torch.full((1, cin), sign, dtype=I8, device=dev), ones, scale=torch.full((1,), 3e38, device=dev))
+            assert bool((y == sign * float("inf")).all())
+
+
+def test_far_scales(oracle):
+    with _lib.use_library(oracle):
+        far_scales("cpu", [(3, 64, 5), (20, 33, 18)])
+
+
+@pytest.mark.gpu
+def test_hip_far_scales(hip):
+    far_scales("cuda", [(3, 64, 5), (20, 500, 70), (1700, 300, 130), (3000, 700, 70), (600, 4200, 130), (6500, 600, 300)])
