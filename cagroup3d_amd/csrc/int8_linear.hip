@@ -1021,16 +1021,17 @@ static i8_plan i8_choose(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows
     p.bytes = at;
     return p;
 }
-extern "C" int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts, int32_t grouped) {
+extern "C" int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts, int32_t flags) {
     if (dtype < CG3D_DT_F32 || dtype > CG3D_DT_I8 || i8_bad_shape(n_experts, cin, cout) || n_x < 0 || n_x > 0x7fffffffll || n_rows < 0 ||
-        n_rows > 0x7fffffffll || (grouped != 0 && grouped != 1))
+        n_rows > 0x7fffffffll || (flags & ~3))
         return CG3D_ERR_ARG;
-    return i8_choose(dtype, n_x, cin, n_rows, cout, n_experts, grouped, true).bytes;
+    return i8_choose(dtype, n_x, cin, n_rows, cout, n_experts, flags & 1, (cin & 15) || !(flags & 2)).bytes;
 }
 extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, int64_t n_x, int32_t cin, const int8_t *w, const float *sw,
                                 const float *bias, int32_t bias_per_expert, const int32_t *offsets, const int32_t *rows, void *y,
                                 int32_t out_dtype, int64_t n_rows, int32_t cout, int32_t n_experts, void *ws, cg3d_stream_t stream) {
-    const int64_t need = cg3d_int8_linear_ws_bytes(dtype, n_x, cin, n_rows, cout, n_experts, offsets != nullptr);
+    const bool padded = (cin & 15) || ((uintptr_t)x & 15);
+    const int64_t need = cg3d_int8_linear_ws_bytes(dtype, n_x, cin, n_rows, cout, n_experts, (offsets ? 1 : 0) | (padded ? 0 : 2));
     if (need < 0 || out_dtype < CG3D_DT_F32 || out_dtype > CG3D_DT_F16 || (bias_per_expert != 0 && bias_per_expert != 1)) return CG3D_ERR_ARG;
     if (offsets ? (!rows && n_x != n_rows) : (rows || n_x != n_rows || n_experts != 1)) return CG3D_ERR_ARG;
     if (n_rows == 0) return CG3D_OK;
@@ -1039,7 +1040,6 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
         (((uintptr_t)sx | (uintptr_t)sw | (uintptr_t)bias | (uintptr_t)offsets | (uintptr_t)rows) & 3) || ((uintptr_t)ws & 15))
         return CG3D_ERR_ARG;
     hipStream_t s = cg3d_hs(stream);
-    const bool padded = (cin & 15) || ((uintptr_t)x & 15);
     const i8_plan p = i8_choose(dtype, n_x, cin, n_rows, cout, n_experts, offsets != nullptr, padded);
     const int64_t panels = i8_panels(cout);
     if (p.tiles >= (1ll << 24) || (p.kind == i8_plan::TILE && p.tiles * p.ny >= (p.big ? 1ll << 23 : 1ll << 24))) return CG3D_ERR_ARG;      // (2^32 threads of a launch)

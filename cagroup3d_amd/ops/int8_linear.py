@@ -183,7 +183,7 @@ def _linear(x, weight, bias, scale, out_dtype, plan, gather):
     lib.check(x)
     code = DTYPES[dtype]
     with on_device(x):
-        ws_bytes = _ws_bytes(lib, code, n_x, cin, n_rows, cout, n_experts, int(plan is not None))
+        ws_bytes = _ws_bytes(lib, code, n_x, cin, n_rows, cout, n_experts, int(plan is not None) | (0 if x.data_ptr() & 15 else 2))
         y = torch.empty((n_rows, cout), dtype=out_dtype, device=dev)
         ws = torch.empty(ws_bytes, dtype=torch.int8, device=dev) if ws_bytes > 0 else None
         lib.call("cg3d_int8_linear", x.data_ptr(), code, ptr(scale), n_x, cin, weight.packed.data_ptr(), weight.scale.data_ptr(), ptr(bias), per_expert,

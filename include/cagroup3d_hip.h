@@ -622,7 +622,9 @@ int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, cons
  *     quantised by the same rule for each (expert, channel), scale [n_experts][cout] is written, ws = 4 * n_experts * cout bytes;
  *     CG3D_DT_I8: packed as they are, scale and ws are not used (the caller holds the scales).
  *   linear: x [n_x][cin] of `dtype`; CG3D_DT_I8: sx [n_x] given; floats: quantised in the call (sx NULL or ignored).  ws =
- *     cg3d_int8_linear_ws_bytes bytes, 16-byte aligned, may be NULL where that is 0 (grouped = 1 for a call with offsets).  bias: NULL, [cout], or [n_experts][cout] (bias_per_expert = 1).
+ *     cg3d_int8_linear_ws_bytes bytes, 16-byte aligned, may be NULL where that is 0; flags: 1 for a call with offsets, + 2 where the address of x is a
+ *     multiple of 16 (rows in 8 bits are then not copied; without it the size serves any address).  bias: NULL, [cout], or
+ *     [n_experts][cout] (bias_per_expert = 1).
  *     Dense: offsets = rows = NULL, n_experts = 1, n_x = n_rows.  Grouped: offsets [n_experts + 1] of cg3d_expert_plan; row r of y
  *     is the product of row rows[r] of x (rows NULL: row r, n_x = n_rows) with its expert's matrix; rows at and behind
  *     offsets[n_experts] are zeros.  y [n_rows][cout] of out_dtype.  n_rows < 2^30, fewer than 2^36 results. */
@@ -631,7 +633,7 @@ int cg3d_int8_weight(const void *w, int32_t dtype, int32_t n_experts, int32_t ci
                      cg3d_stream_t stream);
 int cg3d_int8_quantize_rows(const void *x, int32_t dtype, int64_t n, int32_t cin, int64_t pitch, int8_t *q, float *scale,
                             cg3d_stream_t stream);
-int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts, int32_t grouped);
+int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts, int32_t flags);
 int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, int64_t n_x, int32_t cin, const int8_t *w, const float *sw,
                      const float *bias, int32_t bias_per_expert, const int32_t *offsets, const int32_t *rows, void *y, int32_t out_dtype,
                      int64_t n_rows, int32_t cout, int32_t n_experts, void *ws, cg3d_stream_t stream);

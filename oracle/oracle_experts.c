@@ -206,9 +206,9 @@ int cg3d_int8_quantize_rows(const void *x, int32_t dtype, int64_t n, int32_t cin
     }
     return CG3D_OK;
 }
-int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts, int32_t grouped) {
+int64_t cg3d_int8_linear_ws_bytes(int32_t dtype, int64_t n_x, int32_t cin, int64_t n_rows, int32_t cout, int32_t n_experts, int32_t flags) {
     if (dtype < CG3D_DT_F32 || dtype > CG3D_DT_I8 || bad_shape(n_experts, cin, cout) || n_x < 0 || n_x > 0x7fffffffll || n_rows < 0 ||
-        n_rows > 0x7fffffffll || (grouped != 0 && grouped != 1))
+        n_rows > 0x7fffffffll || (flags & ~3))
         return CG3D_ERR_ARG;
     return dtype == CG3D_DT_I8 ? 0 : n_x * (4 + (int64_t)cin);
 }

@@ -699,3 +699,47 @@ def test_far_scales(oracle):
 @pytest.mark.gpu
 def test_hip_far_scales(hip):
     far_scales("cuda", [(3, 64, 5), (20, 500, 70), (1700, 300, 130), (3000, 700, 70), (600, 4200, 130), (6500, 600, 300)])
+
+
+@pytest.mark.parametrize("n,cin,cout", [(4000000, 1024, 64), (3000, 1024, 192), (4096, 4096, 4096), (512, 43904, 128), (5, 512, 64), (300000, 64, 64)])
+@pytest.mark.parametrize("grouped_call", [0, 1])
+def test_aligned_rows_in_8_bits_need_no_copy(n, cin, cout, grouped_call):
+    """Rows in 8 bits that the kernels read where they are ask for no memory to be copied to; other rows, and a query that does not say
+    how they are aligned, for theirs."""
+    ws = _lib.bind(_lib.HIP_LIB_PATH).raw("cg3d_int8_linear_ws_bytes")
+    copy = n * cin
+    for c, flags, copied in ((cin, grouped_call | 2, False), (cin, grouped_call, None), (cin + 1, grouped_call | 2, None)):
+        got = ws(3, n, c, n, cout, 1, flags)
+        parts = ws(3, n, cin, n, cout, 1, grouped_call | 2)       # (partial sums of a long contraction: less than the rows)
+        assert 0 <= got and (copied is None or got < copy) and got in (parts, parts + n * ((c + 63) // 64 * 64) + (4 * n + 255) // 256 * 256)
+    assert ws(3, n, cin, n, cout, 1, 4) == -1
+    for dtype in range(3):                                        # rows in floats: the same either way
+        assert ws(dtype, n, cin, n, cout, 1, grouped_call | 2) == ws(dtype, n, cin, n, cout, 1, grouped_call)
+
+
+@pytest.mark.gpu
+def test_hip_aligned_rows_in_8_bits_need_no_copy(hip):
+    """A product of rows that are aligned allocates its result and nothing of the rows' size; at an odd address it copies them, with
+    the same bits; the workspace of one does not serve the other."""
+    g = torch.Generator(device="cuda").manual_seed(110)
+    n, cin = 60000, 1024
+    store = torch.randint(-128, 127, (n * cin + 16,), generator=g, device="cuda", dtype=I8)
+    sx, w = torch.rand(n, generator=g, device="cuda") + 0.1, int8_weight(torch.randn(cin, 64, generator=g, device="cuda"))
+    x = store[:n * cin].view(n, cin)
+
+    def extra(rows):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        y = int8_linear(rows, w, scale=sx, out_dtype=BF16)
+        torch.cuda.synchronize()
+        return y, torch.cuda.max_memory_allocated() - before
+    int8_linear(x[:300], w, scale=sx[:300])
+    for _ in range(2):
+        y, more = extra(x)
+        assert more < 2 * 2 * n * 64
+        for off in (1, 4, 8, 15):
+            odd = store[off:off + n * cin].view(n, cin)
+            z, more = extra(odd)
+            assert more >= n * cin and torch.equal(z, int8_linear(odd.clone(), w, scale=sx, out_dtype=BF16))
+    assert torch.equal(y, int8_linear(x, w, scale=sx, out_dtype=BF16))
