@@ -794,10 +794,12 @@ __global__ __launch_bounds__(512, KEEP == 1 || (KEEP == 2 && !__is_same(T, float
 static __device__ __forceinline__ void i8_dma(const void *src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"((uint64_t)(uintptr_t)src), "s"(lds) : "memory");
 }
+template <int RG, int WR, int WC> static constexpr bool i8_in_parts = WR * RG * 16 == 128;      // (the larger tiles are for whole contractions)
 template <int RG, int WR, int WC>
 __global__ __launch_bounds__(WR * WC * 64, 2) void k_i8_tile(i8_args a, const int8_t *__restrict__ q, int64_t pitch, int32_t ny, i32x4 *__restrict__ part) {
     extern __shared__ __attribute__((aligned(16))) uint8_t i8_sm[];
     constexpr int NW = WR * WC, BM = WR * RG * 16, NA = WC * 4, NB = WR * RG, NL = (NA + NB) / NW, STAGE = (NA + NB) * 1024, NBUF = 4;
+    constexpr bool PARTS = i8_in_parts<RG, WR, WC>;
     static_assert((NA + NB) % NW == 0 && NA % NL == 0, "a wave's loads are of one operand");
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave % WR, wc = wave / WR;
@@ -810,7 +812,7 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void k_i8_tile(i8_args a, const in
     int64_t row0;
     if (!i8_tile<BM>(a, id / ny, e, row0, rows)) return;            // (the whole workgroup)
     const bool live = e < a.n_experts;
-    const int c_lo = (int)((int64_t)chunks * blockIdx.z / gridDim.z), nc = (int)((int64_t)chunks * (blockIdx.z + 1) / gridDim.z) - c_lo;
+    const int c_lo = PARTS ? (int)((int64_t)chunks * blockIdx.z / gridDim.z) : 0, nc = PARTS ? (int)((int64_t)chunks * (blockIdx.z + 1) / gridDim.z) - c_lo : chunks;
     i32x4 acc[RG][4];
 #pragma unroll
     for (int h = 0; h < RG; h++)
@@ -882,7 +884,7 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void k_i8_tile(i8_args a, const in
         }
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");          // (nothing may land in LDS after the workgroup has ended)
     }
-    if (gridDim.z > 1) {
+    if (PARTS && gridDim.z > 1) {
         i32x4 *to = part + ((((int64_t)blockIdx.z * total + id) * NW + wave) * (RG * 4)) * 64 + lane;
 #pragma unroll
         for (int h = 0; h < RG; h++)
@@ -1122,13 +1124,15 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
             return CG3D_ERR_LAUNCH;                                                                                                 \
         hipLaunchKernelGGL((k_i8_tile<RG, WR, WC>), dim3((unsigned)total, 1, (unsigned)p.splits), dim3(WR * WC * 64), lds, s, a, q, pitch, p.ny, part); \
         CG3D_CHECK_LAUNCH();                                                                                                        \
-        if (part) {                                                                                                                 \
-            hipLaunchKernelGGL((k_i8_join<RG, WR, WC>), dim3((unsigned)(total * (RG * WR * WC))), dim3(512), 0, s, a, p.ny, total, p.splits, part); \
-            CG3D_CHECK_LAUNCH();                                                                                                    \
-        }                                                                                                                           \
     } while (0)
     if (p.big) I8_T(8, 2, 4);
-    else I8_T(4, 2, 2);
+    else {
+        I8_T(4, 2, 2);
+        if (part) {
+            hipLaunchKernelGGL((k_i8_join<4, 2, 2>), dim3((unsigned)(total * 16)), dim3(512), 0, s, a, p.ny, total, p.splits, part);
+            CG3D_CHECK_LAUNCH();
+        }
+    }
 #undef I8_T
     return CG3D_OK;
 }

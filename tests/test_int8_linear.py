@@ -743,3 +743,12 @@ def test_hip_aligned_rows_in_8_bits_need_no_copy(hip):
             z, more = extra(odd)
             assert more >= n * cin and torch.equal(z, int8_linear(odd.clone(), w, scale=sx, out_dtype=BF16))
     assert torch.equal(y, int8_linear(x, w, scale=sx, out_dtype=BF16))
+
+
+def test_large_tiles_take_whole_contractions():
+    """Only the smaller tiles are used in parts (the larger ones have no code for it): partial sums ask for memory, whole contractions do not."""
+    ws = _lib.bind(_lib.HIP_LIB_PATH).raw("cg3d_int8_linear_ws_bytes")
+    for cin in (4096, 43904, 131056):
+        for n, cout in ((8192, 4096), (65536, 256), (16384, 1024)):
+            assert ws(3, n, cin, n, cout, 1, 2) == 0
+        assert ws(3, 512, cin, 512, 128, 1, 2) > 0
