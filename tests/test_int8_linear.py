@@ -751,4 +751,4 @@ def test_large_tiles_take_whole_contractions():
     for cin in (4096, 43904, 131056):
         for n, cout in ((8192, 4096), (65536, 256), (16384, 1024)):
             assert ws(3, n, cin, n, cout, 1, 2) == 0
-        assert ws(3, 512, cin, 512, 128, 1, 2) > 0
+    assert ws(3, 512, 43904, 512, 128, 1, 2) > 0                  # (shorter ones of so few rows go to the kernel for few rows)
