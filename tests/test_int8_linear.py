@@ -752,3 +752,42 @@ def test_large_tiles_take_whole_contractions():
         for n, cout in ((8192, 4096), (65536, 256), (16384, 1024)):
             assert ws(3, n, cin, n, cout, 1, 2) == 0
     assert ws(3, 512, 43904, 512, 128, 1, 2) > 0                  # (shorter ones of so few rows go to the kernel for few rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,cin,cout", [(36, 4160, 1 << 20), (36, 131056, 33000)])
+def test_hip_matrix_past_32_bits(hip, n, cin, cout):
+    """A matrix, and its packed form, of more than 2^32 bytes, for the larger and the smaller tiles: its first and last channels are those
+    of a small call."""
+    assert cin * cout > 2 ** 32
+    g = torch.Generator(device="cuda").manual_seed(120)
+    x = torch.randint(-128, 127, (n, cin), generator=g, device="cuda", dtype=I8)
+    sx, sw = torch.rand(n, generator=g, device="cuda") + 0.1, torch.rand(cout, generator=g, device="cuda") + 0.1
+    wq = torch.randint(-128, 127, (cin, cout), generator=g, device="cuda", dtype=I8)
+    y = int8_linear(x, int8_weight(wq, sw), scale=sx, out_dtype=F32)
+    for cols in (slice(0, 70), slice(cout // 2, cout // 2 + 70), slice(cout - 70, cout)):
+        assert torch.equal(y[:, cols], int8_linear(x, int8_weight(wq[:, cols].contiguous(), sw[cols].contiguous()), scale=sx))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,cin,cout,dtype", [(20, 2048, 2112, I8), (20, 2048, 2112, BF16), (300, 512, 8320, I8), (700, 2048, 2080, I8)])
+def test_hip_experts_past_32_bits(hip, t, cin, cout, dtype):
+    """The matrices of 1024 experts, of more than 2^32 bytes, for few rows, one pass and tiles: rows of the first, a middle and the last
+    expert are those of a product with its matrix alone."""
+    e = 1024
+    assert e * cin * cout > 2 ** 32
+    g = torch.Generator(device="cuda").manual_seed(121)
+    x = torch.randn(t, cin, generator=g, device="cuda").to(BF16)
+    ids = torch.randint(0, e, (t, 1), generator=g, device="cuda")
+    ids[::3], ids[1::7] = e - 1, 0
+    ids[2], ids[4] = 513, -1
+    wq = torch.randint(-128, 127, (e, cin, cout), generator=g, device="cuda", dtype=I8) if dtype == I8 else \
+        torch.randn(e, cin, cout, generator=g, device="cuda", dtype=BF16)
+    sw = torch.rand(e, cout, generator=g, device="cuda") + 0.1 if dtype == I8 else None
+    plan = expert_plan(ids, e)
+    y = int8_linear(x, int8_weight(wq, sw), plan=plan, gather=True, out_dtype=F32)
+    for i in (0, 513, e - 1):
+        at = plan.pos[:, 0][ids[:, 0] == i].long()
+        assert at.numel() > 0
+        assert torch.equal(y[at], int8_linear(x[ids[:, 0] == i], int8_weight(wq[i], None if sw is None else sw[i]), out_dtype=F32))
+    assert bool((y[int(plan.offsets[-1]):] == 0).all())
