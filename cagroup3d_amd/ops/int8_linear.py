@@ -7,6 +7,13 @@ its own for each expert's rows: the served form of the kernel-size-1 convolution
     y = int8_linear(q, weight, bias, scale=scale, out_dtype=torch.bfloat16)
     y = int8_linear(x, weight, plan=plan, gather=True)      # each expert's tokens with its matrix (ops/expert_rows.expert_plan)
 
+Results are rounded to the rows' own type unless out_dtype says otherwise.  Rows of 16 bits that are to be combined are therefore rounded
+twice, before and after the weighted sum (bf16: results 0.0023 off instead of 0.0016, in the 2-norm), for half the memory traffic between
+the two; rounded once:
+
+    y = int8_linear(x, weight, plan=plan, gather=True, out_dtype=torch.float32)
+    out = expert_combine(y, plan, gate, out_dtype=x.dtype)
+
 The integer sums are exact, so results do not depend on how the work is split.  There is no gradient: a call on inputs that require
 one, with gradients enabled, or that carry a tangent is refused.  torch.jit.trace records the calls; weights are laid out and plans
 made outside of it."""

@@ -791,3 +791,38 @@ def test_hip_experts_past_32_bits(hip, t, cin, cout, dtype):
         assert at.numel() > 0
         assert torch.equal(y[at], int8_linear(x[ids[:, 0] == i], int8_weight(wq[i], None if sw is None else sw[i]), out_dtype=F32))
     assert bool((y[int(plan.offsets[-1]):] == 0).all())
+
+
+def layer_rounds_once(dev):
+    """A layer of experts on 16-bit rows whose results stay in fp32 until they are combined is off by one rounding to the type; with the
+    default types by two."""
+    t, k, e, cin, cout = 200, 2, 5, 64, 40
+    ids, gate = ids_of(t, k, e, "dropped", 130), torch.rand(t, k, generator=torch.Generator().manual_seed(131))
+    for dtype in (BF16, F16):
+        x, _, w, b = make(t, cin, cout, dtype, 132, e)
+        wq, sw = plain_levels(w.transpose(1, 2).reshape(-1, cin))
+        plan = expert_plan(ids.to(dev), e)
+        rows, off, pos = plan.rows.cpu().long(), plan.offsets.cpu().long(), plan.pos.cpu().long()
+        expert = torch.bucketize(torch.arange(t * k), off[1:], right=True)
+        expert[expert == e] = -1
+        y, size = reference(x, None, wq.view(e, cout, cin).transpose(1, 2), sw.view(e, cout), b, expert, rows.clamp(min=0))
+        terms = torch.where((pos >= 0).unsqueeze(2), y[pos.clamp(min=0)] * gate.double().unsqueeze(2), 0.0)
+        sizes = torch.where((pos >= 0).unsqueeze(2), size[pos.clamp(min=0)] * gate.double().unsqueeze(2), 0.0).sum(1)
+        want, fp32 = terms.sum(1), (6 + k + 2) * 2.0 ** -24 * sizes     # the product's 6 half-steps and the sum's
+        weight = int8_weight(w.to(dev))
+        once = expert_combine(int8_linear(x.to(dev), weight, b.to(dev), plan=plan, gather=True, out_dtype=F32), plan, gate.to(dev), dtype)
+        twice = expert_combine(int8_linear(x.to(dev), weight, b.to(dev), plan=plan, gather=True), plan, gate.to(dev))
+        assert once.dtype == twice.dtype == dtype
+        for got, before in ((once, 0.0), (twice, HALF[dtype] * terms.abs().sum(1))):
+            off_by = (got.cpu().double() - want).abs()
+            assert bool((off_by <= HALF[dtype] * want.abs() * (1 + 2.0 ** -7) + (before + fp32) * (1 + 2.0 ** -7) + 2 * TINY[dtype] * k).all())
+
+
+def test_layer_of_experts_rounds_once(oracle):
+    with _lib.use_library(oracle):
+        layer_rounds_once("cpu")
+
+
+@pytest.mark.gpu
+def test_hip_layer_of_experts_rounds_once(hip):
+    layer_rounds_once("cuda")
