@@ -57,12 +57,7 @@ def recorded():
 
 def whole(t):
     """t contiguous, its memory holding its values (that of a lazily negated view holds the opposite ones)."""
-    return (t.resolve_neg() if t.is_neg() else t).contiguous()
-
-
-def held(*things):
-    """What a launch has the addresses of is used once more behind it: torch.compile, which stops at an address and resumes with what
-    the rest of the function uses, would free workspaces and copies of inputs before the launch."""
+    return t.resolve_neg().contiguous() if t.is_neg() else t if t.is_contiguous() else t.contiguous()
 
 
 class ExpertPlan:
@@ -126,7 +121,9 @@ def expert_plan(experts, n_experts):
         rows = plan.address(ROWS)
         lib.call("cg3d_expert_plan", ids.data_ptr(), int(ids.dtype == torch.int64), t, k, n_experts, plan.address(OFFSETS), rows,
                  plan.address(PAIRS), plan.address(POS), rows - 4 * at if at else None, lib.stream())
-    held(ids)
+    # (named behind the launch, here and in the passes: torch.compile stops at an address and resumes with what the rest of the function
+    # names, so that it would free copies of inputs before the launch)
+    del ids
     return plan
 
 
@@ -146,11 +143,12 @@ def _gather(x, plan):
     x = whole(x)
     lib.check(x)
     with on_device(x):
-        c = int(x.shape[1])                                     # (in a trace sizes are tensors)
+        c = x.shape[1]
+        c = c if type(c) is int else int(c)                     # (in a trace)
         out = torch.empty((plan.n_rows, c), dtype=x.dtype, device=x.device)
         lib.call("cg3d_expert_gather", x.data_ptr(), DTYPES[x.dtype], plan.address(ROWS), plan.n_tokens, plan.k, c, out.data_ptr(),
                  lib.stream())
-    held(x, plan)
+    del x, plan
     return out
 
 
@@ -175,11 +173,12 @@ def _combine(y, plan, w, out_dtype, tables=None):
     lib = _lib.get()
     lib.check(y, w)
     with on_device(y):
-        c = int(y.shape[1])
+        c = y.shape[1]
+        c = c if type(c) is int else int(c)
         out = torch.empty((plan.n_tokens, c), dtype=out_dtype, device=y.device)
         lib.call("cg3d_expert_combine", y.data_ptr(), DTYPES[y.dtype], plan.address(POS, tables), ptr(w), 0 if w is None else DTYPES[w.dtype],
                  plan.n_tokens, plan.k, c, out.data_ptr(), DTYPES[out_dtype], lib.stream())
-    held(y, w, plan, tables)
+    del y, w, plan, tables
     return out
 
 
@@ -236,13 +235,12 @@ class _Combine(torch.autograd.Function):
             dw = torch.empty_like(w) if ctx.needs_input_grad[2] else None
             lib.call("cg3d_expert_combine_bwd", dout.data_ptr(), ptr(y), DTYPES[dout.dtype], plan.address(PAIRS, tables), ptr(w),
                      0 if w is None else DTYPES[w.dtype], plan.n_tokens, plan.k, c, ptr(dy), ptr(dw), lib.stream())
-        held(dout, y, w, plan, tables)
         return dy, None, None if dw is None else dw.view(ctx.w_shape), None
 
 
 def expert_gather(x, plan):
     """x [T, C] float32 / bfloat16 / float16 -> [T * k, C], the tokens' rows in the plan's order (differentiable in x)."""
-    if recorded() or (torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad):
+    if recorded() or (torch.is_grad_enabled() and getattr(x, "requires_grad", False)):
         return _Gather.apply(x, plan)
     return _gather(x, plan)
 
@@ -251,7 +249,7 @@ def expert_combine(rows, plan, weights=None, out_dtype=None):
     """rows [T * k, C] in the plan's order -> [T, C]: out[t] = sum_s weights[t, s] * rows[pos[t, s]] over the slots that have a
     row, summed in float32 in slot order and rounded once, to out_dtype (default: the rows' own; float32 rows: any of the three)
     -- differentiable in rows and weights.  weights [T, k] float32 / bfloat16 / float16; None: all ones."""
-    if recorded() or (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (rows, weights))):
+    if recorded() or (torch.is_grad_enabled() and (getattr(rows, "requires_grad", False) or getattr(weights, "requires_grad", False))):
         return _Combine.apply(rows, plan, weights, out_dtype)
     rows, weights, out_dtype = _combine_inputs(rows, plan, weights, out_dtype)
     return _combine(rows, plan, weights, out_dtype)

@@ -24,24 +24,28 @@ from torch.autograd import forward_ad
 
 from .. import _lib
 from .._lib import CG3DError, ptr
-from .expert_rows import DTYPES, FLOATS, OFFSETS, ROWS, ExpertPlan, held, need, on_device, recorded, whole
+from .expert_rows import DTYPES, FLOATS, OFFSETS, ROWS, ExpertPlan, need, on_device, recorded, whole
 
 ROWS_IN = tuple(DTYPES)
 MAX_CIN = 131071                  # the int32 sum of so many products of 8-bit values cannot overflow
 
 
+def _no_grad_for(who, wanted):
+    if wanted and torch.is_grad_enabled():
+        raise CG3DError("%s has no gradient: call it under torch.no_grad() or on detached tensors" % who)
+
+
 def _no_tangent_for(who, *tensors):
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if isinstance(t, torch.Tensor) and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
-                raise CG3DError("%s has no forward-mode derivative" % who)
-
-
-def _no_grad_for(who, *tensors):
     for t in tensors:
-        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
-            raise CG3DError("%s has no gradient: call it under torch.no_grad() or on detached tensors" % who)
+        if forward_ad._current_level >= 0 and isinstance(t, torch.Tensor) and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+            raise CG3DError("%s has no forward-mode derivative" % who)
+
+
+def _record(who, f, args, tensors):
+    tensors = [t for t in tensors if isinstance(t, torch.Tensor)]
+    _no_grad_for(who, any(t.requires_grad for t in tensors))
     _no_tangent_for(who, *tensors)
+    return _Recorded.apply(f, *args)
 
 
 class _Recorded(torch.autograd.Function):
@@ -95,7 +99,7 @@ def int8_weight(w, scale=None):
             out, ws = scale.detach().resolve_neg().clone(memory_format=torch.contiguous_format).view(e, cout), None      # (the handle's own: the caller may reuse the memory)
         lib.call("cg3d_int8_weight", ptr(w), DTYPES[w.dtype], e, cin, cout, ptr(packed),
                  ptr(out) if ws is not None else None, ptr(ws), lib.stream())
-    held(w, ws)
+    del w, ws                                                     # (held until the launch has been made, under torch.compile too)
     return Int8Weight(packed, out, e, cin, cout, grouped)
 
 
@@ -114,22 +118,24 @@ def quantize_rows(x):
     """x [rows, cin] float32 / bfloat16 / float16 -> (q int8 [rows, cin], scale float32 [rows]): scale = max |x| / 127 of each row,
     q = the nearest level, ties to the even one.  A row of zeros has the scale 0, one with an infinity or a NaN the scale NaN;
     the scale of a row whose largest magnitude is below 1.5e-36 is subnormal and has fewer bits."""
-    _no_grad_for("quantize_rows", x)
-    return _Recorded.apply(_quantize, x) if recorded() else _quantize(x)
+    return _record("quantize_rows", _quantize, (x,), (x,)) if recorded() else _quantize(x)
 
 
 def _quantize(x):
     _rows_in("quantize_rows", x, FLOATS)
+    _no_grad_for("quantize_rows", x.requires_grad)
     lib = _lib.get()
     x = whole(x.detach())
     lib.check(x)
-    n, cin = (int(i) for i in x.shape)                            # (in a trace sizes are tensors)
+    n, cin = x.shape
+    if type(cin) is not int:                                      # (in a trace)
+        n, cin = int(n), int(cin)
     with on_device(x):
         q = torch.empty((n, cin), dtype=torch.int8, device=x.device)
         scale = torch.empty(n, dtype=torch.float32, device=x.device)
         lib.call("cg3d_int8_quantize_rows", ptr(x), DTYPES[x.dtype], n, cin, cin, ptr(q), ptr(scale),
                  lib.stream())
-    held(x)
+    del x                                                         # (held until the launch has been made, under torch.compile too)
     return q, scale
 
 
@@ -140,9 +146,9 @@ def int8_linear(x, weight, bias=None, scale=None, out_dtype=None, plan=None, gat
     plan (ops/expert_rows.expert_plan): weight holds plan.n_experts matrices and each row is multiplied by its expert's; x has the
     plan's rows ([T * k, cin], what expert_gather gives), or with gather=True the tokens ([T, cin]), whose rows are picked in the
     product.  Rows behind the last are zeros."""
-    _no_grad_for("int8_linear", x, bias, scale)
-    args = x, weight, bias, scale, out_dtype, plan, gather
-    return _Recorded.apply(_linear, *args) if recorded() else _linear(*args)
+    if recorded():
+        return _record("int8_linear", _linear, (x, weight, bias, scale, out_dtype, plan, gather), (x, bias, scale))
+    return _linear(x, weight, bias, scale, out_dtype, plan, gather)
 
 
 def _linear(x, weight, bias, scale, out_dtype, plan, gather):
@@ -151,7 +157,8 @@ def _linear(x, weight, bias, scale, out_dtype, plan, gather):
         raise CG3DError("int8_linear: weight must come from int8_weight")
     _rows_in("int8_linear", x, ROWS_IN)
     n_x, cin = x.shape
-    n_x, cin = int(n_x), int(cin)                                 # (in a trace sizes are tensors)
+    if type(cin) is not int:                                      # (in a trace)
+        n_x, cin = int(n_x), int(cin)
     dtype, dev, cout, n_experts = x.dtype, x.device, weight.cout, weight.n_experts
     if cin != weight.cin:
         raise CG3DError("int8_linear: x has %d columns, weight %d rows" % (cin, weight.cin))
@@ -183,17 +190,20 @@ def _linear(x, weight, bias, scale, out_dtype, plan, gather):
             bias.shape == (cout,) or (weight.grouped and bias.shape == (n_experts, cout))),
             "int8_linear: bias must be floats [%d] (or [%d, %d] with a matrix for each expert) on %s", cout, n_experts, cout, dev)
         per_expert = int(bias.dim() == 2)
+    _no_grad_for("int8_linear", x.requires_grad or (bias is not None and bias.requires_grad) or (scale is not None and scale.requires_grad))
     if bias is not None and not (bias.dtype is torch.float32 and bias.is_contiguous() and not bias.is_neg()):
         bias = whole(bias.detach().to(torch.float32))
     lib = _lib.get()
     x = whole(x)
     lib.check(x)
-    code = DTYPES[dtype]
+    code, at = DTYPES[dtype], x.data_ptr()
     with on_device(x):
-        ws_bytes = _ws_bytes(lib, code, n_x, cin, n_rows, cout, n_experts, int(plan is not None) | (0 if x.data_ptr() & 15 else 2))
+        ws_bytes = _ws_bytes(lib, code, n_x, cin, n_rows, cout, n_experts, int(plan is not None) | (0 if at & 15 else 2))
         y = torch.empty((n_rows, cout), dtype=out_dtype, device=dev)
         ws = torch.empty(ws_bytes, dtype=torch.int8, device=dev) if ws_bytes > 0 else None
-        lib.call("cg3d_int8_linear", x.data_ptr(), code, ptr(scale), n_x, cin, weight.packed.data_ptr(), weight.scale.data_ptr(), ptr(bias), per_expert,
+        lib.call("cg3d_int8_linear", at, code, ptr(scale), n_x, cin, weight.packed.data_ptr(), weight.scale.data_ptr(), ptr(bias), per_expert,
                  offsets, rows, y.data_ptr(), DTYPES[out_dtype], n_rows, cout, n_experts, ptr(ws), lib.stream())
-    held(x, scale, weight, bias, plan, ws)
+    # (named behind the launch: torch.compile stops at an address and resumes with what the rest of the function names, so that it would
+    # free workspaces and copies of inputs before the launch)
+    del x, scale, weight, bias, plan, ws
     return y
