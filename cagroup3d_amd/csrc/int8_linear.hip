@@ -1087,11 +1087,13 @@ extern "C" int cg3d_int8_linear(const void *x, int32_t dtype, const float *sx, i
         int64_t whole = 0, parts = cg3d_divup(384, p.tiles);
         parts = parts < panels ? parts : panels;
         const int32_t each = (int32_t)cg3d_divup(panels, parts);
-        // and those of the last few tiles behind whole rounds of the chip (four workgroups a CU), four panels or more to a part: 512 -> 512,
-        // 73 728 rows (128 tiles of 1152) 49.0 -> 44.9 us, 82 107 rows (259 of 1283) 52.3 -> 50.9; 256 -> 2048, 82 107 rows 118.9 -> 105.4; with
-        // 512 tiles left it loses (98 304 rows 55.4 -> 58.3)
-        const int64_t late = p.tiles % 1024;
-        if (p.tiles > 1024 && late > 0 && late <= 384 && panels >= 8) {
+        // and those of the last few tiles behind whole rounds of the chip -- four workgroups a CU, or the three that the levels of more than
+        // 576 columns leave room for --, four panels or more to a part: 512 -> 512, 73 728 rows (128 tiles of 1152) 49.0 -> 44.9 us, 82 107
+        // rows (259 of 1283) 52.3 -> 50.9; 256 -> 2048, 82 107 rows 118.9 -> 105.4; with 512 tiles left it loses (98 304 rows 55.4 -> 58.3).
+        // Rounds of three: 704 -> 1024, 51 712 rows (40 tiles of 808) 91.7 -> 72.8, 64 512 rows (240 of 1008) 97.1 -> 93.6; 832 -> 512, 58 752
+        // rows (150 of 918) 67.7 -> 66.5; with 300 left 704 -> 1024 102.1 -> 106.6
+        const int64_t round = i8_chunks(cin) <= 9 ? 1024 : 768, late = p.tiles % round;
+        if (p.tiles > round && late > 0 && late <= (round == 1024 ? 384 : 240) && panels >= 8) {
             whole = p.tiles - late;
             parts = cg3d_divup(768, late);
             parts = parts < panels / 4 ? parts : panels / 4;

@@ -826,3 +826,11 @@ def test_layer_of_experts_rounds_once(oracle):
 @pytest.mark.gpu
 def test_hip_layer_of_experts_rounds_once(hip):
     layer_rounds_once("cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,cin,cout,dtype", [(64 * (768 + 40) + 5, 600, 520, BF16), (64 * (768 + 239) + 1, 832, 530, F16), (64 * (768 + 300), 700, 520, BF16),
+                                              (64 * (1024 + 30) + 63, 500, 520, I8)])
+def test_hip_last_tiles_behind_whole_rounds(hip, n, cin, cout, dtype):
+    """Tiles whose panels are shared out, behind whole rounds of three and of four workgroups a CU."""
+    dense(n, cin, cout, dtype, F32 if dtype == I8 else dtype, True, 140, "cuda")
