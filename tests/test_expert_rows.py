@@ -599,3 +599,60 @@ def test_negated_views(oracle):
 @pytest.mark.gpu
 def test_hip_negated_views(hip):
     negated_views("cuda")
+
+
+def weights_of_one_slot(dev):
+    """Weights [T] of a plan of one slot: their gradient has their shape."""
+    plan = expert_plan(torch.tensor([1, 0, 1, -1]).to(dev), 2)
+    y = torch.arange(8.0).view(4, 2).to(dev).requires_grad_()
+    for w in (torch.tensor([1.0, 10.0, 100.0, 1000.0]).to(dev), torch.tensor([[1.0], [10.0], [100.0], [1000.0]]).to(dev)):
+        w.requires_grad_()
+        out = expert_combine(y, plan, w)
+        dy, dw = torch.autograd.grad(out.sum(), [y, w])
+        assert out.tolist() == [[2.0, 3.0], [0.0, 10.0], [400.0, 500.0], [0.0, 0.0]]
+        assert dw.shape == w.shape and dw.view(-1).tolist() == [5.0, 1.0, 9.0, 0.0]
+        assert dy.tolist() == [[10.0, 10.0], [1.0, 1.0], [100.0, 100.0], [0.0, 0.0]]
+
+
+def test_weights_of_one_slot(oracle):
+    with _lib.use_library(oracle):
+        weights_of_one_slot("cpu")
+
+
+@pytest.mark.gpu
+def test_hip_weights_of_one_slot(hip):
+    weights_of_one_slot("cuda")
+
+
+@pytest.mark.gpu
+def test_hip_training_pass_in_a_graph(hip):
+    """Plan, both passes and all gradients captured once and replayed with other ids and rows, eager passes in between."""
+    t, k, e, c = 3000, 2, 18, 40
+    g = torch.Generator().manual_seed(95)
+
+    def inputs(seed):
+        ids = routing(t, k, e, "dropped", seed).cuda()
+        return [ids] + [torch.randn(*s, generator=g).cuda() for s in ((t, c), (t * k, c), (t, k), (t * k, c), (t, c))]
+
+    def step(ids, x, y, w, dr, do):
+        plan = expert_plan(ids, e)
+        x, y, w = (v.detach().requires_grad_() for v in (x, y, w))
+        outs = expert_gather(x, plan), expert_combine(y, plan, w)
+        return [o.detach() for o in outs] + list(torch.autograd.grad(outs, [x, y, w], [dr, do]))
+    static = inputs(96)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(*static)
+    for seed in (97, 98, 99):
+        new = inputs(seed)
+        for a, b in zip(static, new):
+            a.copy_(b)
+        graph.replay()
+        want = step(*new)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
