@@ -186,7 +186,7 @@ static __device__ __forceinline__ i8_lev<T> i8_levels(const i8_level &lev, bool 
 
 // ---------------------------------------------------------------- weights (once per model)
 // w [E][cin][cout]: a thread of 16 to a channel, reads along the contraction are rows of the matrix (18 x 1024 x 1024 fp32: 13 us,
-// 5.7 TB/s; the packing 27 us)
+// 5.7 TB/s; the packing 27 us = 3.5 TB/s: a lane's channels are 4 apart, so that four waves read each line.  Once for a model)
 template <typename T>
 __global__ __launch_bounds__(1024) void k_i8_weight_scale(const T *__restrict__ w, int32_t cin, int32_t cout, float *__restrict__ scale,
                                                           uint32_t *__restrict__ top) {
@@ -556,9 +556,10 @@ static __device__ __forceinline__ int i8_place(int r, int p) { return r * 64 + (
 // (wm, wn) multiplies RG of the 4 row groups by panels wn, wn + RG, ... of its part of the channels, the weights streaming past from the
 // caches, every fragment used RG times.  RG = 4 / 2 / 1 for at least 4 / 2 / 1 panels a part.  The first `whole` tiles are one workgroup
 // each, the panels of every other are shared out to `parts`.
-// Bound by memory where panels are few (155 773 x 64 fp32 -> 64: 14.7 us = 5.4 TB/s, a copy's rate); with many, by what a workgroup does one
-// after the other -- rows in, products, results out -- which the three others of its CU overlap only in part: 82 107 x 512 bf16 -> 512
-// 48 us = 3.5 TB/s and 0.9 POP/s (31 us to read and write, 18 us to multiply), 131 072 rows 3.9 TB/s.
+// Bound by memory where panels are few: 155 773 x 64 fp32 -> 64, 80 MB, 15.3 us among others where the 256 MB memory-side cache still has
+// the rows, 19.2 us = 4.2 TB/s with 600 MB of rows in turn.  With many panels by what a workgroup does one after the other -- rows in,
+// products, results out --, which the three others of its CU overlap only in part: 82 107 x 512 bf16 -> 512 46 - 52 us, 54.6 from memory
+// = 3.1 TB/s and 0.8 POP/s (31 us to read and write, 18 us to multiply).  The library's bf16 product of these sizes: 20.0 and 63.8 us.
 template <typename T, int RG, int KEEP>                  // KEEP: chunks of a row held in registers; longer rows are read again, from the caches
 __global__ __launch_bounds__(256, RG == 4 || KEEP * sizeof(T) > 8 ? 4 : RG == 2 ? 5 : 6) void k_i8_fused(i8_args a, const T *__restrict__ x, int32_t whole, int32_t parts) {
     extern __shared__ __attribute__((aligned(16))) uint8_t i8_sm[];
@@ -689,8 +690,9 @@ __global__ __launch_bounds__(256, RG == 4 || KEEP * sizeof(T) > 8 ? 4 : RG == 2 
 // floats that fit (CHUNKS chunks of a wave) are quantised here, in the operand's own layout -- each workgroup finds the rows' maxima for
 // itself, through LDS; the waves' sums are joined there too.  grid: (16-row tiles, pairs of tiles).  KEEP: chunks of a wave held at once;
 // registers for no more than there are let up to three workgroups onto a CU (8 experts of 640 -> 256, 1000 rows: 24.4 us with 8, 10.9 with 2).
-// Bound by the weights' way from memory, and for small ones by a launch and two trips to memory: 1 x 4096 bf16 -> 4096 8.5 us = 2.0 TB/s
-// of weights, 1003 x 200 fp16 -> 77 5.3 us, 8 rows of 64 experts 512 -> 512 4.8 us.
+// Bound by the weights' way from memory: 1 x 4096 bf16 -> 4096 8.2 us = 2.0 TB/s of weights that the memory-side cache holds, 9.5 us from
+// memory (the library in bf16: 17.1) -- its 128 workgroups are on half of the CUs, and the other half reads nothing.  Small ones by a
+// launch and two trips to memory: 1003 x 200 fp16 -> 77 5.5 us, 8 rows of 64 experts 512 -> 512 4.8 us.
 template <typename T> struct i8_few { static constexpr int CHUNKS = sizeof(T) == 4 ? 4 : 8; };
 template <typename T, int KEEP>
 __global__ __launch_bounds__(512, KEEP == 1 || (KEEP == 2 && !__is_same(T, float) && !__is_same(T, i8_f16)) ? 6 : KEEP * sizeof(T) <= 8 ? 4 : 2) void k_i8_few(i8_args a, const T *__restrict__ x, int64_t pitch) {
