@@ -471,8 +471,9 @@ static __device__ __forceinline__ bool i8_is_far(float sx) {
     const float size = fabsf(sx);
     return size >= 0x1p96f || (size > 0.f && size < 0x1p-126f);
 }
-// a lane's N sums of one row, scaled, as many of them as there are channels left (n); live = 0: a row behind the last; far: one of the
-// wave's rows may be (the same for all lanes).  to: where the workgroup's first lane would store (the same for all lanes), at: this lane's elements behind it
+// a lane's N sums of one row, scaled, as many of them as there are channels left (n); far: one of the wave's rows may be (the same for
+// all lanes); live = 0: a row behind the last.  to: where the workgroup's first lane would store (the same for all lanes), at: this lane's
+// elements behind it
 template <int N>
 static __device__ __forceinline__ void i8_store(const i8_args &a, int64_t to, uint32_t at, int n, float sx, bool far, bool live, const i8_chan<N> &ch,
                                                 const int (&sum)[N]) {
@@ -520,8 +521,8 @@ static __device__ __forceinline__ void i8_store(const i8_args &a, int64_t to, ui
     }
 }
 // a wave's results of 16 rows x one panel: acc[nb][i] of lane (g, m) is row 4 g + i, channel 4 m + nb; sx: of the lane's four rows
-static __device__ __forceinline__ void i8_store_panel(const i8_args &a, int e, int panel, int64_t row0, int rows, const float (&sx)[4], bool far, bool live,
-                                                      const i32x4 (&acc)[4]) {
+static __device__ __forceinline__ void i8_store_panel(const i8_args &a, int e, int panel, int64_t row0, int rows, const float (&sx)[4], bool far,
+                                                      bool live, const i32x4 (&acc)[4]) {
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, c0 = panel * 64 + m * 4, n = a.cout - c0;
     if (n <= 0) return;
     const i8_chan<4> ch(a, live ? e : 0, c0);

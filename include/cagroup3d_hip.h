@@ -617,14 +617,15 @@ int cg3d_expert_combine_bwd(const void *dout, const void *y, int32_t dtype, cons
  *   y[r, n] = (sum_k q[r, k] * w[k, n]) * sx[r] * sw[n] + bias[n]; the sum is exact (int32, cin <= 131071), and no step on the way
  *     leaves fp32's range where the scaled sum does not, for any scales.
  *   quantize_rows: scale[r] = max_k |x[r, k]| / 127, q = 127 x / max rounded to the nearest level, ties to even, decided exactly;
- *     a row with an infinity or NaN: scale NaN, q 0; the scale of a row below 1.5e-36 is subnormal and has fewer bits; q [n][pitch], bytes [cin, pitch) zeros.
+ *     a row with an infinity or NaN: scale NaN, q 0; the scale of a row below 1.5e-36 is subnormal and has fewer bits; q [n][pitch], bytes
+ *     [cin, pitch) zeros.
  *   weight: w [n_experts][cin][cout] -> packed (cg3d_int8_weight_bytes bytes, 16-byte aligned; the kernels' own order).  Floats:
  *     quantised by the same rule for each (expert, channel), scale [n_experts][cout] is written, ws = 4 * n_experts * cout bytes;
  *     CG3D_DT_I8: packed as they are, scale and ws are not used (the caller holds the scales).
  *   linear: x [n_x][cin] of `dtype`; CG3D_DT_I8: sx [n_x] given; floats: quantised in the call (sx NULL or ignored).  ws =
- *     cg3d_int8_linear_ws_bytes bytes, 16-byte aligned, may be NULL where that is 0; flags: 1 for a call with offsets, + 2 where the address of x is a
- *     multiple of 16 (rows in 8 bits are then not copied; without it the size serves any address).  bias: NULL, [cout], or
- *     [n_experts][cout] (bias_per_expert = 1).
+ *     cg3d_int8_linear_ws_bytes bytes, 16-byte aligned, may be NULL where that is 0; flags: 1 for a call with offsets, + 2
+ *     where the address of x is a multiple of 16 (rows in 8 bits are then not copied; without it the size serves any address).
+ *     bias: NULL, [cout], or [n_experts][cout] (bias_per_expert = 1).
  *     Dense: offsets = rows = NULL, n_experts = 1, n_x = n_rows.  Grouped: offsets [n_experts + 1] of cg3d_expert_plan; row r of y
  *     is the product of row rows[r] of x (rows NULL: row r, n_x = n_rows) with its expert's matrix; rows at and behind
  *     offsets[n_experts] are zeros.  y [n_rows][cout] of out_dtype.  n_rows < 2^30, fewer than 2^36 results. */
